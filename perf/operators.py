@@ -1,0 +1,500 @@
+"""The operators of a training step beside the losses, and how they are measured:
+attention with a learned relative position bias (``fa.relative_attention``), that
+bias by itself (``fa.relative_bias``) and the orthogonalised update of a weight
+matrix (``fa.orthogonalize``).
+
+``listed()`` holds the fixed cases, ``draw(rng)`` gives further ones of the same
+ranges, ``prepare`` makes what a program has in hand before the call, ``run`` makes
+one call (with its backward pass where the case trains), and ``exact`` gives the
+same outputs in float64.  ``own`` chooses between the public functions of
+``frame_analytics_amd`` and their plain form in elementary float32 torch operations.
+
+A case is a dict.  ``op`` is "attention", "bias" or "orthogonalize".  Attention:
+``batch, heads, kv_heads, q_len, k_len, dim`` and element type ``dtype``; positions
+on a line (``grid_w`` 0; ``buckets, max_distance, bidirectional``) or in a window of
+``grid_h x grid_w`` tokens; ``causal``; ``windows`` > 0: a boolean mask that repeats
+over that many windows of a shifted frame; ``ragged``: each batch entry has keys of
+its own length, some none; ``train``: with gradients.  Bias: ``heads, q_len, k_len``
+and the positions.  Orthogonalize: ``batch`` matrices of ``rows x cols``, ``steps``.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+_DTYPES = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch.float32}
+_BYTES = {"float16": 2, "bfloat16": 2, "float32": 4}
+#: steep at zero, so that few steps lift small singular values (the default), and the
+#: polynomial of degree five that converges to the polar factor
+_STEEP = (3.4445, -4.7750, 2.0315)
+_POLAR = (1.875, -1.25, 0.375)
+
+
+def _attention(name, dtype, batch, heads, kv_heads, q_len, k_len, dim, *, grid=(0, 0), buckets=32,
+               max_distance=128, bidirectional=True, causal=False, windows=0, ragged=False,
+               train=True):
+    return {"name": name, "op": "attention", "dtype": dtype, "batch": batch, "heads": heads,
+            "kv_heads": kv_heads, "q_len": q_len, "k_len": k_len, "dim": dim,
+            "grid_h": grid[0], "grid_w": grid[1], "buckets": buckets,
+            "max_distance": max_distance, "bidirectional": bidirectional, "causal": causal,
+            "windows": windows, "ragged": ragged, "train": train}
+
+
+def _bias(name, dtype, heads, q_len, k_len, *, grid=(0, 0), buckets=32, max_distance=128,
+          bidirectional=True):
+    return {"name": name, "op": "bias", "dtype": dtype, "heads": heads, "q_len": q_len,
+            "k_len": k_len, "grid_h": grid[0], "grid_w": grid[1], "buckets": buckets,
+            "max_distance": max_distance, "bidirectional": bidirectional}
+
+
+def _orthogonalize(name, dtype, batch, rows, cols, steps=5, polar=False):
+    return {"name": name, "op": "orthogonalize", "dtype": dtype, "batch": batch, "rows": rows,
+            "cols": cols, "steps": steps, "polar": polar}
+
+
+def listed():
+    return [
+        # a restoration network's attention in shifted 8 x 8 windows over 16 training
+        # patches of 128 x 128: many windows, heads of a dimension that is no power of 2
+        _attention("windows_8x8_train", "bfloat16", 4096, 6, 6, 64, 64, 30, grid=(8, 8),
+                   windows=256),
+        # the same layer with 16 x 16 windows, unshifted
+        _attention("windows_16x16_train", "float16", 512, 8, 8, 256, 256, 32, grid=(16, 16)),
+        # a causal sequence of frame tokens in mixed-precision training
+        _attention("line_causal_train", "bfloat16", 2, 8, 8, 2048, 2048, 64, causal=True,
+                   bidirectional=False),
+        # full-precision training on a sequence of an odd length, shared key/value heads
+        _attention("line_f32_train", "float32", 2, 8, 2, 777, 777, 64),
+        # scoring long clips of different lengths in one batch
+        _attention("line_long_infer", "bfloat16", 4, 8, 8, 4096, 4096, 64, ragged=True,
+                   train=False),
+        # one new token for each of 16 clips against their cached keys and values
+        _attention("single_token_infer", "bfloat16", 16, 16, 4, 1, 4096, 128, ragged=True,
+                   bidirectional=False, train=False),
+        # the bias of a 16 x 16 window for an attention that takes it as a tensor: one
+        # short call each way, where latency counts
+        _bias("bias_window_16x16", "float32", 8, 256, 256, grid=(16, 16)),
+        # the bias of a long sequence, where the memory's rate counts
+        _bias("bias_line_long", "bfloat16", 16, 2048, 2048),
+        # updates of small projection matrices in full precision
+        _orthogonalize("update_small_f32", "float32", 6, 180, 180, steps=6, polar=True),
+        # updates of 3 x 3 convolutions (256 channels each way), flattened, full precision
+        _orthogonalize("update_conv_f32", "float32", 8, 256, 2304, steps=6, polar=True),
+        # updates of one layer's projections in bfloat16
+        _orthogonalize("update_blocks", "bfloat16", 8, 1024, 1024),
+        # the largest matrices
+        _orthogonalize("update_large", "bfloat16", 2, 4096, 4096),
+    ]
+
+
+def _log_uniform(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """One more case: any operator and form, sizes spread over the logarithm of their
+    ranges, odd ones as often as even ones."""
+    form = rng.choice(("windows", "line", "line", "long", "token", "bias", "bias", "update",
+                       "update", "update"))
+    narrow = rng.choice(("float16", "bfloat16"))
+    line = {"buckets": rng.choice((16, 32, 64)), "max_distance": rng.choice((64, 128, 512)),
+            "bidirectional": rng.random() < 0.5}
+    if form == "windows":
+        side = rng.choice((4, 7, 8, 12, 16))
+        length = side * side
+        windows = rng.choice((0, 16, 64))
+        heads, dim = rng.randint(2, 8), rng.choice((24, 30, 32, 64))
+        most = min(4096, (512 * 8 * 256 * 256 * 32) // (heads * length * length * dim))
+        batch = _log_uniform(rng, 64, max(65, most))
+        if windows:
+            batch = max(1, batch // windows) * windows
+        case = _attention("", rng.choice((narrow, "float32")), batch, heads, heads, length, length,
+                          dim, grid=(side, side), windows=windows)
+    elif form in ("line", "long"):
+        train = form == "line"
+        length = _log_uniform(rng, 60, 2048) if train else _log_uniform(rng, 500, 6000)
+        kv = rng.choice((1, 2, 4))
+        heads = kv * rng.choice((1, 2))
+        batch = max(1, min(_log_uniform(rng, 1, 64), 2 * 8 * 2048 * 2048 // (heads * length ** 2)))
+        dtype = rng.choice((narrow, "float32")) if train and length <= 1024 else narrow
+        case = _attention("", dtype, batch, heads, kv, length, length, rng.choice((40, 64, 96)),
+                          causal=train and not line["bidirectional"], ragged=not train,
+                          train=train, **line)
+    elif form == "token":
+        kv = rng.choice((1, 2, 4))
+        case = _attention("", narrow, _log_uniform(rng, 1, 32), kv * rng.choice((1, 4)), kv, 1,
+                          _log_uniform(rng, 100, 8192), rng.choice((64, 80, 128)),
+                          ragged=True, train=False, **{**line, "bidirectional": False})
+    elif form == "bias":
+        dtype, heads = rng.choice((narrow, "float32")), rng.randint(2, 16)
+        if rng.random() < 0.5:
+            gh, gw = rng.randint(4, 24), rng.randint(4, 24)
+            case = _bias("", dtype, heads, gh * gw, gh * gw, grid=(gh, gw))
+        else:
+            case = _bias("", dtype, heads, _log_uniform(rng, 60, 2048), _log_uniform(rng, 60, 2048),
+                         **line)
+    else:
+        full = rng.random() < 0.4
+        rows = _log_uniform(rng, 64, 800 if full else 2048)
+        cols = min(4 * 2048, max(64, int(rows * math.exp(rng.uniform(-1.4, 1.4)))))
+        least = min(rows, cols)
+        most = (2 if full else 8) * 2048 ** 3 // (4 * least * rows * cols)
+        case = _orthogonalize("", "float32" if full else narrow,
+                              max(1, min(_log_uniform(rng, 1, 24), most)), rows, cols,
+                              steps=6 if full else 5, polar=full)
+    del case["name"]
+    return case
+
+
+# --------------------------------------------------------------------------- #
+# inputs
+# --------------------------------------------------------------------------- #
+
+
+def _device():
+    return torch.device("cuda" if torch.cuda.is_available() else "cpu")
+
+
+def _table_rows(case):
+    if case["grid_w"]:
+        return (2 * case["grid_h"] - 1) * (2 * case["grid_w"] - 1)
+    return case["buckets"]
+
+
+def _shift_mask(case, dev):
+    """(windows, 1, L, L), True where attention is allowed: the windows of a frame that
+    was shifted by half a window, whose last row and column hold parts of the frame
+    that are not neighbours."""
+    n, gh, gw = case["windows"], case["grid_h"], case["grid_w"]
+    across = max(d for d in range(1, int(math.isqrt(n)) + 1) if n % d == 0)
+    w = torch.arange(n, device=dev)
+    t = torch.arange(gh * gw, device=dev)
+    below = ((w // across) == n // across - 1)[:, None] & (t // gw >= gh - gh // 2)[None]
+    right = ((w % across) == across - 1)[:, None] & (t % gw >= gw - gw // 2)[None]
+    region = 2 * below.int() + right.int()
+    return (region[:, None, :, None] == region[:, None, None, :]).contiguous()
+
+
+def prepare(case, seed):
+    dev, dt = _device(), _DTYPES[case["dtype"]]
+    gen = torch.Generator(device=dev).manual_seed(int(seed))
+
+    def normal(*shape):
+        return torch.randn(*shape, device=dev, generator=gen)
+
+    if case["op"] == "orthogonalize":
+        # a gradient: a few strong directions over a floor of noise
+        b, m, n = case["batch"], case["rows"], case["cols"]
+        r = min(m, n)
+        s = 1.0 / (1.0 + torch.arange(r, device=dev)) ** 0.5
+        g = (normal(b, m, r) * s) @ normal(b, r, n) / math.sqrt(r) + 0.2 * normal(b, m, n)
+        return {"case": case, "update": (1e-3 * g).to(dt)}
+    table = (0.5 * normal(_table_rows(case), case["heads"])).to(dt)
+    if case["op"] == "bias":
+        up = normal(case["heads"], case["q_len"], case["k_len"]).to(dt)
+        return {"case": case, "table": table.requires_grad_(True), "up": up}
+    b, h, hk, d = case["batch"], case["heads"], case["kv_heads"], case["dim"]
+    # tokens first, as a projection leaves them: (batch, tokens, heads, dim), seen
+    # as (batch, heads, tokens, dim)
+    q = normal(b, case["q_len"], h, d).to(dt).transpose(1, 2)
+    k = normal(b, case["k_len"], hk, d).to(dt).transpose(1, 2)
+    v = normal(b, case["k_len"], hk, d).to(dt).transpose(1, 2)
+    state = {"case": case, "q": q, "k": k, "v": v, "table": table, "mask": None, "lengths": None,
+             "start": 0}
+    if case["windows"]:
+        state["mask"] = _shift_mask(case, dev)
+    if case["ragged"]:
+        lengths = torch.randint(case["k_len"] // 4, case["k_len"] + 1, (b,), device=dev,
+                                generator=gen)
+        lengths[0] = case["k_len"]
+        if b > 2:
+            lengths[-1] = 0  # a slot that holds no clip
+        state["lengths"] = lengths.to(torch.int32)
+        if case["q_len"] == 1:  # the new token stands after the cached ones
+            state["start"] = (lengths - 1).clamp_min(0).to(torch.int32)
+    if case["train"]:
+        state["up"] = normal(b, case["q_len"], h, d).to(dt).transpose(1, 2)
+        for x in (state["q"], state["k"], state["v"], table):
+            x.requires_grad_(True)
+    return state
+
+
+# --------------------------------------------------------------------------- #
+# one pass
+# --------------------------------------------------------------------------- #
+
+
+def _buckets(case, q_pos, k_len):
+    """The table row of each pair: ``q_pos`` (..., q_len) integers, the answer
+    (..., q_len, k_len)."""
+    dev = q_pos.device
+    if case["grid_w"]:
+        gh, gw = case["grid_h"], case["grid_w"]
+        k = torch.arange(k_len, device=dev)
+        dy = q_pos[..., :, None] // gw - k // gw
+        dx = q_pos[..., :, None] % gw - k % gw
+        return (dy + gh - 1) * (2 * gw - 1) + dx + gw - 1
+    rel = torch.arange(k_len, device=dev) - q_pos[..., :, None]
+    n = case["buckets"]
+    base = torch.zeros_like(rel)
+    if case["bidirectional"]:
+        n //= 2
+        base = n * (rel > 0)
+        dist = rel.abs()
+    else:
+        dist = (-rel).clamp_min(0)
+    exact_n = n // 2
+    # row exact_n + j starts at exact_n * (max_distance / exact_n) ** (j / (n - exact_n)),
+    # compared in whole numbers
+    starts, wide = [], n - exact_n
+    for j in range(1, wide):
+        at = exact_n
+        while at ** wide < exact_n ** (wide - j) * case["max_distance"] ** j:
+            at += 1
+        starts.append(at)
+    far = exact_n + torch.bucketize(dist, torch.tensor(starts, device=dev), right=True)
+    return base + torch.where(dist < exact_n, dist, far)
+
+
+def _plain_bias(case, table, q_pos):
+    """(1 or batch, heads, q_len, k_len) from the float32 table."""
+    lq, lk = case["q_len"], case["k_len"]
+    if case["grid_w"] or q_pos.shape[0] > 1:
+        return table[_buckets(case, q_pos, lk)].permute(0, 3, 1, 2)
+    # a line: one value for each distance, j - i from 1 - lq to lk - 1, picked from the
+    # table by a product; laid out again and again, one element further in each row
+    wide = lq + lk - 1
+    row = _buckets(case, torch.full((1,), lq - 1, device=table.device), wide)[0]
+    pick = (row[:, None] == torch.arange(table.shape[0], device=table.device)).float()
+    by_distance = (pick @ table).t()
+    laid = torch.nn.functional.pad(by_distance[:, None].expand(-1, lq, -1), (0, 1))
+    laid = laid.reshape(table.shape[1], -1)[:, :lq * wide].view(-1, lq, wide)
+    return laid[None, :, :, lq - 1:]
+
+
+def _plain_attention(state):
+    case, dt = state["case"], state["q"].dtype
+    q, k, v, table = (state[x].float() for x in ("q", "k", "v", "table"))
+    dev, lk, lq = q.device, case["k_len"], case["q_len"]
+    group = case["heads"] // case["kv_heads"]
+    if group > 1:
+        k, v = (x.repeat_interleave(group, dim=1) for x in (k, v))
+    start = torch.as_tensor(state["start"], device=dev).reshape(-1, 1)
+    q_pos = start + torch.arange(lq, device=dev)  # (1 or batch, q_len)
+    s = (q @ k.transpose(-1, -2)) / math.sqrt(case["dim"]) + _plain_bias(case, table, q_pos)
+    keys = torch.arange(lk, device=dev)
+    hidden = None
+    if case["causal"]:
+        hidden = (keys > q_pos[..., None])[:, None]
+    if state["mask"] is not None:
+        blocked = ~state["mask"].repeat(case["batch"] // case["windows"], 1, 1, 1)
+        hidden = blocked if hidden is None else hidden | blocked
+    if state["lengths"] is not None:
+        beyond = keys >= state["lengths"][:, None, None, None]
+        hidden = beyond if hidden is None else hidden | beyond
+    if hidden is not None:
+        s = s.masked_fill(hidden, float("-inf"))
+    top = s.detach().amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    total = p.sum(-1, keepdim=True)
+    out = (p @ v) / torch.where(total == 0, torch.ones_like(total), total)
+    return out.to(dt)
+
+
+def _positions(fa, case):
+    if case["grid_w"]:
+        return fa.GridPositions(case["grid_h"], case["grid_w"])
+    return fa.LinePositions(case["buckets"], case["max_distance"],
+                            bidirectional=case["bidirectional"])
+
+
+def run(state):
+    case = state["case"]
+    if own:
+        import frame_analytics_amd as fa
+    if case["op"] == "orthogonalize":
+        g, coefficients = state["update"], _POLAR if case["polar"] else _STEEP
+        if own:
+            return fa.orthogonalize(g, steps=case["steps"], coefficients=coefficients)
+        a, b, c = coefficients
+        x = g.float()
+        if case["rows"] > case["cols"]:
+            x = x.transpose(-1, -2)
+        x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + 1e-7)
+        for _ in range(case["steps"]):
+            gram = x @ x.transpose(-1, -2)
+            x = a * x + (b * gram + c * (gram @ gram)) @ x
+        if case["rows"] > case["cols"]:
+            x = x.transpose(-1, -2)
+        return x.to(g.dtype)
+    if case["op"] == "bias":
+        table = state["table"]
+        table.grad = None
+        if own:
+            bias = fa.relative_bias(table, _positions(fa, case), case["q_len"], case["k_len"])
+        else:
+            q_pos = torch.arange(case["q_len"], device=table.device)[None]
+            bias = _plain_bias(case, table.float(), q_pos)[0].to(table.dtype)
+        bias.backward(state["up"])
+        return bias.detach(), table.grad
+    q, k, v, table = (state[x] for x in ("q", "k", "v", "table"))
+    for x in (q, k, v, table):
+        x.grad = None
+    if own:
+        out = fa.relative_attention(q, k, v, table, _positions(fa, case), causal=case["causal"],
+                                    mask=state["mask"], key_lengths=state["lengths"],
+                                    q_start=state["start"])
+    else:
+        out = _plain_attention(state)
+    if not case["train"]:
+        return out
+    out.backward(state["up"])
+    return out.detach(), q.grad, k.grad, v.grad, table.grad
+
+
+# --------------------------------------------------------------------------- #
+# what a pass cannot do without
+# --------------------------------------------------------------------------- #
+
+
+def work(case):
+    """Inputs read once, outputs written once.  Attention: two products forward and
+    four backward, over the pairs that the mask of the future leaves (a ragged batch:
+    the mean length).  Orthogonalize: the Gram matrix and its square are symmetric, so
+    half of each product counts."""
+    size = _BYTES[case["dtype"]]
+    if case["op"] == "orthogonalize":
+        m, n = sorted((case["rows"], case["cols"]))
+        flops = case["batch"] * case["steps"] * (m * m * n + m ** 3 + 2 * m * m * n)
+        return {"bytes": 2 * case["batch"] * m * n * size, "flops": flops}
+    rows = _table_rows(case) * case["heads"]
+    if case["op"] == "bias":
+        pairs = case["heads"] * case["q_len"] * case["k_len"]
+        return {"bytes": (2 * pairs + 2 * rows) * size, "flops": pairs}
+    b, h, hk, d = case["batch"], case["heads"], case["kv_heads"], case["dim"]
+    keys = case["k_len"] * (0.625 if case["ragged"] else 1.0)
+    pairs = b * h * case["q_len"] * keys * (0.5 if case["causal"] else 1.0)
+    q_size, k_size = b * h * case["q_len"] * d * size, b * hk * keys * d * size
+    nbytes = 2 * q_size + 2 * k_size + rows * size
+    if case["train"]:  # the output's gradient in; the gradients of q, k, v, table out
+        nbytes += 2 * q_size + 2 * k_size + rows * size
+    return {"bytes": int(nbytes), "flops": int(pairs * d * (12 if case["train"] else 4))}
+
+
+# --------------------------------------------------------------------------- #
+# the same outputs in float64
+# --------------------------------------------------------------------------- #
+
+
+def _exact_rows(case, q_pos, k_len):
+    """The bucket rule again, pair by pair distance in numpy-like integer steps: a list
+    over every distance that occurs, then an index."""
+    dev = q_pos.device
+    if case["grid_w"]:
+        gh, gw = case["grid_h"], case["grid_w"]
+        code = torch.arange(gh * gw, device=dev)
+        code = (code // gw) * (2 * gw - 1) + code % gw
+        return code[:, None] - code[None, :] + (gh - 1) * (2 * gw - 1) + gw - 1
+    lo = -int(q_pos.max())
+    hi = k_len - 1 - int(q_pos.min())
+    rows = []
+    for rel in range(lo, hi + 1):
+        n, base, dist = case["buckets"], 0, max(0, -rel)
+        if case["bidirectional"]:
+            n //= 2
+            base, dist = (n if rel > 0 else 0), abs(rel)
+        half = n // 2
+        if dist >= half:
+            j = 0
+            while j + 1 < n - half and dist ** (n - half) >= (
+                    half ** (n - half - j - 1) * case["max_distance"] ** (j + 1)):
+                j += 1
+            dist = half + j
+        rows.append(base + dist)
+    rows = torch.tensor(rows, device=dev)
+    return rows[torch.arange(k_len, device=dev) - q_pos[..., None] - lo]
+
+
+def _exact_attention(state):
+    case = state["case"]
+    q, k, v, table = (state[x].detach() for x in ("q", "k", "v", "table"))
+    dev, lq, lk, h, hk = q.device, case["q_len"], case["k_len"], case["heads"], case["kv_heads"]
+    group, scale = h // hk, case["dim"] ** -0.5
+    start = state["start"]
+    out = torch.zeros(q.shape, dtype=torch.float64, device=dev)
+    train = case["train"]
+    if train:
+        dq, dk, dv = (torch.zeros(x.shape, dtype=torch.float64, device=dev) for x in (q, k, v))
+        dbias = torch.zeros(h, lq, lk, dtype=torch.float64, device=dev)
+    step = max(1, 2 ** 27 // (lq * lk))  # batch entries at once, for one head
+    own_rows = torch.is_tensor(start)
+    if own_rows:
+        step = 1
+    else:
+        rows = _exact_rows(case, torch.arange(lq, device=dev) + start, lk)
+    j = torch.arange(lk, device=dev)
+    for b0 in range(0, case["batch"], step):
+        part = slice(b0, min(case["batch"], b0 + step))
+        n = part.stop - b0
+        pos = torch.arange(lq, device=dev) + (int(start[b0]) if own_rows else start)
+        if own_rows:
+            rows = _exact_rows(case, pos, lk)
+        keep = torch.ones(n, lq, lk, dtype=torch.bool, device=dev)
+        if case["causal"]:
+            keep &= j[None, :] <= pos[:, None]
+        if state["mask"] is not None:
+            which = torch.arange(part.start, part.stop, device=dev) % case["windows"]
+            keep &= state["mask"][which, 0]
+        if state["lengths"] is not None:
+            keep &= (j[None, :] < state["lengths"][part].long()[:, None])[:, None, :]
+        for head in range(h):
+            qq, kk, vv = (q[part, head].double(), k[part, head // group].double(),
+                          v[part, head // group].double())
+            s = torch.matmul(qq, kk.transpose(1, 2).contiguous()) * scale
+            s += table[:, head].double()[rows]
+            s = torch.where(keep, s, torch.full_like(s, -1e300))
+            p = torch.exp(s - s.amax(2, keepdim=True)) * keep
+            p /= p.sum(2, keepdim=True).clamp_min(1e-300)
+            out[part, head] = torch.matmul(p, vv)
+            if not train:
+                continue
+            g = state["up"][part, head].double()
+            dp = torch.matmul(g, vv.transpose(1, 2).contiguous())
+            ds = p * (dp - (p * dp).sum(2, keepdim=True))
+            dv[part, head // group] += torch.matmul(p.transpose(1, 2).contiguous(), g)
+            dk[part, head // group] += scale * torch.matmul(ds.transpose(1, 2).contiguous(), qq)
+            dq[part, head] = scale * torch.matmul(ds, kk)
+            dbias[head] += ds.sum(0)
+    if not train:
+        return out
+    dtable = torch.zeros(table.shape[0], h, dtype=torch.float64, device=dev)
+    dtable.index_add_(0, rows.reshape(-1), dbias.reshape(h, -1).t().contiguous())
+    return out, dq, dk, dv, dtable
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    if case["op"] == "attention":
+        return _exact_attention(state)
+    if case["op"] == "bias":
+        table, up = state["table"].detach(), state["up"].double()
+        rows = _exact_rows(case, torch.arange(case["q_len"], device=up.device), case["k_len"])
+        grad = torch.zeros(table.shape, dtype=torch.float64, device=up.device)
+        grad.index_add_(0, rows.reshape(-1), up.reshape(up.shape[0], -1).t().contiguous())
+        bias = torch.stack([table[:, i].double()[rows] for i in range(table.shape[1])])
+        return bias, grad
+    a, b, c = _POLAR if case["polar"] else _STEEP
+    results = []
+    for g in state["update"].double():
+        x = g.t().contiguous() if case["rows"] > case["cols"] else g
+        x = x / (torch.linalg.vector_norm(x) + 1e-7)
+        eye = torch.eye(x.shape[0], dtype=torch.float64, device=x.device)
+        for _ in range(case["steps"]):
+            gram = torch.mm(x, x.t().contiguous())
+            x = torch.mm(a * eye + torch.mm(gram, b * eye + c * gram), x)
+        results.append(x.t() if case["rows"] > case["cols"] else x)
+    return torch.stack(results)

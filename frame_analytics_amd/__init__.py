@@ -41,13 +41,22 @@ from .modules import (  # noqa: F401
     StreamingMetrics,
 )
 
+from .training import (  # noqa: F401
+    GridPositions,
+    LinePositions,
+    orthogonalize,
+    relative_attention,
+    relative_bias,
+)
+
 __version__ = "0.1.0"
 
 __all__ = [
     "mse", "psnr", "ssim", "ms_ssim", "gmsd", "gms", "l1", "charbonnier", "huber",
     "rgb_to_luma", "MSE", "PSNR", "SSIM", "MSSSIM", "GMSD", "L1", "Charbonnier",
     "Huber", "StreamingMetrics", "gaussian_window_1d", "set_compile_enabled",
-    "backend_status", "MS_SSIM_WEIGHTS",
+    "backend_status", "MS_SSIM_WEIGHTS", "relative_attention", "relative_bias",
+    "orthogonalize", "LinePositions", "GridPositions",
 ]
 
 

@@ -91,6 +91,26 @@ SIGNATURES = {
 }
 
 
+# one line per entry point of include/fa_train_abi.h
+TRAIN_SIGNATURES = {
+    "fa_gpu_rel_bias": ([_P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _L, _P, _I, _P], _I),
+    "fa_gpu_rel_bias_workspace": ([_I, _I, _I, _I, _P], _I),
+    "fa_gpu_rel_bias_backward":
+        ([_P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _L, _P, _P, _L, _I, _P], _I),
+    "fa_gpu_rel_attention_workspace": ([_I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P], _I),
+    "fa_gpu_rel_attention":
+        ([_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _L, _P, _P, _P, _I,
+          _P, _I, _D, _P, _P, _P, _L, _I, _P], _I),
+    "fa_gpu_rel_attention_backward_workspace": ([_I, _I, _I, _I, _I, _P], _I),
+    "fa_gpu_rel_attention_backward":
+        ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _L, _P,
+          _P, _P, _I, _P, _I, _D, _P, _P, _P, _P, _P, _L, _I, _P], _I),
+    "fa_gpu_orthogonalize_workspace": ([_I, _I, _I, _I, _P], _I),
+    "fa_gpu_orthogonalize":
+        ([_P, _I, _I, _I, _I, _I, _D, _D, _D, _D, _P, _P, _L, _I, _P], _I),
+}
+
+
 # one line per entry point of include/fa_cpu_abi.h (reference _cabi.py:416-423)
 CPU_SIGNATURES = {
     "fa_cpu_abi_version": ([], _I),
@@ -154,6 +174,7 @@ def load_gpu(path: Optional[Path] = None) -> Tuple[ctypes.CDLL, str]:
     # RTLD_GLOBAL is not needed: nothing links against this library.
     lib = bind(ctypes.CDLL(str(p)))
     _check_abi(lib, p)
+    bind(lib, TRAIN_SIGNATURES)
     return lib, origin
 
 
@@ -161,9 +182,10 @@ def load_gpu(path: Optional[Path] = None) -> Tuple[ctypes.CDLL, str]:
 _LETTER = {_P: "p", _I: "i", _L: "l", _D: "d"}
 
 
-def load_callers(lib: ctypes.CDLL) -> dict:
+def load_callers(lib: ctypes.CDLL, signatures: Optional[dict] = None) -> dict:
     """Entry point name -> callable of the ``_fa_call`` extension module for the
-    entry points of ``lib`` that are called often (the rest stay with ctypes).
+    entry points of ``lib`` that are called often (the rest stay with ctypes), of
+    ``signatures``: those of ``include/fa_abi.h`` unless given.
     The module holds prototypes of its own, so only those that are the ones
     ctypes would use are taken.  Empty where the module cannot be built or loaded (no
     Python headers) or is of another ABI version: the same library is then called
@@ -178,7 +200,7 @@ def load_callers(lib: ctypes.CDLL) -> dict:
         spec.loader.exec_module(module)
         if module.abi_version != FA_ABI_VERSION:
             return {}
-        for name, (args, _) in SIGNATURES.items():
+        for name, (args, _) in (SIGNATURES if signatures is None else signatures).items():
             fn = module.entry(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value,
                               "".join(_LETTER.get(a, "?") for a in args))
             if fn is not None:

@@ -105,7 +105,8 @@ def load(force: bool = False) -> Optional[_Native]:
     native = _Native()
     try:
         native.gpu, native.gpu_origin = _cabi.load_gpu()
-        native.callers = _cabi.load_callers(native.gpu)
+        native.callers = {**_cabi.load_callers(native.gpu),
+                          **_cabi.load_callers(native.gpu, _cabi.TRAIN_SIGNATURES)}
     except Exception as exc:
         _load_error = f"{type(exc).__name__}: {exc}"
         raise RuntimeError(

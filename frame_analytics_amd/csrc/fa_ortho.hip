@@ -1,0 +1,433 @@
+// The orthogonalised update: X <- a X + (b A + c A^2) X with A = X X^T, from X =
+// g / (|g| + eps), which drives every singular value of g towards one.
+//
+// All the work is matrix products, on the matrix cores in float16 with float32
+// accumulators.  Matrices are held times a power of two (X and A 2^11, the polynomial
+// 2^10) so that float16's range serves them: singular values stay near or below one,
+// so entries do.  Two precisions:
+//
+//   single (bfloat16 input of more than 64 rows): one float16 per entry.  Rounding X to 11 bits is noise
+//     in every direction, and a step multiplies a small singular direction by a, so X
+//     is also kept in float32 for the a X term while three or more steps follow; the
+//     result is within 1.5e-3 of exact before it is rounded to bfloat16 (1.7e-3).
+//   pair (the rest): hi + lo, 22 bits, three products hi hi + hi lo +
+//     lo hi; the result is within 3e-6, as with float32 products.
+//
+// A and its square are symmetric: only tiles on and above the diagonal are computed.
+// Products are rows times rows (both operands contiguous along k), so X is kept both
+// ways round.  The norm's factor is a power of two, exact, in the operands and the rest
+// (in (1, 2]) in the first step's epilogues: 16-bit input enters unrounded.
+#include "fa_matrix.h"
+#include "fa_train_abi.h"
+
+#include <utility>
+
+namespace fa {
+namespace {
+
+typedef _Float16 f16;
+constexpr int NT = 256;
+constexpr int SUMS = 64;                     // partial sums of squares per matrix
+constexpr float SX = 2048.0f, SP = 1024.0f;  // scale of X and A, of the polynomial
+
+template <typename T> __device__ inline float widen(T v) { return static_cast<float>(v); }
+
+struct Poly {
+  float a, b, c;
+};
+
+// Where the matrices of a call stand: batch after batch in each.
+struct Bufs {
+  f16 *x[2], *a[2], *p[2];  // hi, lo (lo null in single precision)
+  // X^T, an operand of the step that overwrites X: read from one buffer and written to
+  // the other (X itself is read only where the same thread then writes it)
+  f16 *xt[2], *xt_out[2];
+  float* xf;                         // X in float32 (single precision only)
+  float* f;                          // [batch] the first step's factor
+  double* sums;                      // [batch][SUMS]
+};
+
+// ---------------------------------------------------------------------------
+// |g|^2, then X and its transpose
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(NT) void ortho_norm_kernel(const T* g, int64_t count, double* sums) {
+  const T* p = g + blockIdx.y * count;
+  double acc = 0.0;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(NT) + threadIdx.x; i < count; i += NT * SUMS) {
+    const double v = static_cast<double>(widen(p[i]));
+    acc += v * v;
+  }
+  __shared__ double smem[WAVES_PER_BLOCK];
+  const double s = block_sum(acc, smem);
+  if (threadIdx.x == 0) sums[blockIdx.y * SUMS + blockIdx.x] = s;
+}
+
+__device__ inline void put(f16* hi, f16* lo, int64_t at, float v) {
+  const f16 h = f16(v);
+  hi[at] = h;
+  if (lo) lo[at] = f16(v - float(h));
+}
+
+constexpr int PT = 64;  // side of a transposed piece
+template <typename T>
+__global__ __launch_bounds__(NT) void ortho_prep_kernel(const T* g, int rows, int cols, int m, int n,
+                                                        int mp, int np, double eps, Bufs w) {
+  __shared__ float tile[PT][PT + 1];
+  __shared__ double smem[WAVES_PER_BLOCK];
+  __shared__ int exponent;
+  const int b = blockIdx.z;
+  {
+    const double s = block_sum(threadIdx.x < SUMS ? w.sums[b * SUMS + threadIdx.x] : 0.0, smem);
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(s) + eps;
+      int ex = 0;
+      const double mant = frexp(norm, &ex);
+      const bool fine = norm < __builtin_inf();  // not inf, not NaN: the result is NaN there
+      exponent = fine ? ex : 0;
+      if (blockIdx.x == 0 && blockIdx.y == 0)
+        w.f[b] = fine ? static_cast<float>(1.0 / mant) : __builtin_nanf("");
+    }
+    __syncthreads();
+  }
+  const int shift = 11 - exponent;  // SX is 2^11
+  const int i0 = blockIdx.y * PT, j0 = blockIdx.x * PT;  // of X, m x n
+  const T* src = g + static_cast<int64_t>(b) * rows * cols;
+  const bool tall = rows > cols;
+  for (int t = threadIdx.x; t < PT * PT; t += NT) {
+    // consecutive threads along the input's rows
+    const int u = t / PT, v = t % PT;
+    const int i = tall ? v : u, j = tall ? u : v;
+    float x = 0.0f;
+    if (i0 + i < m && j0 + j < n)
+      x = widen(src[tall ? static_cast<int64_t>(j0 + j) * cols + i0 + i
+                         : static_cast<int64_t>(i0 + i) * cols + j0 + j]);
+    tile[i][j] = ldexpf(x, shift);
+  }
+  __syncthreads();
+  const int64_t base = static_cast<int64_t>(b) * mp * np;
+  f16* xl = w.x[1] ? w.x[1] + base : nullptr;
+  f16* tl = w.xt[1] ? w.xt[1] + base : nullptr;
+  for (int t = threadIdx.x; t < PT * PT; t += NT) {
+    const int u = t / PT, v = t % PT;
+    put(w.x[0] + base, xl, static_cast<int64_t>(i0 + u) * np + j0 + v, tile[u][v]);
+    put(w.xt[0] + base, tl, static_cast<int64_t>(j0 + u) * mp + i0 + v, tile[v][u]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------
+enum Mode : int { GRAM = 0, SQUARE = 1, STEP = 2 };
+
+struct Step {
+  int m, n, mp, np;
+  Poly poly;
+  bool first, last;     // of the steps
+  bool read_f, write_f;  // X in float32
+  bool tall;
+  int tiles_i, tiles_j;
+};
+
+// Tile t of the tiles on and above the diagonal of a k x k grid, row by row.
+__device__ inline void upper(int t, int k, int* ti, int* tj) {
+  int i = static_cast<int>((2 * k + 1 - sqrtf(static_cast<float>((2 * k + 1) * (2 * k + 1) - 8 * t))) * 0.5f);
+  auto before = [k](int r) { return r * k - r * (r - 1) / 2; };
+  while (i > 0 && before(i) > t) --i;
+  while (before(i + 1) <= t) ++i;
+  *ti = i;
+  *tj = i + t - before(i);
+}
+
+template <int TM, bool PAIR, int MODE, typename T>
+__global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* out) {
+  constexpr int BK = PAIR ? 32 : 64, PARTS = PAIR ? 2 : 1, WT = TM / 2, NB = WT / 32;
+  using TL = Tile<f16, BK>;
+  using M = Mat<f16>;
+  constexpr int PIECE = TM * TL::LD;
+  extern __shared__ __align__(16) unsigned char smem[];
+  f16* lds = reinterpret_cast<f16*>(smem);  // [2][A, B][PARTS][TM][LD]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const int per = MODE == STEP ? st.tiles_i * st.tiles_j : st.tiles_i * (st.tiles_i + 1) / 2;
+  const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
+  const int b = wg / per, t = wg % per;
+  int ti, tj;
+  if (MODE == STEP) {
+    ti = t / st.tiles_j;
+    tj = t % st.tiles_j;
+  } else {
+    upper(t, st.tiles_i, &ti, &tj);
+  }
+  const int K = MODE == GRAM ? st.np : st.mp;
+  const int64_t xs = static_cast<int64_t>(st.mp) * st.np, as = static_cast<int64_t>(st.mp) * st.mp;
+  f16* const* A = MODE == GRAM ? w.x : MODE == SQUARE ? w.a : w.p;
+  f16* const* B = MODE == GRAM ? w.x : MODE == SQUARE ? w.a : w.xt;
+  const int64_t abase = b * (MODE == GRAM ? xs : as), bbase = b * (MODE == SQUARE ? as : xs);
+  const f16 *ap[PARTS], *bp[PARTS];
+#pragma unroll
+  for (int s = 0; s < PARTS; ++s) {
+    ap[s] = A[s] + abase + static_cast<int64_t>(ti) * TM * K;
+    bp[s] = B[s] + bbase + static_cast<int64_t>(tj) * TM * K;
+  }
+  TileLoad<f16, BK, TM, NT> al[PARTS], bl[PARTS];
+  auto load = [&](int k) {
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s) {
+      al[s].load(ap[s] + k, K, 0, TM, BK, 8, tid);
+      bl[s].load(bp[s] + k, K, 0, TM, BK, 8, tid);
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s) {
+      al[s].store(lds + ((buf * 2 + 0) * PARTS + s) * PIECE, tid);
+      bl[s].store(lds + ((buf * 2 + 1) * PARTS + s) * PIECE, tid);
+    }
+  };
+  const int wi = (wave >> 1) * WT, wj = (wave & 1) * WT;
+  f32x16 acc[NB][NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  load(0);
+  store(0);
+  const int steps = K / BK;
+  for (int k = 0; k < steps; ++k) {
+    __syncthreads();
+    if (k + 1 < steps) load((k + 1) * BK);
+    const f16* la = lds + ((k & 1) * 2 + 0) * PARTS * PIECE;
+    const f16* lb = lds + ((k & 1) * 2 + 1) * PARTS * PIECE;
+#pragma unroll
+    for (int c = 0; c < BK / 16; ++c) {
+      f16x8 af[PARTS][NB], bf[PARTS][NB];
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          af[s][i] = TL::straight(la + s * PIECE, wi + 32 * i + col, 16 * c + 8 * hh);
+          bf[s][i] = TL::straight(lb + s * PIECE, wj + 32 * i + col, 16 * c + 8 * hh);
+        }
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          acc[i][j] = M::mma(af[0][i], bf[0][j], acc[i][j]);
+          if constexpr (PAIR) {
+            acc[i][j] = M::mma(af[0][i], bf[1][j], acc[i][j]);
+            acc[i][j] = M::mma(af[1][i], bf[0][j], acc[i][j]);
+          }
+        }
+    }
+    if (k + 1 < steps) store((k + 1) & 1);
+  }
+
+  const float f = st.first ? w.f[b] : 1.0f;
+#pragma unroll
+  for (int bi = 0; bi < NB; ++bi)
+#pragma unroll
+    for (int bj = 0; bj < NB; ++bj) {
+      const int j = tj * TM + wj + 32 * bj + col;
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int i = ti * TM + wi + 32 * bi + 8 * r4 + 4 * hh;  // four rows from here
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[bi][bj][4 * r4 + e];
+        if constexpr (MODE == GRAM || MODE == SQUARE) {
+          f16* const* dst = MODE == GRAM ? w.a : w.p;
+          const int64_t o = b * as;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t at = o + static_cast<int64_t>(i + e) * st.mp + j;
+            if constexpr (MODE == GRAM) {
+              v[e] *= f * f / SX;  // SX A of (SX X)(SX X)^T
+            } else {
+              float x = float(w.a[0][at]);
+              if constexpr (PAIR) x += float(w.a[1][at]);
+              v[e] = (SP / SX) * st.poly.b * x + (SP / SX / SX) * st.poly.c * v[e];
+            }
+            put(dst[0], PAIR ? dst[1] : nullptr, at, v[e]);
+          }
+          if (ti != tj) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              put(dst[0], PAIR ? dst[1] : nullptr, o + static_cast<int64_t>(j) * st.mp + i + e, v[e]);
+          }
+        } else {
+          const int64_t o = b * xs;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t at = o + static_cast<int64_t>(i + e) * st.np + j;
+            float x;
+            if (!PAIR && st.read_f) {
+              x = w.xf[at];
+            } else {
+              x = float(w.x[0][at]);
+              if constexpr (PAIR) x += float(w.x[1][at]);
+            }
+            v[e] = f * (st.poly.a * x + v[e] / SP);
+          }
+          if (st.last) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < st.m && j < st.n) {
+                const int64_t at = st.tall ? static_cast<int64_t>(j) * st.m + i + e
+                                           : static_cast<int64_t>(i + e) * st.n + j;
+                out[static_cast<int64_t>(b) * st.m * st.n + at] = T(v[e] / SX);
+              }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int64_t at = o + static_cast<int64_t>(i + e) * st.np + j;
+              put(w.x[0], PAIR ? w.x[1] : nullptr, at, v[e]);
+              put(w.xt_out[0], PAIR ? w.xt_out[1] : nullptr, o + static_cast<int64_t>(j) * st.mp + i + e, v[e]);
+              if (!PAIR && st.write_f) w.xf[at] = v[e];
+            }
+          }
+        }
+      }
+    }
+}
+
+struct Plan {
+  int m, n, mp, np, tile, parts;
+  int64_t off_x, off_xt0, off_xt1, off_a, off_p, off_xf, off_f, off_sums, bytes;
+};
+
+inline int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+inline int plan(int dtype, int batch, int rows, int cols, Plan* p) {
+  if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return FA_E_DTYPE;
+  if (batch < 1 || rows < 1 || cols < 1 || batch > 65535 || rows > (1 << 20) || cols > (1 << 20))
+    return FA_E_SHAPE;
+  p->m = rows < cols ? rows : cols;
+  p->n = rows < cols ? cols : rows;
+  // up to 64 rows a product is a launch's time whatever its precision, and little
+  // averages the noise of single float16
+  p->parts = dtype == FA_BF16 && p->m > 64 ? 1 : 2;
+  p->tile = 128;
+  p->mp = (p->m + p->tile - 1) / p->tile * p->tile;
+  p->np = (p->n + p->tile - 1) / p->tile * p->tile;
+  const int64_t xs = static_cast<int64_t>(batch) * p->mp * p->np, as = static_cast<int64_t>(batch) * p->mp * p->mp;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += align256(bytes);
+    return o;
+  };
+  p->off_x = take(xs * 2 * p->parts);
+  p->off_xt0 = take(xs * 2 * p->parts);
+  p->off_xt1 = take(xs * 2 * p->parts);
+  p->off_a = take(as * 2 * p->parts);
+  p->off_p = take(as * 2 * p->parts);
+  p->off_xf = take(p->parts == 1 ? xs * 4 : 0);
+  p->off_f = take(batch * 4);
+  p->off_sums = take(static_cast<int64_t>(batch) * SUMS * 8);
+  p->bytes = at;
+  return FA_OK;
+}
+
+template <int TM, bool PAIR, int MODE, typename T>
+int launch_product(const Bufs& w, const Step& st, int batch, T* out, hipStream_t s) {
+  constexpr int BK = PAIR ? 32 : 64, PARTS = PAIR ? 2 : 1;
+  constexpr size_t lds = size_t(4) * PARTS * TM * Tile<f16, BK>::LD * sizeof(f16);
+  const int64_t per = MODE == STEP ? static_cast<int64_t>(st.tiles_i) * st.tiles_j
+                                   : static_cast<int64_t>(st.tiles_i) * (st.tiles_i + 1) / 2;
+  if (per * batch > 0x7fffffff) return FA_E_SHAPE;
+  auto kernel = ortho_product_kernel<TM, PAIR, MODE, T>;
+  if (lds > 64 * 1024)
+    FA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+  kernel<<<static_cast<unsigned>(per * batch), NT, lds, s>>>(w, st, out);
+  FA_LAUNCH_CHECK();
+  return FA_OK;
+}
+
+template <typename T, bool PAIR>
+int orthogonalize(const void* g, int batch, int rows, int cols, int steps, const Poly& poly, double eps,
+                  void* out, char* ws, const Plan& p, hipStream_t s) {
+  const int64_t xs = static_cast<int64_t>(batch) * p.mp * p.np, as = static_cast<int64_t>(batch) * p.mp * p.mp;
+  auto set = [&](f16** dst, int64_t off, int64_t count) {
+    dst[0] = reinterpret_cast<f16*>(ws + off);
+    dst[1] = PAIR ? dst[0] + count : nullptr;
+  };
+  Bufs w{};
+  set(w.x, p.off_x, xs);
+  set(w.xt, p.off_xt0, xs);
+  set(w.a, p.off_a, as);
+  set(w.p, p.off_p, as);
+  w.xf = PAIR ? nullptr : reinterpret_cast<float*>(ws + p.off_xf);
+  w.f = reinterpret_cast<float*>(ws + p.off_f);
+  w.sums = reinterpret_cast<double*>(ws + p.off_sums);
+  ortho_norm_kernel<T><<<dim3(SUMS, batch), NT, 0, s>>>(static_cast<const T*>(g),
+                                                        static_cast<int64_t>(rows) * cols, w.sums);
+  FA_LAUNCH_CHECK();
+  ortho_prep_kernel<T><<<dim3(p.np / PT, p.mp / PT, batch), NT, 0, s>>>(
+      static_cast<const T*>(g), rows, cols, p.m, p.n, p.mp, p.np, eps, w);
+  FA_LAUNCH_CHECK();
+  Step st{};
+  st.m = p.m;
+  st.n = p.n;
+  st.mp = p.mp;
+  st.np = p.np;
+  st.poly = poly;
+  st.tall = rows > cols;
+  st.tiles_i = p.mp / p.tile;
+  st.tiles_j = p.np / p.tile;
+  set(w.xt_out, p.off_xt1, xs);
+  T* o = static_cast<T*>(out);
+  for (int k = 0; k < steps; ++k) {
+    st.first = k == 0;
+    st.last = k == steps - 1;
+    st.read_f = k >= 1 && steps - k >= 3;
+    st.write_f = steps - (k + 1) >= 3;
+    if (const int e = launch_product<128, PAIR, GRAM, T>(w, st, batch, o, s)) return e;
+    if (const int e = launch_product<128, PAIR, SQUARE, T>(w, st, batch, o, s)) return e;
+    if (const int e = launch_product<128, PAIR, STEP, T>(w, st, batch, o, s)) return e;
+    std::swap(w.xt, w.xt_out);
+  }
+  return FA_OK;
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" {
+
+FA_API int fa_gpu_orthogonalize_workspace(int dtype, int batch, int rows, int cols,
+                                          int64_t* out_bytes) {
+  if (!out_bytes) return FA_E_ARG;
+  fa::Plan p;
+  if (const int e = fa::plan(dtype, batch, rows, cols, &p)) return e;
+  *out_bytes = p.bytes;
+  return FA_OK;
+}
+
+FA_API int fa_gpu_orthogonalize(const void* g, int dtype, int batch, int rows, int cols, int steps,
+                                double a, double b, double c, double eps, void* out,
+                                void* workspace, int64_t workspace_bytes, int device,
+                                void* stream) {
+  using namespace fa;
+  if (!g || !out || !workspace) return FA_E_ARG;
+  Plan p;
+  if (const int e = plan(dtype, batch, rows, cols, &p)) return e;
+  if (steps < 1 || !(eps > 0.0) || workspace_bytes < p.bytes) return FA_E_ARG;
+  DeviceScope scope(device);
+  if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
+  const Poly poly{static_cast<float>(a), static_cast<float>(b), static_cast<float>(c)};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  switch (dtype) {
+    case FA_BF16:
+      return p.parts == 1
+                 ? orthogonalize<__bf16, false>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s)
+                 : orthogonalize<__bf16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s);
+    case FA_F16: return orthogonalize<f16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s);
+    default: return orthogonalize<float, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s);
+  }
+}
+
+}  // extern "C"

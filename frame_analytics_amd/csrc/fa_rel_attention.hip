@@ -1,0 +1,298 @@
+// Attention with a relative position bias, forward.
+//
+// A wave owns 32 queries and walks over the keys, 64 at a time through LDS, with the
+// running maximum and sum of its rows' softmax.  It forms S^T = K Q^T, so a lane
+// holds one query's scores (a row's statistics are the lane's own, and one exchange
+// with lane l ^ 32), and O^T = V^T P^T, whose B operand is the rounded scores as they
+// stand in the registers.  The bias is added from one head's table in LDS: on a line a
+// block of keys that is far from the wave's queries has one bias for all its pairs.
+#include "fa_rel_attention.h"
+
+namespace fa {
+namespace {
+
+template <typename T, int DP> struct Shape {
+  static constexpr int BN = sizeof(T) == 2 || DP <= 64 ? 64 : 32;  // keys per tile
+  static constexpr size_t TILE = size_t(BN) * Tile<T, DP>::LD * sizeof(T);
+};
+
+// 16 scores of a block whose pairs may be hidden: those are -inf.  k: the key of
+// register 0 of this lane, q: its query (row q of the mask, position qpos).
+__device__ inline void hide(f32x16& s, const RelAttn& a, const uint8_t* mask, int q, int qpos, int k,
+                            int len) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int key = k + 8 * (r / 4) + r % 4;
+    bool on = key < len && (!a.causal || key <= qpos);
+    if (mask && on) on = mask[q * a.mq + key * a.mk] != 0;
+    if (!on) s[r] = -INF;
+  }
+}
+
+// acc += V^T P^T over 16 keys of which some are hidden from some queries: a value
+// that is not finite must not reach the queries that do not see it (0 x inf).  The
+// finite values go through the product; the others are counted by two more, with 1 in
+// the place of each value and of each visible pair.
+template <typename T>
+__device__ inline f32x16 guarded(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x16 acc) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(widen(v[i])) < INF);
+  if (__ballot(bad) == 0) return Mat<T>::mma(v, p, acc);
+  typename Mat<T>::V8 fine, up, down, seen;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = widen(v[i]);
+    fine[i] = __builtin_fabsf(x) < INF ? v[i] : T(0);
+    up[i] = x < INF ? T(0) : T(1);       // +inf, NaN
+    down[i] = x > -INF ? T(0) : T(1);    // -inf, NaN
+    seen[i] = widen(p[i]) == 0.0f ? T(0) : T(1);
+  }
+  acc = Mat<T>::mma(fine, p, acc);
+  f32x16 u, d;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) u[r] = d[r] = 0.0f;
+  u = Mat<T>::mma(up, seen, u);
+  d = Mat<T>::mma(down, seen, d);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    if (u[r] > 0.0f) acc[r] += INF;
+    if (d[r] > 0.0f) acc[r] -= INF;
+  }
+  return acc;
+}
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* out, View os,
+                                                                int ovec, float* lse,
+                                                                int q_tiles) {
+  using M = Mat<T>;
+  using TL = Tile<T, DP>;
+  constexpr int NT = NW * 64, BN = Shape<T, DP>::BN, NB = BN / 32, CH = DP / 16, OB = DP / 32;
+  extern __shared__ __align__(16) unsigned char smem[];
+  T* kt = reinterpret_cast<T*>(smem);           // [2][BN][LD]
+  T* vt = kt + 2 * BN * TL::LD;                 // [2][BN][LD]
+  float* eb = reinterpret_cast<float*>(vt + 2 * BN * TL::LD);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
+  const int tile = q_tiles - 1 - int(wg % q_tiles);  // the longest of a causal head first
+  const int h = int(wg / q_tiles) % a.H, b = int(wg / q_tiles) / a.H, hk = h / (a.H / a.Hk);
+  const int qw = tile * (NW * 32) + wave * 32;  // the wave's first query
+  const int q = qw + col, qc = min(q, a.Lq - 1), s0 = a.start(b), len = a.keys(b);
+  const int qpos = s0 + q, cq = s0 + a.pos.code(qc);
+  const uint8_t* mask = a.mask_of(b, h);
+  const float c = a.scale * LOG2E;
+
+  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, a.pos, tid, NT);
+
+  typename M::V8 qf[CH];
+  const T* qrow = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h + qc * a.qs.t;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) qf[i] = load8<T>(qrow, 16 * i + 8 * hh, a.D, a.vec, q < a.Lq);
+
+  f32x16 o[OB];
+#pragma unroll
+  for (int i = 0; i < OB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+  float m = -INF, l = 0.0f;
+
+  // keys that any query of the workgroup sees
+  int end = len;
+  if (a.causal) {
+    const int64_t last = int64_t(s0) + min(tile * (NW * 32) + NW * 32, a.Lq);
+    end = static_cast<int>(max<int64_t>(0, min<int64_t>(end, last)));
+  }
+  const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
+  TileLoad<T, DP, BN, NT> kl, vl;
+  const int tiles = (end + BN - 1) / BN;
+  if (tiles > 0) {
+    kl.load(kb, a.ks.t, 0, len, a.D, a.vec, tid);
+    vl.load(vb, a.vs.t, 0, len, a.D, a.vec, tid);
+    kl.store(kt, tid);
+    vl.store(vt, tid);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    __syncthreads();
+    const T* kk = kt + (t & 1) * BN * TL::LD;
+    const T* vv = vt + (t & 1) * BN * TL::LD;
+    const bool more = t + 1 < tiles;
+    if (more) {
+      kl.load(kb, a.ks.t, (t + 1) * BN, len, a.D, a.vec, tid);
+      vl.load(vb, a.vs.t, (t + 1) * BN, len, a.D, a.vec, tid);
+    }
+    f32x16 s[NB];
+    bool partial[NB];
+    float top = -INF;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[nb][r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        s[nb] = M::mma(TL::straight(kk, nb * 32 + col, 16 * i + 8 * hh), qf[i], s[nb]);
+      const int k0 = t * BN + nb * 32;
+      if (a.pos.grid_w == 0) {
+        // differences of the whole block: uniform over the wave
+        const int dmax = s0 + qw + 31 - k0, dmin = s0 + qw - (k0 + 31);
+        const int kind = block_kind(a.pos, dmin, dmax);
+        if (kind == NEAR) {
+          // rows past Lq stand at their own positions here: the block's reads stay
+          // within PAD of the table
+          const float* e = eb + (s0 + q - k0 - 4 * hh - a.pos.lo + PAD);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[nb][r] = s[nb][r] * c + e[-(8 * (r / 4) + r % 4)];
+        } else {
+          const float e = kind == ALL_BELOW ? eb[0] : eb[a.pos.n + 2 * PAD - 1];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[nb][r] = s[nb][r] * c + e;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = min(k0 + 4 * hh + 8 * (r / 4) + r % 4, a.Lk - 1);
+          s[nb][r] = s[nb][r] * c + eb[cq - a.pos.code(key) - a.pos.lo + PAD];
+        }
+      }
+      partial[nb] = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
+      if (partial[nb]) hide(s[nb], a, mask, qc, qpos, k0 + 4 * hh, len);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
+    }
+    top = both_max(top);
+    const float mn = fmaxf(m, top);
+    if (__ballot(mn > m)) {  // a row's maximum grew: what was summed shrinks by it
+      const float shrink = mn == -INF ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      l *= shrink;
+#pragma unroll
+      for (int i = 0; i < OB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= shrink;
+      m = mn;
+    }
+    const float sub = m == -INF ? 0.0f : m;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[nb][r] = __builtin_amdgcn_exp2f(s[nb][r] - sub);
+        l += s[nb][r];
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // the weights are rounded to the element type for the product with V; their
+        // sum is not
+        typename M::V8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = T(s[nb][8 * half + i]);
+#pragma unroll
+        for (int i = 0; i < OB; ++i) {
+          const typename M::V8 vf = TL::transposed(vv, nb * 32 + 16 * half, 32 * i, lane);
+          o[i] = partial[nb] ? guarded<T>(vf, p, o[i]) : M::mma(vf, p, o[i]);
+        }
+      }
+    }
+    if (more) {
+      kl.store(kt + ((t + 1) & 1) * BN * TL::LD, tid);
+      vl.store(vt + ((t + 1) & 1) * BN * TL::LD, tid);
+    }
+  }
+  l = both_sum(l);
+  if (q < a.Lq) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* orow = out + b * os.b + h * os.h + q * os.t;
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = o[i][4 * g + e] * inv;
+        store4<T>(orow, 32 * i + 8 * g + 4 * hh, a.D, ovec, w);
+      }
+    if (lse && hh == 0)
+      lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + q] = l == 0.0f ? INF : m + __builtin_log2f(l);
+  }
+}
+
+template <typename T, int DP, int NW>
+int launch_one(const RelAttn& a, T* out, const View& os, int ovec, float* lse, hipStream_t s) {
+  const int q_tiles = (a.Lq + NW * 32 - 1) / (NW * 32);
+  const int64_t wgs = static_cast<int64_t>(a.B) * a.H * q_tiles;
+  if (wgs > 0x7fffffff) return FA_E_SHAPE;
+  const size_t lds = 4 * Shape<T, DP>::TILE + (a.pos.n + 2 * PAD) * sizeof(float);
+  auto kernel = rel_attention_kernel<T, DP, NW>;
+  if (const int e = launch_lds(kernel, lds)) return e;
+  kernel<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, out, os, ovec, lse, q_tiles);
+  FA_LAUNCH_CHECK();
+  return FA_OK;
+}
+
+template <typename T, int DP>
+int launch_dim(const RelAttn& a, T* out, const View& os, int ovec, float* lse, hipStream_t s) {
+  return a.Lq <= 64 ? launch_one<T, DP, 2>(a, out, os, ovec, lse, s)
+                    : launch_one<T, DP, 4>(a, out, os, ovec, lse, s);
+}
+
+template <typename T>
+int forward(RelAttn a, void* out, const View& os, float* lse, hipStream_t s) {
+  const void* in[3] = {a.q, a.k, a.v};
+  const View iv[3] = {a.qs, a.ks, a.vs};
+  a.vec = widest_load<T>(in, iv, 3, a.D);
+  const void* op[1] = {out};
+  const int ovec = widest_load<T>(op, &os, 1, a.D);
+  T* o = static_cast<T*>(out);
+  if (a.D <= 32) return launch_dim<T, 32>(a, o, os, ovec, lse, s);
+  if (a.D <= 64) return launch_dim<T, 64>(a, o, os, ovec, lse, s);
+  return launch_dim<T, 128>(a, o, os, ovec, lse, s);
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" {
+
+FA_API int fa_gpu_rel_attention_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int n,
+                                          int has_mask, int need_lse, int device,
+                                          int64_t* out_bytes) {
+  (void)has_mask;
+  (void)need_lse;
+  (void)device;
+  if (!out_bytes) return FA_E_ARG;
+  if (n < 1 || n > FA_REL_MAX) return FA_E_SHAPE;
+  if (const int e = fa::check_attention(B, H, Hk, Lq, Lk, D, nullptr, 1, nullptr)) return e;
+  *out_bytes = 0;
+  return FA_OK;
+}
+
+FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int dtype, int B,
+                                int H, int Hk, int Lq, int Lk, int D, const int64_t* strides,
+                                const void* table, int rows, const int* row_of, int lo, int n,
+                                int grid_w, int64_t q_start, const int* q_starts,
+                                const int* key_lengths, const uint8_t* mask, int mask_b,
+                                const int64_t* mask_strides, int causal, double scale, void* out,
+                                float* lse, void* workspace, int64_t workspace_bytes, int device,
+                                void* stream) {
+  using namespace fa;
+  (void)workspace;
+  (void)workspace_bytes;
+  if (!q || !k || !v || !strides || !table || !out) return FA_E_ARG;
+  if (const int e = check_attention(B, H, Hk, Lq, Lk, D, mask, mask_b, mask_strides)) return e;
+  if (const int e = check_relpos(row_of, rows, lo, n, grid_w, Lq, Lk, q_start, q_starts)) return e;
+  DeviceScope scope(device);
+  if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
+  const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table,
+                                  RelPos{row_of, lo, n, grid_w}, q_start, q_starts, key_lengths,
+                                  mask, mask_b, mask_strides, causal, scale);
+  const View os{strides[9], strides[10], strides[11]};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case FA_F16: return forward<_Float16>(a, out, os, lse, s);
+    case FA_BF16: return forward<__bf16>(a, out, os, lse, s);
+    case FA_F32: return forward<float>(a, out, os, lse, s);
+    default: return FA_E_DTYPE;
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,566 @@
+// Attention with a relative position bias, backward.
+//
+// With P the weights (formed again from the scores and each row's log-sum) and D_i =
+// dout_i . out_i:  dS = P (dout V^T - D);  dQ = scale dS K;  dK = scale dS^T Q;
+// dV = P^T dout;  dtable[r] = the sum of dS over the pairs of row r.
+//
+// Two kernels, so that every sum has one owner and a fixed order: one whose waves own
+// queries (dQ, and the table's sums by difference), one whose waves own keys (dK, dV,
+// over the query heads that share them).  Each forms S and dout V^T again: seven
+// products in place of five, against atomic sums of dQ in memory in no fixed order.
+#include "fa_rel_attention.h"
+
+namespace fa {
+
+template <typename T>
+void launch_table_sum(const float* partial, int parts, int n, const int* row_of, int rows, int H,
+                      T* dtable, hipStream_t s);
+
+namespace {
+
+struct Grads {
+  const void *out, *dout;
+  View os, gs;
+  const float* lse;
+  float* dsum;  // [B, H, Lq]: D_i
+  void *dq, *dk, *dv;
+  View dqs, dks, dvs;
+  int dqvec, dkvec;
+  float* parts;  // [H][B * q_tiles][n], or null: the table needs no gradient
+};
+
+constexpr int NW = 4, NT = NW * 64;
+
+template <typename T, int DP> struct Shape {
+  static constexpr int BN = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
+  static constexpr int BUFS = sizeof(T) == 4 && DP == 128 ? 1 : 2;
+  static constexpr size_t TILE = size_t(BN) * Tile<T, DP>::LD * sizeof(T);
+};
+
+// Elements that are not finite become 0.  K of a pair that is seen and not finite has
+// made that pair's dS NaN already; one that is hidden must not turn 0 x K into NaN.
+template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<T>::V8 v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __builtin_fabsf(widen(v[i])) < INF ? v[i] : T(0);
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// dQ and the table
+// ---------------------------------------------------------------------------
+template <typename T, int DP, bool TABLE>
+__global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g, int q_tiles) {
+  using M = Mat<T>;
+  using TL = Tile<T, DP>;
+  constexpr int BN = Shape<T, DP>::BN, NB = BN / 32, CH = DP / 16, OB = DP / 32;
+  constexpr int BUFS = Shape<T, DP>::BUFS;
+  extern __shared__ __align__(16) unsigned char smem[];
+  T* kt = reinterpret_cast<T*>(smem);
+  T* vt = kt + BUFS * BN * TL::LD;
+  float* eb = reinterpret_cast<float*>(vt + BUFS * BN * TL::LD);
+  const int np = a.pos.n + 2 * PAD;
+  float* sums = eb + np;  // [NW][np]: the table's sums by slot, one copy for each wave
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
+  const int tile = q_tiles - 1 - int(wg % q_tiles);
+  const int h = int(wg / q_tiles) % a.H, b = int(wg / q_tiles) / a.H, hk = h / (a.H / a.Hk);
+  const int qw = tile * (NW * 32) + wave * 32;
+  const int q = qw + col, qc = min(q, a.Lq - 1), s0 = a.start(b), len = a.keys(b);
+  const int qpos = s0 + q, cq = s0 + a.pos.code(qc);
+  const uint8_t* mask = a.mask_of(b, h);
+  const float c = a.scale * LOG2E;
+
+  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, a.pos, tid, NT);
+  if (TABLE)
+    for (int t = tid; t < NW * np; t += NT) sums[t] = 0.0f;
+  float* mine = sums + wave * np;
+  float far_lo = 0.0f, far_hi = 0.0f;
+
+  typename M::V8 qf[CH], gf[CH];
+  const T* qrow = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h + qc * a.qs.t;
+  const T* grow = static_cast<const T*>(g.dout) + b * g.gs.b + h * g.gs.h + qc * g.gs.t;
+  const T* orow = static_cast<const T*>(g.out) + b * g.os.b + h * g.os.h + qc * g.os.t;
+  const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.Lq + qc;
+  // a row that sees no key: its weights are 2^(s - inf) = 0 whatever dout holds
+  const float lse = g.lse[row];
+  const bool on = q < a.Lq && lse != INF;
+  // D_i by the matrix instructions, in the order that dout V^T is summed in (the
+  // diagonal of dout out^T): a row that sees one key has out = v, and dS exactly 0
+  f32x16 dd;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) dd[r] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    qf[i] = load8<T>(qrow, 16 * i + 8 * hh, a.D, a.vec, on);
+    gf[i] = load8<T>(grow, 16 * i + 8 * hh, a.D, a.vec, on);
+    dd = M::mma(load8<T>(orow, 16 * i + 8 * hh, a.D, a.vec, on), gf[i], dd);
+  }
+  float dsum = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (8 * (r / 4) + 4 * hh + r % 4 == col) dsum = dd[r];
+  dsum = both_sum(dsum);
+  if (q < a.Lq && hh == 0) g.dsum[row] = dsum;
+
+  f32x16 dq[OB];
+#pragma unroll
+  for (int i = 0; i < OB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[i][r] = 0.0f;
+
+  int end = len;
+  if (a.causal) {
+    const int64_t last = int64_t(s0) + min(tile * (NW * 32) + NW * 32, a.Lq);
+    end = static_cast<int>(max<int64_t>(0, min<int64_t>(end, last)));
+  }
+  const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
+  const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
+  TileLoad<T, DP, BN, NT> kl, vl;
+  const int tiles = (end + BN - 1) / BN;
+  if (tiles > 0) {
+    kl.load(kb, a.ks.t, 0, len, a.D, a.vec, tid);
+    vl.load(vb, a.vs.t, 0, len, a.D, a.vec, tid);
+    kl.store(kt, tid);
+    vl.store(vt, tid);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    __syncthreads();
+    const T* kk = kt + (t % BUFS) * BN * TL::LD;
+    const T* vv = vt + (t % BUFS) * BN * TL::LD;
+    const bool more = t + 1 < tiles;
+    if (more) {
+      kl.load(kb, a.ks.t, (t + 1) * BN, len, a.D, a.vec, tid);
+      vl.load(vb, a.vs.t, (t + 1) * BN, len, a.D, a.vec, tid);
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int k0 = t * BN + nb * 32;
+      const bool hidden = a.causal && k0 > s0 + qw + 31;  // nothing for this wave
+      if (hidden || k0 >= len) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        s = M::mma(TL::straight(kk, nb * 32 + col, 16 * i + 8 * hh), qf[i], s);
+        dp = M::mma(TL::straight(vv, nb * 32 + col, 16 * i + 8 * hh), gf[i], dp);
+      }
+      const bool partial = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
+      int kind = NEAR;
+      int slot[16];  // of each pair, where it has one of its own
+      if (a.pos.grid_w == 0) {
+        kind = block_kind(a.pos, s0 + qw - (k0 + 31), s0 + qw + 31 - k0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          slot[r] = s0 + q - k0 - 4 * hh - a.pos.lo + PAD - (8 * (r / 4) + r % 4);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = min(k0 + 4 * hh + 8 * (r / 4) + r % 4, a.Lk - 1);
+          slot[r] = cq - a.pos.code(key) - a.pos.lo + PAD;
+        }
+      }
+      if (kind == NEAR) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + eb[slot[r]];
+      } else {
+        const float e = kind == ALL_BELOW ? eb[0] : eb[np - 1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + e;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(s[r] - lse);
+        s[r] = p * (dp[r] - dsum);
+      }
+      if (partial) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + 4 * hh + 8 * (r / 4) + r % 4;
+          bool seen = key < len && (!a.causal || key <= qpos);
+          if (mask && seen) seen = mask[qc * a.mq + key * a.mk] != 0;
+          if (!seen) s[r] = 0.0f;
+        }
+      }
+      if (TABLE) {
+        if (kind == NEAR) {
+          // within one half of the lanes one key meets 32 queries: 32 slots.  The
+          // halves add one after the other, so the order of every slot's sum is fixed.
+          if (hh == 0) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (q < a.Lq) unsafeAtomicAdd(mine + slot[r], s[r]);
+          }
+          __builtin_amdgcn_wave_barrier();
+          if (hh == 1) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (q < a.Lq) unsafeAtomicAdd(mine + slot[r], s[r]);
+          }
+          __builtin_amdgcn_wave_barrier();
+        } else {
+          float acc = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc += s[r];
+          acc = q < a.Lq ? acc : 0.0f;
+          if (kind == ALL_BELOW) far_lo += acc;
+          else far_hi += acc;
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        typename M::V8 ds;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ds[i] = T(s[8 * half + i]);
+#pragma unroll
+        for (int i = 0; i < OB; ++i) {
+          typename M::V8 kf = TL::transposed(kk, nb * 32 + 16 * half, 32 * i, lane);
+          if (partial) kf = finite<T>(kf);
+          dq[i] = M::mma(kf, ds, dq[i]);
+        }
+      }
+    }
+    if (more) {
+      if (BUFS == 1) __syncthreads();
+      kl.store(kt + ((t + 1) % BUFS) * BN * TL::LD, tid);
+      vl.store(vt + ((t + 1) % BUFS) * BN * TL::LD, tid);
+    }
+  }
+  if (q < a.Lq) {
+    T* drow = static_cast<T*>(g.dq) + b * g.dqs.b + h * g.dqs.h + q * g.dqs.t;
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = dq[i][4 * e4 + e] * a.scale;
+        store4<T>(drow, 32 * i + 8 * e4 + 4 * hh, a.D, g.dqvec, w);
+      }
+  }
+  if (TABLE) {
+    // what the padding holds belongs to the ends
+    far_lo += mine[lane];  // slots 0 .. PAD - 1
+    far_hi += mine[a.pos.n + PAD + lane];
+    far_lo = wave_sum(far_lo);
+    far_hi = wave_sum(far_hi);
+    if (lane == 0) {
+      mine[PAD] += far_lo;
+      mine[PAD + a.pos.n - 1] += far_hi;
+    }
+    __syncthreads();
+    float* dst = g.parts + (static_cast<int64_t>(h) * a.B * q_tiles + b * q_tiles + tile) * a.pos.n;
+    for (int t = tid; t < a.pos.n; t += NT) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) v += sums[w * np + PAD + t];
+      dst[t] = v;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dK and dV
+// ---------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads g, int k_tiles) {
+  using M = Mat<T>;
+  using TL = Tile<T, DP>;
+  constexpr int BM = Shape<T, DP>::BN, NB = BM / 32, CH = DP / 16, OB = DP / 32;
+  constexpr int BUFS = Shape<T, DP>::BUFS;
+  extern __shared__ __align__(16) unsigned char smem[];
+  T* qt = reinterpret_cast<T*>(smem);
+  T* gt = qt + BUFS * BM * TL::LD;
+  float* eb = reinterpret_cast<float*>(gt + BUFS * BM * TL::LD);
+  const int np = a.pos.n + 2 * PAD;
+  float* ls = eb + (np + 3) / 4 * 4;  // [2][BM]: each query's log-sum
+  float* dd = ls + 2 * BM;            // [2][BM]: and D_i
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
+  const int tile = int(wg % k_tiles), hk = int(wg / k_tiles) % a.Hk, b = int(wg / k_tiles) / a.Hk;
+  const int group = a.H / a.Hk;
+  const int kw = tile * (NW * 32) + wave * 32;  // the wave's first key
+  const int key = kw + col, kc = min(key, a.Lk - 1), s0 = a.start(b), len = a.keys(b);
+  const int ck = a.pos.code(kc);
+  const float c = a.scale * LOG2E;
+  const int k_first = tile * (NW * 32);
+
+  typename M::V8 kf[CH], vf[CH];
+  const T* krow = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + kc * a.ks.t;
+  const T* vrow = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h + kc * a.vs.t;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    kf[i] = load8<T>(krow, 16 * i + 8 * hh, a.D, a.vec, key < len);
+    vf[i] = load8<T>(vrow, 16 * i + 8 * hh, a.D, a.vec, key < len);
+  }
+  f32x16 dk[OB], dv[OB];
+#pragma unroll
+  for (int i = 0; i < OB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.0f;
+
+  // queries that see any key of the workgroup: from `first` on
+  int first = 0;
+  if (a.causal) {
+    const int64_t f = static_cast<int64_t>(k_first) - s0;
+    first = static_cast<int>(max<int64_t>(0, min<int64_t>(f, a.Lq)));
+  }
+  const int t0 = first / BM;
+  const int tiles = k_first < len ? (a.Lq + BM - 1) / BM : 0;
+  TileLoad<T, DP, BM, NT> ql, gl;
+  float lse_r = 0.0f, d_r = 0.0f;
+  float row_lse[TileLoad<T, DP, BM, NT>::N];  // of the rows that this thread brings
+
+  for (int hg = 0; hg < group; ++hg) {
+    const int h = hk * group + hg;
+    const uint8_t* mask = a.mask_of(b, h);
+    const T* qb = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h;
+    const T* gb = static_cast<const T*>(g.dout) + b * g.gs.b + h * g.gs.h;
+    const int64_t row0 = (static_cast<int64_t>(b) * a.H + h) * a.Lq;
+    auto load = [&](int t) {
+      ql.load(qb, a.qs.t, t * BM, a.Lq, a.D, a.vec, tid);
+      gl.load(gb, g.gs.t, t * BM, a.Lq, a.D, a.vec, tid);
+#pragma unroll
+      for (int i = 0; i < ql.N; ++i) {
+        const int r = t * BM + (tid + i * NT) / ql.PER_ROW;
+        row_lse[i] = r < a.Lq ? g.lse[row0 + r] : INF;
+      }
+      if (tid < BM) {
+        const int i = t * BM + tid;
+        lse_r = i < a.Lq ? g.lse[row0 + i] : INF;
+        d_r = i < a.Lq ? g.dsum[row0 + i] : 0.0f;
+      }
+    };
+    auto store = [&](int t) {
+      // a query that sees no key may hold anything, and 0 x anything has to be 0
+#pragma unroll
+      for (int i = 0; i < ql.N; ++i)
+        if (row_lse[i] == INF)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ql.r[i][e] = gl.r[i][e] = T(0);
+      ql.store(qt + (t % BUFS) * BM * TL::LD, tid);
+      gl.store(gt + (t % BUFS) * BM * TL::LD, tid);
+      if (tid < BM) {
+        ls[(t & 1) * BM + tid] = lse_r;
+        dd[(t & 1) * BM + tid] = d_r;
+      }
+    };
+    __syncthreads();  // the head before is done with its tiles and bias
+    load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, a.pos, tid, NT);
+    if (t0 < tiles) {
+      load(t0);
+      store(t0);
+    }
+    for (int t = t0; t < tiles; ++t) {
+      __syncthreads();
+      const T* qq = qt + (t % BUFS) * BM * TL::LD;
+      const T* gg = gt + (t % BUFS) * BM * TL::LD;
+      const float* lt = ls + (t & 1) * BM;
+      const float* dt = dd + (t & 1) * BM;
+      const bool more = t + 1 < tiles;
+      if (more) load(t + 1);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int i0 = t * BM + nb * 32;  // the block's first query
+        if ((a.causal && s0 + i0 + 31 < kw) || kw >= len || i0 >= a.Lq) continue;
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          s = M::mma(TL::straight(qq, nb * 32 + col, 16 * i + 8 * hh), kf[i], s);
+          dp = M::mma(TL::straight(gg, nb * 32 + col, 16 * i + 8 * hh), vf[i], dp);
+        }
+        const bool partial = mask || kw + 32 > len || (a.causal && kw + 31 > s0 + i0);
+        int kind = NEAR;
+        if (a.pos.grid_w == 0) {
+          kind = block_kind(a.pos, s0 + i0 - (kw + 31), s0 + i0 + 31 - kw);
+          if (kind == NEAR) {
+            const float* e = eb + (s0 + i0 + 4 * hh - key - a.pos.lo + PAD);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = s[r] * c + e[8 * (r / 4) + r % 4];
+          } else {
+            const float e = kind == ALL_BELOW ? eb[0] : eb[np - 1];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = s[r] * c + e;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = min(i0 + 4 * hh + 8 * (r / 4) + r % 4, a.Lq - 1);
+            s[r] = s[r] * c + eb[a.pos.code(i) - ck - a.pos.lo + PAD];
+          }
+        }
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(lt + nb * 32 + 8 * r4 + 4 * hh);
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(dt + nb * 32 + 8 * r4 + 4 * hh);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * r4 + e;
+            // a row with a log-sum of +inf sees no key, whatever its query holds
+            const float p = l4[e] == INF ? 0.0f : __builtin_amdgcn_exp2f(s[r] - l4[e]);
+            s[r] = p;
+            dp[r] = l4[e] == INF ? 0.0f : p * (dp[r] - d4[e]);
+          }
+        }
+        if (partial) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = i0 + 4 * hh + 8 * (r / 4) + r % 4;
+            bool seen = key < len && (!a.causal || key <= s0 + i);
+            if (mask && seen && i < a.Lq) seen = mask[i * a.mq + key * a.mk] != 0;
+            if (!seen) s[r] = dp[r] = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          typename M::V8 p, ds;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            p[i] = T(s[8 * half + i]);
+            ds[i] = T(dp[8 * half + i]);
+          }
+#pragma unroll
+          for (int i = 0; i < OB; ++i) {
+            typename M::V8 gf = TL::transposed(gg, nb * 32 + 16 * half, 32 * i, lane);
+            typename M::V8 qf = TL::transposed(qq, nb * 32 + 16 * half, 32 * i, lane);
+            dv[i] = M::mma(gf, p, dv[i]);
+            dk[i] = M::mma(qf, ds, dk[i]);
+          }
+        }
+      }
+      if (more) {
+        if (BUFS == 1) __syncthreads();
+        store(t + 1);
+      }
+    }
+  }
+  if (key < a.Lk) {
+    T* krow_o = static_cast<T*>(g.dk) + b * g.dks.b + hk * g.dks.h + key * g.dks.t;
+    T* vrow_o = static_cast<T*>(g.dv) + b * g.dvs.b + hk * g.dvs.h + key * g.dvs.t;
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        float w[4], x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = dk[i][4 * e4 + e] * a.scale;
+          x[e] = dv[i][4 * e4 + e];
+        }
+        store4<T>(krow_o, 32 * i + 8 * e4 + 4 * hh, a.D, g.dkvec, w);
+        store4<T>(vrow_o, 32 * i + 8 * e4 + 4 * hh, a.D, g.dkvec, x);
+      }
+  }
+}
+
+inline int tiles_of(int n) { return (n + NW * 32 - 1) / (NW * 32); }
+
+template <typename T, int DP>
+int launch_dim(const RelAttn& a, const Grads& g, hipStream_t s) {
+  const int qt = tiles_of(a.Lq), kt = tiles_of(a.Lk);
+  const int64_t wq = static_cast<int64_t>(a.B) * a.H * qt, wk = static_cast<int64_t>(a.B) * a.Hk * kt;
+  if (wq > 0x7fffffff || wk > 0x7fffffff) return FA_E_SHAPE;
+  const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
+  const size_t lds_q = tiles + (g.parts ? 1 + NW : 1) * np * sizeof(float);
+  const size_t lds_k = tiles + ((np + 3) / 4 * 4 + 4 * Shape<T, DP>::BN) * sizeof(float);
+  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, true> : rel_attention_dq_kernel<T, DP, false>;
+  auto dkv = rel_attention_dkv_kernel<T, DP>;
+  if (const int e = launch_lds(dq, lds_q)) return e;
+  if (const int e = launch_lds(dkv, lds_k)) return e;
+  dq<<<static_cast<unsigned>(wq), NT, lds_q, s>>>(a, g, qt);
+  FA_LAUNCH_CHECK();
+  dkv<<<static_cast<unsigned>(wk), NT, lds_k, s>>>(a, g, kt);
+  FA_LAUNCH_CHECK();
+  return FA_OK;
+}
+
+template <typename T>
+int backward(RelAttn a, Grads g, int rows, void* dtable, hipStream_t s) {
+  const void* in[5] = {a.q, a.k, a.v, g.out, g.dout};
+  const View iv[5] = {a.qs, a.ks, a.vs, g.os, g.gs};
+  a.vec = widest_load<T>(in, iv, 5, a.D);
+  const void* dqp[1] = {g.dq};
+  g.dqvec = widest_load<T>(dqp, &g.dqs, 1, a.D);
+  const void* dkp[2] = {g.dk, g.dv};
+  const View dkv[2] = {g.dks, g.dvs};
+  g.dkvec = widest_load<T>(dkp, dkv, 2, a.D);
+  int e;
+  if (a.D <= 32) e = launch_dim<T, 32>(a, g, s);
+  else if (a.D <= 64) e = launch_dim<T, 64>(a, g, s);
+  else e = launch_dim<T, 128>(a, g, s);
+  if (e) return e;
+  if (dtable) {
+    launch_table_sum<T>(g.parts, a.B * tiles_of(a.Lq), a.pos.n, a.pos.row_of, rows, a.H,
+                        static_cast<T*>(dtable), s);
+    FA_LAUNCH_CHECK();
+  }
+  return FA_OK;
+}
+
+inline int64_t align16(int64_t v) { return (v + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace fa
+
+extern "C" {
+
+FA_API int fa_gpu_rel_attention_backward_workspace(int B, int H, int Lq, int n, int need_table,
+                                                   int64_t* out_bytes) {
+  if (!out_bytes) return FA_E_ARG;
+  if (n < 1 || n > FA_REL_MAX) return FA_E_SHAPE;
+  if (const int e = fa::check_attention(B, H, H, Lq, 1, 1, nullptr, 1, nullptr)) return e;
+  const int64_t bh = static_cast<int64_t>(B) * H;
+  *out_bytes = fa::align16(bh * Lq * 4) + (need_table ? bh * fa::tiles_of(Lq) * n * 4 : 0);
+  return FA_OK;
+}
+
+FA_API int fa_gpu_rel_attention_backward(
+    const void* q, const void* k, const void* v, const void* out, const void* dout,
+    const float* lse, int dtype, int B, int H, int Hk, int Lq, int Lk, int D,
+    const int64_t* strides, const void* table, int rows, const int* row_of, int lo, int n,
+    int grid_w, int64_t q_start, const int* q_starts, const int* key_lengths, const uint8_t* mask,
+    int mask_b, const int64_t* mask_strides, int causal, double scale, void* dq, void* dk,
+    void* dv, void* dtable, void* workspace, int64_t workspace_bytes, int device, void* stream) {
+  using namespace fa;
+  if (!q || !k || !v || !out || !dout || !lse || !strides || !table || !dq || !dk || !dv ||
+      !workspace)
+    return FA_E_ARG;
+  if (const int e = check_attention(B, H, Hk, Lq, Lk, D, mask, mask_b, mask_strides)) return e;
+  if (const int e = check_relpos(row_of, rows, lo, n, grid_w, Lq, Lk, q_start, q_starts)) return e;
+  int64_t need = 0;
+  if (const int e = fa_gpu_rel_attention_backward_workspace(B, H, Lq, n, dtable != nullptr, &need))
+    return e;
+  if (workspace_bytes < need) return FA_E_ARG;
+  DeviceScope scope(device);
+  if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
+  const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table,
+                                  RelPos{row_of, lo, n, grid_w}, q_start, q_starts, key_lengths,
+                                  mask, mask_b, mask_strides, causal, scale);
+  Grads g{};
+  g.out = out;
+  g.dout = dout;
+  g.os = {strides[9], strides[10], strides[11]};
+  g.gs = {strides[12], strides[13], strides[14]};
+  g.dqs = {strides[15], strides[16], strides[17]};
+  g.dks = {strides[18], strides[19], strides[20]};
+  g.dvs = {strides[21], strides[22], strides[23]};
+  g.lse = lse;
+  g.dsum = static_cast<float*>(workspace);
+  g.parts = dtable ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                              align16(static_cast<int64_t>(B) * H * Lq * 4))
+                   : nullptr;
+  g.dq = dq;
+  g.dk = dk;
+  g.dv = dv;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case FA_F16: return backward<_Float16>(a, g, rows, dtable, s);
+    case FA_BF16: return backward<__bf16>(a, g, rows, dtable, s);
+    case FA_F32: return backward<float>(a, g, rows, dtable, s);
+    default: return FA_E_DTYPE;
+  }
+}
+
+}  // extern "C"

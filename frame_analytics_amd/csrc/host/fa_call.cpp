@@ -25,6 +25,7 @@
 #include <utility>
 
 #include "fa_abi.h"
+#include "fa_train_abi.h"
 
 namespace {
 
@@ -154,6 +155,9 @@ const Known KNOWN[] = {
     FA_ENTRY(fa_gpu_ms_ssim),           FA_ENTRY(fa_gpu_ms_ssim_head),
     FA_ENTRY(fa_gpu_ms_ssim_head_backward), FA_ENTRY(fa_gpu_gmsd_ex),
     FA_ENTRY(fa_gpu_gmsd_once),         FA_ENTRY(fa_gpu_gmsd_backward),
+    FA_ENTRY(fa_gpu_rel_bias),          FA_ENTRY(fa_gpu_rel_bias_backward),
+    FA_ENTRY(fa_gpu_rel_attention),     FA_ENTRY(fa_gpu_rel_attention_backward),
+    FA_ENTRY(fa_gpu_orthogonalize),
 };
 
 void entry_dealloc(PyObject* self) { Py_TYPE(self)->tp_free(self); }

@@ -1,0 +1,424 @@
+"""The training operators' kernels against float64, on the GPU.
+
+Tolerances, set from the arithmetic.  float32: sums of n terms in float32 are off by at
+most n 2^-24 of the sum of magnitudes; the longest here (keys plus head dimension) give
+2e-5 of the result's norm.  16-bit types (unit roundoff u = 2^-9 for bfloat16, 2^-12
+... 2^-11 relative spacing for float16): the output rounds once and the weights once, 2
+u; gradients round the weights, dS, and themselves, and read an output rounded once,
+4 u.  The largest single error may be 8 times as much of the largest value."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import frame_analytics_amd as fa
+from oracle import training as ref
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+UNIT = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 1e-5}
+STEEP, POLAR = (3.4445, -4.7750, 2.0315), (1.875, -1.25, 0.375)
+
+
+def near(got, want, tol, what=""):
+    got = got.detach().double().cpu().numpy()
+    assert got.shape == want.shape, what
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    norm, top = np.linalg.norm(want), np.abs(want).max(initial=0.0)
+    err = np.abs(got - want)
+    assert np.linalg.norm(got - want) <= tol * norm, (what, np.linalg.norm(got - want) / norm)
+    assert err.max(initial=0.0) <= 8 * tol * top, (what, err.max() / top)
+
+
+def normal(gen, dt, *shape):
+    return torch.randn(*shape, generator=gen).to(dt)
+
+
+def attention_case(dt, b, h, hk, lq, lk, d, pos, rows, *, scale=None, tokens_first=True, seed=0,
+                   q_start=0, **kw):
+    gen = torch.Generator().manual_seed(seed)
+
+    def make(heads, n):
+        if tokens_first:
+            return normal(gen, dt, b, n, heads, d).transpose(1, 2)
+        return normal(gen, dt, b, heads, n, d)
+
+    q, k, v, g = make(h, lq), make(hk, lk), make(hk, lk), make(h, lq)
+    table = (0.7 * torch.randn(pos.rows, h, generator=gen)).to(dt)
+    see = ref.visible(b, h, lq, lk, causal=kw.get("causal", False),
+                      mask=None if kw.get("mask") is None else kw["mask"].cpu().numpy(),
+                      key_lengths=None if kw.get("key_lengths") is None
+                      else kw["key_lengths"].cpu().numpy(),
+                      q_start=q_start.cpu().numpy() if torch.is_tensor(q_start) else q_start)
+    s = d ** -0.5 if scale is None else scale
+    want = ref.attention(*(t.double().numpy() for t in (q, k, v, table)), rows, see, s,
+                         g.double().numpy())
+    return (q, k, v, table), g, want
+
+
+def run_attention(tensors, g, pos, scale=None, **kw):
+    ts = [t.cuda().requires_grad_(True) for t in tensors]
+    out = fa.relative_attention(*ts, pos, scale=scale, **kw)
+    out.backward(g.cuda())
+    return (out, *(t.grad for t in ts))
+
+
+def check_attention(dt, b, h, hk, lq, lk, d, pos, rows, scale=None, tokens_first=True, seed=0, **kw):
+    tensors, g, want = attention_case(DT[dt], b, h, hk, lq, lk, d, pos, rows, scale=scale,
+                                      tokens_first=tokens_first, seed=seed, **kw)
+    got = run_attention(tensors, g, pos, scale, **kw)
+    u = UNIT[dt]
+    for name, x, y, t in zip(("out", "dq", "dk", "dv", "dtable"), got, want, (2, 4, 4, 4, 4)):
+        near(x, y, t * u / (1 if dt == "f32" else 2), name)
+    with torch.no_grad():  # without gradients: the form that serves
+        only = fa.relative_attention(*(t.cuda() for t in tensors), pos, scale=scale, **kw)
+    near(only, want[0], 2 * u / (1 if dt == "f32" else 2), "out, no gradients")
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("lq,lk,d", [(1, 1, 1), (1, 70, 33), (5, 3, 7), (31, 33, 64), (64, 64, 30),
+                                     (65, 129, 128), (130, 257, 40), (200, 47, 96)])
+def test_attention_on_a_line(gpu, dt, lq, lk, d):
+    pos = fa.LinePositions(8, 20)
+    check_attention(dt, 2, 4, 2, lq, lk, d, pos, ref.line_rows(lq, lk, 0, 8, 20), seed=lq + d)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("start", [0, 3, 150])
+def test_causal(gpu, dt, start):
+    lq, lk = 150, 173
+    pos = fa.LinePositions(16, 40, bidirectional=False)
+    rows = ref.line_rows(lq, lk, start, 16, 40, False)
+    check_attention(dt, 2, 3, 3, lq, lk, 64, pos, rows, causal=True, q_start=start)
+
+
+def test_causal_rows_before_the_first_key_see_nothing(gpu):
+    pos = fa.LinePositions(16, 40)
+    check_attention("f32", 1, 2, 1, 90, 80, 32, pos, ref.line_rows(90, 80, -50, 16, 40),
+                    causal=True, q_start=-50)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("h,w,d", [(1, 1, 16), (4, 4, 30), (7, 5, 24), (8, 8, 32), (16, 16, 64),
+                                   (3, 40, 100)])
+def test_windows(gpu, dt, h, w, d):
+    n = h * w
+    check_attention(dt, 3, 2, 2, n, n, d, fa.GridPositions(h, w), ref.grid_rows(h, w), seed=n)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("heads", [1, 4])
+def test_masks_with_empty_rows(gpu, dt, heads):
+    gen = torch.Generator().manual_seed(5)
+    b, h, n = 6, 4, 64
+    mask = torch.rand(3, heads, n, n, generator=gen) < 0.4
+    mask[0, :, 5] = False           # a query that sees nothing
+    mask[1, :, :, 7] = False        # a key that nothing sees
+    mask[2] = False                 # a whole entry
+    check_attention(dt, b, h, 2, n, n, 32, fa.GridPositions(8, 8), ref.grid_rows(8, 8),
+                    mask=mask.cuda())
+
+
+def test_mask_of_two_dimensions_any_strides(gpu):
+    gen = torch.Generator().manual_seed(6)
+    mask = (torch.rand(50, 70, generator=gen) < 0.5).cuda().t()
+    pos = fa.LinePositions(8, 20)
+    check_attention("bf16", 2, 2, 2, 70, 50, 64, pos, ref.line_rows(70, 50, 0, 8, 20), mask=mask)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_key_lengths(gpu, dt, kind):
+    lens = torch.tensor([0, 1, 64, 100, 177, 500], dtype=kind).cuda()  # the last: past the end
+    pos = fa.LinePositions(32, 128)
+    rows = ref.line_rows(90, 177)
+    check_attention(dt, 6, 2, 1, 90, 177, 40, pos, rows, key_lengths=lens)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("h,hk,d,lk", [(4, 4, 64, 1), (8, 2, 128, 700), (6, 1, 80, 333),
+                                       (16, 4, 128, 2500), (3, 3, 7, 1025)])
+def test_single_tokens(gpu, dt, h, hk, d, lk):
+    b = 5
+    lens = torch.tensor([lk, 0, 1, (lk + 1) // 2, max(1, lk - 1)], dtype=torch.int32)
+    start = (lens - 1).clamp_min(0)
+    pos = fa.LinePositions(32, 128, bidirectional=False)
+    rows = np.stack([ref.line_rows(1, lk, int(s), 32, 128, False) for s in start])
+    check_attention(dt, b, h, hk, 1, lk, d, pos, rows, key_lengths=lens.cuda(),
+                    q_start=start.cuda())
+
+
+@pytest.mark.parametrize("lq", [2, 7, 16, 33])
+def test_few_queries_against_a_long_cache(gpu, lq):
+    lk = 1500
+    pos = fa.LinePositions(32, 128, bidirectional=False)
+    rows = ref.line_rows(lq, lk, lk - lq, 32, 128, False)
+    check_attention("bf16", 2, 8, 2, lq, lk, 64, pos, rows, causal=True, q_start=lk - lq)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_strides_and_alignment(gpu, dt):
+    """Heads first, a cut out of a wider projection, an odd offset, a last dimension
+    that is not contiguous, a broadcast batch: the same as their copies."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    b, n, h, d = 2, 70, 2, 32
+    wide = torch.randn(b, n, 3, h, d + 1, generator=gen, device="cuda").to(DT[dt])
+    pos = fa.LinePositions(8, 20)
+    table = torch.randn(8, h, generator=gen, device="cuda").to(DT[dt])
+    q, k, v = (wide[:, :, i, :, 1:].transpose(1, 2) for i in range(3))
+    flipped = q.transpose(2, 3).contiguous().transpose(2, 3)
+    want = fa.relative_attention(q.contiguous(), k.contiguous(), v.contiguous(), table, pos)
+    assert torch.equal(fa.relative_attention(q, k, v, table, pos), want)
+    assert torch.equal(fa.relative_attention(flipped, k, v, table, pos), want)
+    one = [t[:1].contiguous().requires_grad_(True) for t in (k, v)]
+    kb, vb = (t.expand(b, -1, -1, -1) for t in one)
+    out = fa.relative_attention(q, kb, vb, table, pos)
+    full = [t.detach().contiguous().requires_grad_(True) for t in (kb, vb)]
+    same = fa.relative_attention(q, *full, table, pos)
+    assert torch.equal(out, same)
+    g = torch.randn(out.shape, generator=gen, device="cuda").to(out.dtype)
+    out.backward(g)
+    same.backward(g)
+    for x, y in zip(one, full):
+        near(x.grad, y.grad.double().sum(0, keepdim=True).cpu().numpy(), 2 * UNIT[dt])
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_what_no_query_sees_may_hold_anything(gpu, dt):
+    """NaN and infinities past key_lengths, at keys later than every query, and in
+    queries that see nothing reach no result."""
+    b, h, n, d = 2, 2, 100, 32
+    lens = torch.tensor([40, 77], dtype=torch.int32)
+    pos = fa.LinePositions(8, 20)
+    rows = ref.line_rows(n, n, 0, 8, 20)
+    tensors, g, want = attention_case(DT[dt], b, h, h, n, n, d, pos, rows, key_lengths=lens)
+    q, k, v, table = tensors
+    for i, m in enumerate(lens.tolist()):
+        k[i, :, m:] = float("nan")
+        v[i, :, m:] = float("inf")
+    got = run_attention(tensors, g, pos, key_lengths=lens.cuda())
+    for x, y, t in zip(got, want, (2, 4, 4, 4, 4)):
+        near(x, y, t * UNIT[dt])
+    # the future of a causal line, and a masked-out query
+    mask = torch.ones(n, n, dtype=torch.bool)
+    mask[10] = False
+    mask[:, 50] = False
+    tensors, g, want = attention_case(DT[dt], b, h, h, n, n, d, pos, rows, mask=mask)
+    q, k, v, table = tensors
+    q[:, :, 10] = float("nan")
+    g[:, :, 10] = float("nan")
+    k[:, :, 50] = float("nan")
+    v[:, :, 50] = -float("inf")
+    got = run_attention(tensors, g, pos, mask=mask.cuda())
+    for x, y, t in zip(got, want, (2, 4, 4, 4, 4)):
+        near(x, y, t * UNIT[dt])
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_a_value_that_is_not_finite_stays_with_who_sees_it(gpu, dt, bad):
+    n = 80
+    gen = torch.Generator().manual_seed(2)
+    q, k, v = (normal(gen, DT[dt], 1, 1, n, 32).cuda() for _ in range(3))
+    table = torch.zeros(8, 1, dtype=DT[dt], device="cuda")
+    pos = fa.LinePositions(8, 20)
+    clean = fa.relative_attention(q, k, v, table, pos, causal=True)
+    v[0, 0, 45, 3] = bad
+    out = fa.relative_attention(q, k, v, table, pos, causal=True)
+    keep = torch.ones(n, 32, dtype=torch.bool, device="cuda")
+    keep[45:, 3] = False
+    assert torch.equal(out[0, 0][keep], clean[0, 0][keep])
+    assert not torch.isfinite(out[0, 0, 45:, 3]).any()
+    if bad == bad:
+        assert (out[0, 0, 45:, 3] == bad).all()
+
+
+def test_masks_and_scores_of_large_magnitude(gpu):
+    """A bias of the type's lowest value, scores that overflow exp, and a scale of 0."""
+    n, pos = 40, fa.LinePositions(4, 5, bidirectional=False)
+    rows = ref.line_rows(n, n, 0, 4, 5, False)
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (normal(gen, torch.float32, 1, 2, n, 16) for _ in range(3))
+    table = torch.zeros(4, 2)
+    table[2, 0] = torch.finfo(torch.float32).min / 4
+    table[1, 1] = 3.0e4
+    for scale in (0.0, 0.25, 200.0):
+        see = ref.visible(1, 2, n, n)
+        want = ref.attention(q.numpy(), k.numpy(), v.numpy(), table.numpy(), rows, see, scale)
+        got = fa.relative_attention(q.cuda(), k.cuda(), v.cuda(), table.cuda(), pos, scale=scale)
+        # scores near 3e4 carry 3e4 2^-24 of error into the exponent
+        near(got, want, 2e-5 + 2 * 3.0e4 * 2.0 ** -23)
+
+
+def test_no_pairs(gpu):
+    pos = fa.LinePositions(8, 20)
+    table = torch.randn(8, 2, device="cuda", requires_grad=True)
+    q = torch.randn(2, 2, 5, 8, device="cuda", requires_grad=True)
+    k = torch.randn(2, 2, 0, 8, device="cuda", requires_grad=True)
+    out = fa.relative_attention(q, k, k, table, pos)
+    assert torch.equal(out, torch.zeros_like(q))
+    out.sum().backward()
+    assert torch.equal(q.grad, torch.zeros_like(q)) and k.grad.shape == k.shape
+    assert fa.relative_attention(q[:0], k[:0], k[:0], table, pos).shape == (0, 2, 5, 8)
+    assert fa.relative_bias(table, pos, 3).shape == (2, 3, 3)  # (a kernel ran in this test)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_same_bits_from_run_to_run_and_from_stream_to_stream(gpu, dt):
+    pos = fa.GridPositions(8, 8)
+    tensors, g, _ = attention_case(DT[dt], 40, 4, 4, 64, 64, 32, pos, ref.grid_rows(8, 8))
+    first = [t.clone() for t in run_attention(tensors, g, pos)]
+    side = torch.cuda.Stream()
+    for i in range(4):
+        if i % 2:
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                again = run_attention(tensors, g, pos)
+            side.synchronize()
+        else:
+            again = run_attention(tensors, g, pos)
+        assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+def test_gradients_against_differences(gpu):
+    """Of a fixed direction, by central differences of the float32 kernel itself."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    pos = fa.LinePositions(8, 20)
+
+    def rnd(*s):
+        return torch.randn(*s, generator=gen, device="cuda")
+
+    base = [rnd(1, 2, 40, 16), rnd(1, 1, 50, 16), rnd(1, 1, 50, 16), rnd(8, 2)]
+    up = rnd(1, 2, 40, 16)
+    f = lambda ts: (fa.relative_attention(*ts, pos, causal=True, q_start=9).double()  # noqa: E731
+                    * up.double()).sum().item()
+    ts = [t.clone().requires_grad_(True) for t in base]
+    fa.relative_attention(*ts, pos, causal=True, q_start=9).backward(up)
+    for i in range(4):
+        way, eps = rnd(*base[i].shape), 1e-2
+        ahead, behind = ([t + (s * eps * way if i == j else 0) for j, t in enumerate(base)]
+                         for s in (1, -1))
+        slope = (f(ahead) - f(behind)) / (2 * eps)
+        want = (ts[i].grad.double() * way.double()).sum().item()
+        # differences of eps: eps^2 of the third derivative, and 2^-24 / eps
+        assert abs(slope - want) <= 1e-3 * (1 + abs(want)), (i, slope, want)
+
+
+def test_captured_in_a_graph(gpu):
+    pos = fa.LinePositions(32, 128, bidirectional=False)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (torch.randn(2, 4, n, 64, generator=gen, device="cuda").bfloat16()
+               for n in (1, 900, 900))
+    table = torch.randn(32, 4, generator=gen, device="cuda").bfloat16()
+    lens = torch.tensor([900, 300], dtype=torch.int32, device="cuda")
+    w = torch.randn(3, 96, 160, generator=gen, device="cuda").bfloat16()
+
+    def step():
+        return (fa.relative_attention(q, k, v, table, pos, key_lengths=lens, q_start=lens - 1),
+                fa.orthogonalize(w))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        q.copy_(torch.randn(q.shape, generator=gen, device="cuda"))
+        w.copy_(torch.randn(w.shape, generator=gen, device="cuda"))
+        lens.fill_(250 * (i + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, step()))
+
+
+# --------------------------------------------------------------------------- #
+# the bias by itself
+# --------------------------------------------------------------------------- #
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("lq,lk,start", [(1, 1, 0), (1, 50, 49), (3, 5, 0), (70, 33, -4),
+                                         (129, 300, 10), (200, 513, 0), (500, 31, 0)])
+def test_bias_on_a_line(gpu, dt, lq, lk, start):
+    pos = fa.LinePositions(8, 20)
+    rows = ref.line_rows(lq, lk, start, 8, 20)
+    check_bias(dt, pos, rows, 3, lq, lk, q_start=start)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("h,w", [(1, 1), (1, 9), (5, 6), (16, 16), (33, 33)])
+def test_bias_of_a_window(gpu, dt, h, w):
+    check_bias(dt, fa.GridPositions(h, w), ref.grid_rows(h, w), 2, h * w, h * w)
+
+
+def check_bias(dt, pos, rows, heads, lq, lk, **kw):
+    gen = torch.Generator().manual_seed(lq)
+    table = normal(gen, DT[dt], pos.rows, heads)
+    up = normal(gen, DT[dt], heads, lq, lk)
+    t = table.cuda().requires_grad_(True)
+    out = fa.relative_bias(t, pos, lq, lk, **kw)
+    assert torch.equal(out.detach().cpu(), table[torch.from_numpy(rows)].permute(2, 0, 1))
+    out.backward(up.cuda())
+    want = ref.bias_grad(up.double().numpy(), rows, pos.rows)
+    near(t.grad, want, 2 * UNIT[dt])
+    first = t.grad.clone()
+    for other in (up.cuda().transpose(1, 2).contiguous().transpose(1, 2),
+                  up.cuda()[:1].expand(heads, -1, -1)):
+        t.grad = None
+        fa.relative_bias(t, pos, lq, lk, **kw).backward(other)
+        if other.shape == up.shape and torch.equal(other.cpu(), up):
+            assert torch.equal(t.grad, first)
+        else:
+            near(t.grad, ref.bias_grad(other.double().cpu().numpy(), rows, pos.rows), 2 * UNIT[dt])
+
+
+# --------------------------------------------------------------------------- #
+# orthogonalised updates
+# --------------------------------------------------------------------------- #
+
+# before the result's rounding: bfloat16 runs float16 products (1.5e-3), the others
+# pairs of float16, 22 bits, whose errors the default coefficients multiply by 3.4445^5
+ORTHO = {"bf16": 1.5e-3 + 2.0 ** -9, "f16": 2.0 ** -11 + 3e-5, "f32": 3e-5}
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("batch,m,n", [((), 1, 1), ((2,), 1, 7), ((3,), 5, 5), ((2, 2), 64, 40),
+                                       ((2,), 130, 300), ((), 300, 130), ((1,), 257, 1000)])
+@pytest.mark.parametrize("steps,coefficients", [(5, STEEP), (6, POLAR), (1, STEEP)])
+def test_orthogonalize(gpu, dt, batch, m, n, steps, coefficients):
+    gen = torch.Generator().manual_seed(m)
+    g = (1e-3 * torch.randn(*batch, m, n, generator=gen)).to(DT[dt])
+    got = fa.orthogonalize(g.cuda(), steps=steps, coefficients=coefficients)
+    assert got.dtype == DT[dt] and got.shape == g.shape and not got.requires_grad
+    for i, x in enumerate(g.reshape(-1, m, n)):
+        want = ref.orthogonalize(x.double().numpy(), steps, coefficients)
+        near(got.reshape(-1, m, n)[i], want, ORTHO[dt], i)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_orthogonalize_edges(gpu, dt):
+    z = torch.zeros(2, 33, 70, dtype=DT[dt], device="cuda")
+    z[1, 3, 4] = 1.0
+    got = fa.orthogonalize(z)
+    assert torch.equal(got[0], z[0])           # a zero update stays zero, beside another
+    assert (got[1] != 0).sum() == 1
+    z[1, 3, 4] = float("nan")
+    got = fa.orthogonalize(z)
+    assert torch.equal(got[0], z[0]) and torch.isnan(got[1]).all()
+    top = torch.finfo(DT[dt]).max
+    big = torch.eye(40, dtype=DT[dt], device="cuda") * (top / 2)
+    near(fa.orthogonalize(big, steps=6, coefficients=POLAR),
+         ref.orthogonalize(big.double().cpu().numpy(), 6, POLAR), ORTHO[dt])
+    view = torch.randn(64, 3, 50, device="cuda").to(DT[dt]).transpose(0, 1)
+    assert torch.equal(fa.orthogonalize(view), fa.orthogonalize(view.contiguous()))
+
+
+def test_orthogonalize_tiny_and_low_rank(gpu):
+    gen = torch.Generator().manual_seed(8)
+    g = torch.randn(120, 2, generator=gen) @ torch.randn(2, 200, generator=gen)
+    for scale in (1e-4, 1e20):  # eps counts in the first
+        x = g * scale
+        near(fa.orthogonalize(x.cuda()), ref.orthogonalize(x.double().numpy(), 5, STEEP), 3e-4)

@@ -137,7 +137,7 @@ def rel_attention(q, k, v, table, plan: AttentionPlan, need_lse: bool):
     lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if need_lse else None
     dev, stream = _site(q)
     ws, n = _workspace("fa_gpu_rel_attention_workspace", q.device, b, h, hk, lq, lk, d,
-                       plan.positions.slots, int(plan.mask is not None), int(need_lse), dev)
+                       plan.positions.slots, dev)
     _run("fa_gpu_rel_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE_CODE[q.dtype],
          b, h, hk, lq, lk, d, _strides(q, k, v, out),
          *plan.tail(table, _row_of(plan.positions, q.device)), out.data_ptr(), _ptr(lse), _ptr(ws),

@@ -57,43 +57,81 @@ template <> struct Mat<float> {
   }
 };
 
-// Eight elements d .. d + 7 of a row of D, zero from D on (all zero unless `on`).
-// `vec` elements are read at once: the widest that the row's address, the strides
-// and D allow (16 bytes, 4 bytes or one element; uniform over the launch).
-template <typename T>
-__device__ inline typename Mat<T>::V8 load8(const T* row, int d, int D, int vec, bool on) {
-  typename Mat<T>::V8 r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = T(0);
-  if (vec * int(sizeof(T)) == 16) {
-    constexpr int W = 16 / sizeof(T);
-#pragma unroll
-    for (int e = 0; e < 8; e += W) {
-      if (on && d + e < D) {
-        if constexpr (W == 8) {
-          r = *reinterpret_cast<const typename Mat<T>::V8*>(row + d);
-        } else {
-          const typename Mat<T>::V4 t = *reinterpret_cast<const typename Mat<T>::V4*>(row + d + e);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[e + i] = t[i];
-        }
-      }
+// Rows of a view, read with buffer instructions: what lies outside reads as zero, so
+// edges cost a select and no branch.  `base` is the first row that the workgroup
+// reads (rows further on are reached by 32-bit byte offsets, so a view's token
+// stride times MAX_ROWS has to stay below 2^31 bytes; the base itself is 64-bit).
+constexpr int MAX_ROWS = 256;
+constexpr int OUTSIDE = static_cast<int>(0x80000000u);
+template <typename T> struct Rows {
+  __amdgpu_buffer_rsrc_t rsrc;
+  int stride;  // bytes
+  __device__ inline Rows(const T* base, int64_t stride_elements)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffff, 0x00020000)),
+        stride(static_cast<int>(stride_elements * sizeof(T))) {}
+
+  // Elements d .. d + 7 of row `row`, zero from D on (all zero unless `on`).  `vec`
+  // elements are read at once: the widest that the views' addresses, their strides and
+  // D allow (16 bytes, 4 bytes or one element; uniform over the launch).
+  __device__ inline typename Mat<T>::V8 wide(int row, int d, int D, bool on) const {
+    const int at = row * stride + d * int(sizeof(T));
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(typename Mat<T>::V8, __builtin_amdgcn_raw_buffer_load_b128(
+                                                         rsrc, on && d < D ? at : OUTSIDE, 0, 0));
+    } else {
+      const f32x4 x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    rsrc, on && d < D ? at : OUTSIDE, 0, 0));
+      const f32x4 y = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    rsrc, on && d + 4 < D ? at + 16 : OUTSIDE, 0, 0));
+      return f32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
     }
+  }
+  __device__ inline typename Mat<T>::V8 pairs(int row, int d, int D, bool on) const {
+    if constexpr (sizeof(T) == 2) {
+      const int at = row * stride + d * int(sizeof(T));
+      typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+      u32x4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[e] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, on && d + 2 * e < D ? at + 4 * e : OUTSIDE, 0, 0);
+      return __builtin_bit_cast(typename Mat<T>::V8, r);
+    } else {
+      return single(row, d, D, on);  // (float32: a pair is one element)
+    }
+  }
+  __device__ inline typename Mat<T>::V8 single(int row, int d, int D, bool on) const {
+    const int at = row * stride + d * int(sizeof(T));
+    typename Mat<T>::V8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int o = on && d + e < D ? at + e * int(sizeof(T)) : OUTSIDE;
+      if constexpr (sizeof(T) == 2)
+        r[e] = __builtin_bit_cast(T, static_cast<unsigned short>(
+                                         __builtin_amdgcn_raw_buffer_load_b16(rsrc, o, 0, 0)));
+      else
+        r[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rsrc, o, 0, 0));
+    }
+    return r;
+  }
+};
+
+// Whether a launch's views are all read 16 bytes at a time is part of the kernel's type
+// (WIDE): the narrow reads need up to eight registers for each element pair on its way
+// and would set the register count of the wide ones.
+// N fragments along a row, elements d0 + 16 i .., as Rows reads them.
+template <typename T, bool WIDE, int N>
+__device__ inline void load_row(typename Mat<T>::V8 (&f)[N], const Rows<T>& rows, int row, int d0, int D,
+                                int vec, bool on) {
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = rows.wide(row, d0 + 16 * i, D, on);
   } else if (sizeof(T) == 2 && vec == 2) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      if (on && d + e < D) {
-        const typename Mat<T>::V2 t = *reinterpret_cast<const typename Mat<T>::V2*>(row + d + e);
-        r[e] = t[0];
-        r[e + 1] = t[1];
-      }
-    }
+    for (int i = 0; i < N; ++i) f[i] = rows.pairs(row, d0 + 16 * i, D, on);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (on && d + e < D) r[e] = row[d + e];
+    for (int i = 0; i < N; ++i) f[i] = rows.single(row, d0 + 16 * i, D, on);
   }
-  return r;
 }
 
 // Four elements d .. d + 3 of a row of D, those before D.
@@ -166,21 +204,29 @@ template <typename T, int DP> struct Tile {
   }
 };
 
-// A tile's rows [row0, row0 + ROWS) on their way from memory to LDS: read into
-// registers while the tile before is worked on, stored after.  Rows from row_end on
+// A tile of ROWS rows on its way from memory to LDS: read into registers while the
+// tile before is worked on, stored after.  The first `valid` rows are read, the rest
 // and elements from D on are zeros.
-template <typename T, int DP, int ROWS, int NT> struct TileLoad {
+template <typename T, int DP, int ROWS, int NT, bool WIDE> struct TileLoad {
   static constexpr int PER_ROW = DP / 8;
   static constexpr int N = (ROWS * PER_ROW + NT - 1) / NT;
   typename Mat<T>::V8 r[N];
-  __device__ inline void load(const T* base, int64_t stride, int row0, int row_end, int D, int vec,
-                              int tid) {
+  __device__ inline void load(const T* base, int64_t stride, int valid, int D, int vec, int tid) {
+    const Rows<T> rows(base, stride);
+    valid = min(valid, ROWS);
+    auto each = [&](auto read) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = tid + i * NT, row = c / PER_ROW, d = (c % PER_ROW) * 8;
-      const bool on = row < ROWS && row0 + row < row_end;
-      r[i] = load8<T>(base + (on ? (row0 + row) * stride : 0), d, D, vec, on);
-    }
+      for (int i = 0; i < N; ++i) {
+        const int c = tid + i * NT, row = c / PER_ROW;
+        r[i] = read(row, (c % PER_ROW) * 8, row < valid);
+      }
+    };
+    if constexpr (WIDE)
+      each([&](int row, int d, bool on) { return rows.wide(row, d, D, on); });
+    else if (sizeof(T) == 2 && vec == 2)
+      each([&](int row, int d, bool on) { return rows.pairs(row, d, D, on); });
+    else
+      each([&](int row, int d, bool on) { return rows.single(row, d, D, on); });
   }
   __device__ inline void store(T* lds, int tid) const {
 #pragma unroll

@@ -169,12 +169,12 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* o
     ap[s] = A[s] + abase + static_cast<int64_t>(ti) * TM * K;
     bp[s] = B[s] + bbase + static_cast<int64_t>(tj) * TM * K;
   }
-  TileLoad<f16, BK, TM, NT> al[PARTS], bl[PARTS];
+  TileLoad<f16, BK, TM, NT, true> al[PARTS], bl[PARTS];
   auto load = [&](int k) {
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) {
-      al[s].load(ap[s] + k, K, 0, TM, BK, 8, tid);
-      bl[s].load(bp[s] + k, K, 0, TM, BK, 8, tid);
+      al[s].load(ap[s] + k, K, TM, BK, 8, tid);
+      bl[s].load(bp[s] + k, K, TM, BK, 8, tid);
     }
   };
   auto store = [&](int buf) {

@@ -40,16 +40,29 @@ struct RelAttn {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float INF = __builtin_inff();
 
-// One head's bias by slot in LDS, times log2(e), with PAD copies of either end's
-// value: a 32 x 32 block that has one difference within (lo, lo + n - 1) has none
-// further than 62 past it, so its reads need no clamp.
+// The bias of `heads` heads from h on, by slot in LDS, times log2(e), with PAD copies
+// of either end's value: a 32 x 32 block that has one difference within (lo, lo + n -
+// 1) has none further than 62 past it, so its reads need no clamp.  The two reads of a
+// value depend on one another; four of each are under way at once.
 constexpr int PAD = 64;
 template <typename T>
-__device__ inline void load_bias(float* eb, const T* table, int H, int h, const RelPos& pos,
+__device__ inline void load_bias(float* eb, const T* table, int H, int h, int heads, const RelPos& pos,
                                  int tid, int nt) {
-  for (int t = tid; t < pos.n + 2 * PAD; t += nt) {
-    const int row = pos.row_of[min(max(t - PAD, 0), pos.n - 1)];
-    eb[t] = widen(table[static_cast<int64_t>(row) * H + h]) * LOG2E;
+  const int np = pos.n + 2 * PAD, total = heads * np;
+  for (int t0 = tid; t0 < total; t0 += 4 * nt) {
+    int row[4], head[4];
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int t = min(t0 + e * nt, total - 1);
+      head[e] = heads == 1 ? 0 : t / np;
+      row[e] = pos.row_of[min(max(t - head[e] * np - PAD, 0), pos.n - 1)];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = widen(table[static_cast<int64_t>(row[e]) * H + h + head[e]]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (t0 + e * nt < total) eb[t0 + e * nt] = v[e] * LOG2E;
   }
 }
 
@@ -57,6 +70,52 @@ __device__ inline void load_bias(float* eb, const T* table, int H, int h, const 
 enum : int { NEAR = 0, ALL_BELOW = 1, ALL_ABOVE = 2 };
 __device__ inline int block_kind(const RelPos& pos, int dmin, int dmax) {
   return dmax <= pos.lo ? ALL_BELOW : dmin >= pos.lo + pos.n - 1 ? ALL_ABOVE : NEAR;
+}
+
+// 16 scores of a block whose pairs may be hidden: those are -inf.  k: the key of
+// register 0 of this lane, q: its query (row q of the mask, position qpos).
+__device__ inline void hide(f32x16& s, const RelAttn& a, const uint8_t* mask, int q, int qpos, int k,
+                            int len) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int key = k + 8 * (r / 4) + r % 4;
+    bool on = key < len && (!a.causal || key <= qpos);
+    if (mask && on) on = mask[q * a.mq + key * a.mk] != 0;
+    if (!on) s[r] = -INF;
+  }
+}
+
+// acc += V^T P^T over 16 keys of which some are hidden from some queries: a value
+// that is not finite must not reach the queries that do not see it (0 x inf).  The
+// finite values go through the product; the others are counted by two more, with 1 in
+// the place of each value and of each visible pair.
+template <typename T>
+__device__ inline f32x16 guarded(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x16 acc) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(widen(v[i])) < INF);
+  if (__ballot(bad) == 0) return Mat<T>::mma(v, p, acc);
+  typename Mat<T>::V8 fine;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) fine[i] = __builtin_fabsf(widen(v[i])) < INF ? v[i] : T(0);
+  acc = Mat<T>::mma(fine, p, acc);
+#pragma unroll 1
+  for (float way = INF; way != 0.0f; way = way > 0.0f ? -INF : 0.0f) {
+    typename Mat<T>::V8 bad_v, seen;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = widen(v[i]);
+      bad_v[i] = x == way || x != x ? T(1) : T(0);  // NaN counts both ways
+      seen[i] = widen(p[i]) == 0.0f ? T(0) : T(1);
+    }
+    f32x16 n;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) n[r] = 0.0f;
+    n = Mat<T>::mma(bad_v, seen, n);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] += n[r] > 0.0f ? way : 0.0f;
+  }
+  return acc;
 }
 
 template <typename T>
@@ -79,6 +138,14 @@ inline int check_attention(int B, int H, int Hk, int Lq, int Lk, int D, const ui
   if (static_cast<int64_t>(B) * H > (1 << 30) || Lq > (1 << 29) || Lk > (1 << 29)) return FA_E_SHAPE;
   if (mask && !mask_strides) return FA_E_ARG;
   if (mask && (mask_b < 1 || B % mask_b != 0)) return FA_E_SHAPE;
+  return FA_OK;
+}
+
+// `count` views' token strides (the third of each three): see Rows.
+inline int check_strides(const int64_t* st, int count, int dtype) {
+  const int64_t most = 0x7fffffff / (MAX_ROWS * (dtype == FA_F32 ? 4 : 2));
+  for (int i = 0; i < count; ++i)
+    if (st[3 * i + 2] < 0 || st[3 * i + 2] > most) return FA_E_SHAPE;
   return FA_OK;
 }
 

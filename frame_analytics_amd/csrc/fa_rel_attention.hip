@@ -9,6 +9,13 @@
 #include "fa_rel_attention.h"
 
 namespace fa {
+
+// fa_rel_attention_rows.hip: few queries against many keys
+int rows_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int device, int64_t* bytes);
+bool rows_serve(const RelAttn& a);
+int rows_forward(int dtype, const RelAttn& a, void* out, const View& os, float* lse, void* ws,
+                 int64_t ws_bytes, int device, hipStream_t s);
+
 namespace {
 
 template <typename T, int DP> struct Shape {
@@ -16,53 +23,7 @@ template <typename T, int DP> struct Shape {
   static constexpr size_t TILE = size_t(BN) * Tile<T, DP>::LD * sizeof(T);
 };
 
-// 16 scores of a block whose pairs may be hidden: those are -inf.  k: the key of
-// register 0 of this lane, q: its query (row q of the mask, position qpos).
-__device__ inline void hide(f32x16& s, const RelAttn& a, const uint8_t* mask, int q, int qpos, int k,
-                            int len) {
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int key = k + 8 * (r / 4) + r % 4;
-    bool on = key < len && (!a.causal || key <= qpos);
-    if (mask && on) on = mask[q * a.mq + key * a.mk] != 0;
-    if (!on) s[r] = -INF;
-  }
-}
-
-// acc += V^T P^T over 16 keys of which some are hidden from some queries: a value
-// that is not finite must not reach the queries that do not see it (0 x inf).  The
-// finite values go through the product; the others are counted by two more, with 1 in
-// the place of each value and of each visible pair.
-template <typename T>
-__device__ inline f32x16 guarded(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x16 acc) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(widen(v[i])) < INF);
-  if (__ballot(bad) == 0) return Mat<T>::mma(v, p, acc);
-  typename Mat<T>::V8 fine, up, down, seen;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = widen(v[i]);
-    fine[i] = __builtin_fabsf(x) < INF ? v[i] : T(0);
-    up[i] = x < INF ? T(0) : T(1);       // +inf, NaN
-    down[i] = x > -INF ? T(0) : T(1);    // -inf, NaN
-    seen[i] = widen(p[i]) == 0.0f ? T(0) : T(1);
-  }
-  acc = Mat<T>::mma(fine, p, acc);
-  f32x16 u, d;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) u[r] = d[r] = 0.0f;
-  u = Mat<T>::mma(up, seen, u);
-  d = Mat<T>::mma(down, seen, d);
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    if (u[r] > 0.0f) acc[r] += INF;
-    if (d[r] > 0.0f) acc[r] -= INF;
-  }
-  return acc;
-}
-
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool WIDE>
 __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* out, View os,
                                                                 int ovec, float* lse,
                                                                 int q_tiles) {
@@ -83,12 +44,12 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   const uint8_t* mask = a.mask_of(b, h);
   const float c = a.scale * LOG2E;
 
-  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, a.pos, tid, NT);
+  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
 
   typename M::V8 qf[CH];
-  const T* qrow = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h + qc * a.qs.t;
-#pragma unroll
-  for (int i = 0; i < CH; ++i) qf[i] = load8<T>(qrow, 16 * i + 8 * hh, a.D, a.vec, q < a.Lq);
+  const int q_first = tile * (NW * 32);
+  load_row<T, WIDE>(qf, Rows<T>(static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h + q_first * a.qs.t, a.qs.t),
+              q - q_first, 8 * hh, a.D, a.vec, q < a.Lq);
 
   f32x16 o[OB];
 #pragma unroll
@@ -105,11 +66,11 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   }
   const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
-  TileLoad<T, DP, BN, NT> kl, vl;
+  TileLoad<T, DP, BN, NT, WIDE> kl, vl;
   const int tiles = (end + BN - 1) / BN;
   if (tiles > 0) {
-    kl.load(kb, a.ks.t, 0, len, a.D, a.vec, tid);
-    vl.load(vb, a.vs.t, 0, len, a.D, a.vec, tid);
+    kl.load(kb, a.ks.t, len, a.D, a.vec, tid);
+    vl.load(vb, a.vs.t, len, a.D, a.vec, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
   }
@@ -119,8 +80,9 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
     const T* vv = vt + (t & 1) * BN * TL::LD;
     const bool more = t + 1 < tiles;
     if (more) {
-      kl.load(kb, a.ks.t, (t + 1) * BN, len, a.D, a.vec, tid);
-      vl.load(vb, a.vs.t, (t + 1) * BN, len, a.D, a.vec, tid);
+      const int k1 = (t + 1) * BN;
+      kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
+      vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
     }
     f32x16 s[NB];
     bool partial[NB];
@@ -216,13 +178,13 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   }
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool WIDE>
 int launch_one(const RelAttn& a, T* out, const View& os, int ovec, float* lse, hipStream_t s) {
   const int q_tiles = (a.Lq + NW * 32 - 1) / (NW * 32);
   const int64_t wgs = static_cast<int64_t>(a.B) * a.H * q_tiles;
   if (wgs > 0x7fffffff) return FA_E_SHAPE;
   const size_t lds = 4 * Shape<T, DP>::TILE + (a.pos.n + 2 * PAD) * sizeof(float);
-  auto kernel = rel_attention_kernel<T, DP, NW>;
+  auto kernel = rel_attention_kernel<T, DP, NW, WIDE>;
   if (const int e = launch_lds(kernel, lds)) return e;
   kernel<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, out, os, ovec, lse, q_tiles);
   FA_LAUNCH_CHECK();
@@ -231,8 +193,11 @@ int launch_one(const RelAttn& a, T* out, const View& os, int ovec, float* lse, h
 
 template <typename T, int DP>
 int launch_dim(const RelAttn& a, T* out, const View& os, int ovec, float* lse, hipStream_t s) {
-  return a.Lq <= 64 ? launch_one<T, DP, 2>(a, out, os, ovec, lse, s)
-                    : launch_one<T, DP, 4>(a, out, os, ovec, lse, s);
+  if (a.vec * sizeof(T) == 16)
+    return a.Lq <= 64 ? launch_one<T, DP, 2, true>(a, out, os, ovec, lse, s)
+                      : launch_one<T, DP, 4, true>(a, out, os, ovec, lse, s);
+  return a.Lq <= 64 ? launch_one<T, DP, 2, false>(a, out, os, ovec, lse, s)
+                    : launch_one<T, DP, 4, false>(a, out, os, ovec, lse, s);
 }
 
 template <typename T>
@@ -254,16 +219,12 @@ int forward(RelAttn a, void* out, const View& os, float* lse, hipStream_t s) {
 extern "C" {
 
 FA_API int fa_gpu_rel_attention_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int n,
-                                          int has_mask, int need_lse, int device,
+                                          int device,
                                           int64_t* out_bytes) {
-  (void)has_mask;
-  (void)need_lse;
-  (void)device;
   if (!out_bytes) return FA_E_ARG;
   if (n < 1 || n > FA_REL_MAX) return FA_E_SHAPE;
   if (const int e = fa::check_attention(B, H, Hk, Lq, Lk, D, nullptr, 1, nullptr)) return e;
-  *out_bytes = 0;
-  return FA_OK;
+  return fa::rows_workspace(B, H, Hk, Lq, Lk, D, device, out_bytes);
 }
 
 FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int dtype, int B,
@@ -275,11 +236,10 @@ FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int
                                 float* lse, void* workspace, int64_t workspace_bytes, int device,
                                 void* stream) {
   using namespace fa;
-  (void)workspace;
-  (void)workspace_bytes;
   if (!q || !k || !v || !strides || !table || !out) return FA_E_ARG;
   if (const int e = check_attention(B, H, Hk, Lq, Lk, D, mask, mask_b, mask_strides)) return e;
   if (const int e = check_relpos(row_of, rows, lo, n, grid_w, Lq, Lk, q_start, q_starts)) return e;
+  if (const int e = check_strides(strides, 4, dtype)) return e;
   DeviceScope scope(device);
   if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
   const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table,
@@ -287,6 +247,7 @@ FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int
                                   mask, mask_b, mask_strides, causal, scale);
   const View os{strides[9], strides[10], strides[11]};
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows_serve(a)) return rows_forward(dtype, a, out, os, lse, workspace, workspace_bytes, device, s);
   switch (dtype) {
     case FA_F16: return forward<_Float16>(a, out, os, lse, s);
     case FA_BF16: return forward<__bf16>(a, out, os, lse, s);

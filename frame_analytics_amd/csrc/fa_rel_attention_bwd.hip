@@ -48,7 +48,7 @@ template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<
 // ---------------------------------------------------------------------------
 // dQ and the table
 // ---------------------------------------------------------------------------
-template <typename T, int DP, bool TABLE>
+template <typename T, int DP, bool TABLE, bool WIDE>
 __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g, int q_tiles) {
   using M = Mat<T>;
   using TL = Tile<T, DP>;
@@ -70,16 +70,13 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
   const uint8_t* mask = a.mask_of(b, h);
   const float c = a.scale * LOG2E;
 
-  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, a.pos, tid, NT);
+  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
   if (TABLE)
     for (int t = tid; t < NW * np; t += NT) sums[t] = 0.0f;
   float* mine = sums + wave * np;
   float far_lo = 0.0f, far_hi = 0.0f;
 
   typename M::V8 qf[CH], gf[CH];
-  const T* qrow = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h + qc * a.qs.t;
-  const T* grow = static_cast<const T*>(g.dout) + b * g.gs.b + h * g.gs.h + qc * g.gs.t;
-  const T* orow = static_cast<const T*>(g.out) + b * g.os.b + h * g.os.h + qc * g.os.t;
   const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.Lq + qc;
   // a row that sees no key: its weights are 2^(s - inf) = 0 whatever dout holds
   const float lse = g.lse[row];
@@ -89,11 +86,17 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
   f32x16 dd;
 #pragma unroll
   for (int r = 0; r < 16; ++r) dd[r] = 0.0f;
+  {
+    const int f = tile * (NW * 32);  // the workgroup's first query
+    auto rows = [&](const void* p, const View& s) {
+      return Rows<T>(static_cast<const T*>(p) + b * s.b + h * s.h + f * s.t, s.t);
+    };
+    typename M::V8 of[CH];
+    load_row<T, WIDE>(qf, rows(a.q, a.qs), q - f, 8 * hh, a.D, a.vec, on);
+    load_row<T, WIDE>(gf, rows(g.dout, g.gs), q - f, 8 * hh, a.D, a.vec, on);
+    load_row<T, WIDE>(of, rows(g.out, g.os), q - f, 8 * hh, a.D, a.vec, on);
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    qf[i] = load8<T>(qrow, 16 * i + 8 * hh, a.D, a.vec, on);
-    gf[i] = load8<T>(grow, 16 * i + 8 * hh, a.D, a.vec, on);
-    dd = M::mma(load8<T>(orow, 16 * i + 8 * hh, a.D, a.vec, on), gf[i], dd);
+    for (int i = 0; i < CH; ++i) dd = M::mma(of[i], gf[i], dd);
   }
   float dsum = 0.0f;
 #pragma unroll
@@ -115,11 +118,11 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
   }
   const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
-  TileLoad<T, DP, BN, NT> kl, vl;
+  TileLoad<T, DP, BN, NT, WIDE> kl, vl;
   const int tiles = (end + BN - 1) / BN;
   if (tiles > 0) {
-    kl.load(kb, a.ks.t, 0, len, a.D, a.vec, tid);
-    vl.load(vb, a.vs.t, 0, len, a.D, a.vec, tid);
+    kl.load(kb, a.ks.t, len, a.D, a.vec, tid);
+    vl.load(vb, a.vs.t, len, a.D, a.vec, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
   }
@@ -129,8 +132,9 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
     const T* vv = vt + (t % BUFS) * BN * TL::LD;
     const bool more = t + 1 < tiles;
     if (more) {
-      kl.load(kb, a.ks.t, (t + 1) * BN, len, a.D, a.vec, tid);
-      vl.load(vb, a.vs.t, (t + 1) * BN, len, a.D, a.vec, tid);
+      const int k1 = (t + 1) * BN;
+      kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
+      vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -262,7 +266,7 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
 // ---------------------------------------------------------------------------
 // dK and dV
 // ---------------------------------------------------------------------------
-template <typename T, int DP>
+template <typename T, int DP, bool WIDE>
 __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads g, int k_tiles) {
   using M = Mat<T>;
   using TL = Tile<T, DP>;
@@ -286,13 +290,10 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
   const int k_first = tile * (NW * 32);
 
   typename M::V8 kf[CH], vf[CH];
-  const T* krow = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + kc * a.ks.t;
-  const T* vrow = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h + kc * a.vs.t;
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    kf[i] = load8<T>(krow, 16 * i + 8 * hh, a.D, a.vec, key < len);
-    vf[i] = load8<T>(vrow, 16 * i + 8 * hh, a.D, a.vec, key < len);
-  }
+  load_row<T, WIDE>(kf, Rows<T>(static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + k_first * a.ks.t, a.ks.t),
+              key - k_first, 8 * hh, a.D, a.vec, key < len);
+  load_row<T, WIDE>(vf, Rows<T>(static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h + k_first * a.vs.t, a.vs.t),
+              key - k_first, 8 * hh, a.D, a.vec, key < len);
   f32x16 dk[OB], dv[OB];
 #pragma unroll
   for (int i = 0; i < OB; ++i)
@@ -307,9 +308,9 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
   }
   const int t0 = first / BM;
   const int tiles = k_first < len ? (a.Lq + BM - 1) / BM : 0;
-  TileLoad<T, DP, BM, NT> ql, gl;
+  TileLoad<T, DP, BM, NT, WIDE> ql, gl;
   float lse_r = 0.0f, d_r = 0.0f;
-  float row_lse[TileLoad<T, DP, BM, NT>::N];  // of the rows that this thread brings
+  float row_lse[TileLoad<T, DP, BM, NT, WIDE>::N];  // of the rows that this thread brings
 
   for (int hg = 0; hg < group; ++hg) {
     const int h = hk * group + hg;
@@ -318,8 +319,9 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
     const T* gb = static_cast<const T*>(g.dout) + b * g.gs.b + h * g.gs.h;
     const int64_t row0 = (static_cast<int64_t>(b) * a.H + h) * a.Lq;
     auto load = [&](int t) {
-      ql.load(qb, a.qs.t, t * BM, a.Lq, a.D, a.vec, tid);
-      gl.load(gb, g.gs.t, t * BM, a.Lq, a.D, a.vec, tid);
+      const int i0 = t * BM;
+      ql.load(qb + i0 * a.qs.t, a.qs.t, a.Lq - i0, a.D, a.vec, tid);
+      gl.load(gb + i0 * g.gs.t, g.gs.t, a.Lq - i0, a.D, a.vec, tid);
 #pragma unroll
       for (int i = 0; i < ql.N; ++i) {
         const int r = t * BM + (tid + i * NT) / ql.PER_ROW;
@@ -346,7 +348,7 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
       }
     };
     __syncthreads();  // the head before is done with its tiles and bias
-    load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, a.pos, tid, NT);
+    load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
     if (t0 < tiles) {
       load(t0);
       store(t0);
@@ -457,16 +459,16 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
 
 inline int tiles_of(int n) { return (n + NW * 32 - 1) / (NW * 32); }
 
-template <typename T, int DP>
-int launch_dim(const RelAttn& a, const Grads& g, hipStream_t s) {
+template <typename T, int DP, bool WIDE>
+int launch_wide(const RelAttn& a, const Grads& g, hipStream_t s) {
   const int qt = tiles_of(a.Lq), kt = tiles_of(a.Lk);
   const int64_t wq = static_cast<int64_t>(a.B) * a.H * qt, wk = static_cast<int64_t>(a.B) * a.Hk * kt;
   if (wq > 0x7fffffff || wk > 0x7fffffff) return FA_E_SHAPE;
   const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
   const size_t lds_q = tiles + (g.parts ? 1 + NW : 1) * np * sizeof(float);
   const size_t lds_k = tiles + ((np + 3) / 4 * 4 + 4 * Shape<T, DP>::BN) * sizeof(float);
-  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, true> : rel_attention_dq_kernel<T, DP, false>;
-  auto dkv = rel_attention_dkv_kernel<T, DP>;
+  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, true, WIDE> : rel_attention_dq_kernel<T, DP, false, WIDE>;
+  auto dkv = rel_attention_dkv_kernel<T, DP, WIDE>;
   if (const int e = launch_lds(dq, lds_q)) return e;
   if (const int e = launch_lds(dkv, lds_k)) return e;
   dq<<<static_cast<unsigned>(wq), NT, lds_q, s>>>(a, g, qt);
@@ -474,6 +476,11 @@ int launch_dim(const RelAttn& a, const Grads& g, hipStream_t s) {
   dkv<<<static_cast<unsigned>(wk), NT, lds_k, s>>>(a, g, kt);
   FA_LAUNCH_CHECK();
   return FA_OK;
+}
+
+template <typename T, int DP>
+int launch_dim(const RelAttn& a, const Grads& g, hipStream_t s) {
+  return a.vec * sizeof(T) == 16 ? launch_wide<T, DP, true>(a, g, s) : launch_wide<T, DP, false>(a, g, s);
 }
 
 template <typename T>
@@ -529,6 +536,7 @@ FA_API int fa_gpu_rel_attention_backward(
     return FA_E_ARG;
   if (const int e = check_attention(B, H, Hk, Lq, Lk, D, mask, mask_b, mask_strides)) return e;
   if (const int e = check_relpos(row_of, rows, lo, n, grid_w, Lq, Lk, q_start, q_starts)) return e;
+  if (const int e = check_strides(strides, 8, dtype)) return e;
   int64_t need = 0;
   if (const int e = fa_gpu_rel_attention_backward_workspace(B, H, Lq, n, dtable != nullptr, &need))
     return e;

@@ -59,11 +59,10 @@ FA_API int fa_gpu_rel_bias_backward(const void* up, const int64_t* up_strides, i
  * as within +-2^30.  mask_strides: {batch, head, query, key} in bytes.
  * lse: [B, H, Lq] float32 or null; log2 of each row's sum of exponentials, +inf for
  * a row that sees nothing (what the backward pass reads).
- * workspace: fa_gpu_rel_attention_workspace bytes (0: may be null).
+ * workspace: fa_gpu_rel_attention_workspace bytes, 16-byte aligned (0: may be null).
  */
 FA_API int fa_gpu_rel_attention_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int n,
-                                          int has_mask, int need_lse, int device,
-                                          int64_t* out_bytes);
+                                          int device, int64_t* out_bytes);
 FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int dtype, int B,
                                 int H, int Hk, int Lq, int Lk, int D, const int64_t* strides,
                                 const void* table, int rows, const int* row_of, int lo, int n,

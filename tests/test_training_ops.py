@@ -234,8 +234,8 @@ def test_arguments_are_checked_before_any_gpu_work(lib):
         assert attention(**kw) == 2, kw
     assert attention(mask=p) == 5  # a mask without strides
     aws = lib.fa_gpu_rel_attention_workspace
-    assert aws(1, 2, 1, 4, 4, 8, 9, 0, 0, 0, None) == 5
-    assert aws(1, 2, 1, 4, 4, 8, 0, 0, 0, 0, out) == 2
+    assert aws(1, 2, 1, 4, 4, 8, 9, 0, None) == 5
+    assert aws(1, 2, 1, 4, 4, 8, 0, 0, out) == 2
     bws = lib.fa_gpu_rel_attention_backward_workspace
     assert bws(1, 2, 4, 9, 1, out) == 0 and n64.value >= 2 * 4 * 4 + 2 * 9 * 4
     need = n64.value

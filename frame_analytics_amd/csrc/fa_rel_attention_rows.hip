@@ -3,10 +3,17 @@
 //
 // The memory's rate bounds it: every key and value is read once for all the query
 // heads that share it.  The rows of one key head, its query heads times the queries,
-// are the columns of one 32-wide block.  The keys are dealt out in blocks of 32 to the
-// waves of `splits` workgroups; a wave works on its blocks by itself, through LDS of
-// its own, with the next block on its way in registers, so no wave waits for another.
-// The waves' sums are joined in LDS, the workgroups' by rows_join_kernel.
+// are the columns of one or two 16-wide blocks.  The keys are dealt out in runs to
+// `splits` workgroups, in blocks of 32 to their waves; a wave works on its blocks by
+// itself, the next block on its way in registers, so no wave waits for another: keys
+// arrive as the fragments of S^T = K Q^T, values pass through LDS of the wave's own to
+// be read transposed.  The waves' sums are joined in LDS, the workgroups' by
+// rows_join_kernel.
+//
+// Blocks here are 16 x 16: with l the lane and g = l / 16 a C block holds rows 4 g + r
+// of column l % 16 in registers r = 0 .. 3, and an A or B fragment row or column l % 16
+// with eight of 32 k values, straight (8 g + i) or split (16 (i / 4) + 4 g + i % 4, the
+// rows that two C blocks hold).
 #include "fa_rel_attention.h"
 
 namespace fa {
@@ -18,145 +25,264 @@ namespace {
 constexpr int NW = 4, NT = NW * 64, BN = 32;
 constexpr int MOST_BIAS = 6144;  // floats of LDS for the bias of the heads together
 
-// Workgroups that share the keys of one key head: enough for eight waves on every
-// compute unit, and at least two blocks of keys for each wave.
+// Keys are dealt out in runs of `per` blocks for each wave of a workgroup: as few as keep
+// two workgroups for every compute unit, so that entries of different lengths even out
+// (the runs past an entry's end return at once).
+inline int per_wave(int B, int Hk, int Lk, int device) {
+  const int64_t blocks = static_cast<int64_t>(B) * Hk * ((Lk + BN - 1) / BN);
+  const int64_t per = blocks / (static_cast<int64_t>(NW) * 2 * cu_count(device));
+  return static_cast<int>(per < 1 ? 1 : per > 64 ? 64 : per);
+}
 inline int splits_of(int B, int Hk, int Lk, int device) {
-  const int64_t heads = static_cast<int64_t>(B) * Hk;
-  const int64_t want = (2 * cu_count(device) + heads - 1) / heads;
-  const int64_t most = (Lk + 2 * NW * BN - 1) / (2 * NW * BN);
-  const int64_t s = want < most ? want : most;
-  return static_cast<int>(s < 1 ? 1 : s);
+  const int run = per_wave(B, Hk, Lk, device) * NW * BN;
+  return (Lk + run - 1) / run;
 }
 
-// What a wave's LDS region has to hold: its tiles, and later its O block.
-template <typename T, int DP> constexpr size_t region() {
-  constexpr size_t tiles = 2 * BN * Tile<T, DP>::LD * sizeof(T), o = size_t(DP) * 32 * sizeof(float);
-  return tiles > o ? tiles : o;
+template <typename T> __device__ inline f32x4 mma16(typename Mat<T>::V8 a, typename Mat<T>::V8 b, f32x4 c) {
+  if constexpr (std::is_same<T, _Float16>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  } else if constexpr (std::is_same<T, __bf16>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
 }
 
-template <typename T, int DP, bool WIDE>
+// Over the four lanes l % 16 + 16 g, in all of them.
+__device__ inline float four_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return both_max(fmaxf(__int_as_float(r[0]), __int_as_float(r[1])));
+}
+__device__ inline float four_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return both_sum(__int_as_float(r[0]) + __int_as_float(r[1]));
+}
+
+// Column col0 + l % 16 of a tile's 32 rows, in split slots.
+template <typename T, int DP>
+__device__ inline typename Mat<T>::V8 transposed16(const T* t, int col0, int lane) {
+  constexpr int LD = Tile<T, DP>::LD;
+  typename Mat<T>::V8 r;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    typedef typename Mat<T>::V4 V4;
+    const T* p = t + (lane >> 2) * LD + col0 + 4 * (lane & 3);
+    const V4 x = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p));
+    const V4 y = __builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 16 * LD)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r[i] = x[i];
+      r[4 + i] = y[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = t[(16 * (i / 4) + 4 * (lane >> 4) + i % 4) * LD + col0 + (lane & 15)];
+  }
+  return r;
+}
+
+// As guarded<T>, for 16 x 16 blocks.
+template <typename T>
+__device__ inline f32x4 guarded16(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x4 acc) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(widen(v[i])) < INF);
+  if (__ballot(bad) == 0) return mma16<T>(v, p, acc);
+  typename Mat<T>::V8 fine;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) fine[i] = __builtin_fabsf(widen(v[i])) < INF ? v[i] : T(0);
+  acc = mma16<T>(fine, p, acc);
+#pragma unroll 1
+  for (float way = INF; way != 0.0f; way = way > 0.0f ? -INF : 0.0f) {
+    typename Mat<T>::V8 bad_v, seen;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = widen(v[i]);
+      bad_v[i] = x == way || x != x ? T(1) : T(0);
+      seen[i] = widen(p[i]) == 0.0f ? T(0) : T(1);
+    }
+    const f32x4 n = mma16<T>(bad_v, seen, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] += n[r] > 0.0f ? way : 0.0f;
+  }
+  return acc;
+}
+
+// A wave's LDS: its values, and later its O block of NC x 16 rows.
+template <typename T, int DP, int NC> constexpr size_t region() {
+  constexpr size_t tile = BN * Tile<T, DP>::LD * sizeof(T), o = size_t(DP) * 16 * NC * sizeof(float);
+  return tile > o ? tile : o;
+}
+
+template <typename T, int DP, int NC, bool WIDE>
 __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os, float* lse, int splits,
-                                                  float* part_o, float* part_ml) {
+                                                     int per, float* part_o, float* part_ml) {
   using M = Mat<T>;
-  using TL = Tile<T, DP>;
-  constexpr int CH = DP / 16, OB = DP / 32;
+  constexpr int CH = DP / 32, OB = DP / 16, ROWS = 16 * NC;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, gg = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  T* kt = reinterpret_cast<T*>(smem + wave * region<T, DP>());
-  T* vt = kt + BN * TL::LD;
-  float* ml = reinterpret_cast<float*>(smem + NW * region<T, DP>());  // [NW][2][32]
-  float* eb = ml + NW * 64;                                           // [group][np]
+  T* vt = reinterpret_cast<T*>(smem + wave * region<T, DP, NC>());
+  float* ml = reinterpret_cast<float*>(smem + NW * region<T, DP, NC>());  // [NW][2][ROWS]
+  float* eb = ml + NW * 2 * ROWS;                                         // [group][np]
   const int np = a.pos.n + 2 * PAD, group = a.H / a.Hk, rows = group * a.Lq;
   const int split = blockIdx.x % splits, bh = blockIdx.x / splits, hk = bh % a.Hk, b = bh / a.Hk;
   const int s0 = a.start(b), len = a.keys(b);
-  const int g = min(col, rows - 1) / a.Lq, i = min(col, rows - 1) % a.Lq, h = hk * group + g;
-  const uint8_t* mask = a.mask_of(b, h);
   const float c = a.scale * LOG2E;
 
   int end = len;
   if (a.causal)
     end = static_cast<int>(max<int64_t>(0, min<int64_t>(end, int64_t(s0) + a.Lq)));
+  const int run = per * NW * BN, stride = NW * BN;
+  if (splits > 1 && static_cast<int64_t>(split) * run >= end) {
+    if (tid < rows) {
+      float* none = part_ml + 2 * (static_cast<int64_t>(blockIdx.x) * rows + tid);
+      none[0] = -INF;
+      none[1] = 0.0f;
+    }
+    return;
+  }
+  end = static_cast<int>(min<int64_t>(end, (static_cast<int64_t>(split) + 1) * run));
   const T* kb = static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h;
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
-  TileLoad<T, DP, BN, 64, WIDE> kl, vl;
-  const int stride = splits * NW * BN;
-  int k0 = (split * NW + wave) * BN;
-  if (k0 < end) {
-    kl.load(kb + k0 * a.ks.t, a.ks.t, len - k0, a.D, a.vec, lane);
-    vl.load(vb + k0 * a.vs.t, a.vs.t, len - k0, a.D, a.vec, lane);
+  TileLoad<T, DP, BN, 64, WIDE> vl;
+  typename M::V8 kf[2][CH];
+  auto load = [&](int k) {
+    const Rows<T> kr(kb + k * a.ks.t, a.ks.t);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int row = 16 * n + col, d = 32 * i + 8 * gg;
+        const bool on = k + row < len;
+        if constexpr (WIDE) kf[n][i] = kr.wide(row, d, a.D, on);
+        else if (a.vec == 2) kf[n][i] = kr.pairs(row, d, a.D, on);
+        else kf[n][i] = kr.single(row, d, a.D, on);
+      }
+    vl.load(vb + k * a.vs.t, a.vs.t, len - k, a.D, a.vec, lane);
+  };
+  int k0 = split * run + wave * BN;
+  if (k0 < end) load(k0);
+
+  int qi[NC], gi[NC];
+  const uint8_t* mask[NC];
+  typename M::V8 qf[NC][CH];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int row = min(16 * n + col, rows - 1);
+    gi[n] = row / a.Lq;
+    qi[n] = row % a.Lq;
+    mask[n] = a.mask_of(b, hk * group + gi[n]);
+    // (the head's stride is per lane: its offset is part of the row's)
+    Rows<T> qr(static_cast<const T*>(a.q) + b * a.qs.b + hk * group * a.qs.h, a.qs.t);
+    qr.stride = 1;
+    const int at = static_cast<int>((gi[n] * a.qs.h + qi[n] * a.qs.t) * static_cast<int64_t>(sizeof(T)));
+    const bool on = 16 * n + col < rows;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int d = 32 * i + 8 * gg;
+      if constexpr (WIDE) qf[n][i] = qr.wide(at, d, a.D, on);
+      else if (a.vec == 2) qf[n][i] = qr.pairs(at, d, a.D, on);
+      else qf[n][i] = qr.single(at, d, a.D, on);
+    }
   }
   load_bias<T>(eb, static_cast<const T*>(a.table), a.H, hk * group, group, a.pos, tid, NT);
 
-  typename M::V8 qf[CH];
-  // (the head's stride is per lane: its offset is part of the row's)
-  {
-    const T* q0 = static_cast<const T*>(a.q) + b * a.qs.b + hk * group * a.qs.h;
-    Rows<T> qr(q0, a.qs.t);
-    qr.stride = 1;
-    load_row<T, WIDE>(qf, qr, int((g * a.qs.h + i * a.qs.t) * int64_t(sizeof(T))), 8 * hh, a.D, a.vec, col < rows);
+  f32x4 o[NC][OB];
+  float m[NC], l[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    m[n] = -INF;
+    l[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < OB; ++i) o[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  f32x16 o[OB];
-#pragma unroll
-  for (int n = 0; n < OB; ++n)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
-  float m = -INF, l = 0.0f;
   __syncthreads();  // the bias
   for (; k0 < end; k0 += stride) {
-    kl.store(kt, lane);
     vl.store(vt, lane);
+    f32x4 s[NC][2];
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        s[n][w] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < CH; ++i) s[n][w] = mma16<T>(kf[w][i], qf[n][i], s[n][w]);
+      }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (k0 + stride < end) {
-      const int k1 = k0 + stride;
-      kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, lane);
-      vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, lane);
-    }
-    f32x16 s;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-#pragma unroll
-    for (int n = 0; n < CH; ++n) s = M::mma(TL::straight(kt, col, 16 * n + 8 * hh), qf[n], s);
+    if (k0 + stride < end) load(k0 + stride);
     const int kind = block_kind(a.pos, s0 - (k0 + 31), s0 + a.Lq - 1 - k0);
-    if (kind == NEAR) {
-      const float* e = eb + g * np + (s0 + i - k0 - 4 * hh - a.pos.lo + PAD);
+    const bool partial = a.mask || k0 + 32 > len || (a.causal && k0 + 31 > s0);
+    typename M::V8 p[NC];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = s[r] * c + e[-(8 * (r / 4) + r % 4)];
-    } else {
-      const float e = eb[g * np + (kind == ALL_BELOW ? 0 : np - 1)];
+    for (int n = 0; n < NC; ++n) {
+      const float* e = eb + gi[n] * np + (s0 + qi[n] - k0 - 4 * gg - a.pos.lo + PAD);
+      const float far = eb[gi[n] * np + (kind == ALL_BELOW ? 0 : np - 1)];
+      float top = -INF;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = s[r] * c + e;
-    }
-    const bool partial = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0);
-    if (partial) hide(s, a, mask, i, s0 + i, k0 + 4 * hh, len);
-    float top = -INF;
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
-    top = both_max(top);
-    const float mn = fmaxf(m, top);
-    if (__ballot(mn > m)) {
-      const float shrink = mn == -INF ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-      l *= shrink;
+        for (int r = 0; r < 4; ++r) {
+          float x = s[n][w][r] * c + (kind == NEAR ? e[-(16 * w + r)] : far);
+          if (partial) {
+            const int key = k0 + 16 * w + 4 * gg + r;
+            bool seen = key < len && (!a.causal || key <= s0 + qi[n]);
+            if (a.mask && seen) seen = mask[n][qi[n] * a.mq + key * a.mk] != 0;
+            if (!seen) x = -INF;
+          }
+          s[n][w][r] = x;
+          top = fmaxf(top, x);
+        }
+      top = four_max(top);
+      const float mn = fmaxf(m[n], top);
+      if (__ballot(mn > m[n])) {
+        const float shrink = mn == -INF ? 1.0f : __builtin_amdgcn_exp2f(m[n] - mn);
+        l[n] *= shrink;
 #pragma unroll
-      for (int n = 0; n < OB; ++n)
+        for (int i = 0; i < OB; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[n][r] *= shrink;
-      m = mn;
-    }
-    const float sub = m == -INF ? 0.0f : m;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = __builtin_amdgcn_exp2f(s[r] - sub);
-      l += s[r];
-    }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      typename M::V8 p;
-#pragma unroll
-      for (int n = 0; n < 8; ++n) p[n] = T(s[8 * half + n]);
-#pragma unroll
-      for (int n = 0; n < OB; ++n) {
-        const typename M::V8 vf = TL::transposed(vt, 16 * half, 32 * n, lane);
-        o[n] = partial ? guarded<T>(vf, p, o[n]) : M::mma(vf, p, o[n]);
+          for (int r = 0; r < 4; ++r) o[n][i][r] *= shrink;
+        m[n] = mn;
       }
+      const float sub = m[n] == -INF ? 0.0f : m[n];
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = __builtin_amdgcn_exp2f(s[n][w][r] - sub);
+          l[n] += x;
+          p[n][4 * w + r] = T(x);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < OB; ++i) {
+      const typename M::V8 vf = transposed16<T, DP>(vt, 16 * i, lane);
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        o[n][i] = partial ? guarded16<T>(vf, p[n], o[n][i]) : mma16<T>(vf, p[n], o[n][i]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
-  l = both_sum(l);
 
   // join the waves: O^T in LDS as [d][row], each wave's in its own region
-  float* ob = reinterpret_cast<float*>(smem + wave * region<T, DP>());
+  float* ob = reinterpret_cast<float*>(smem + wave * region<T, DP, NC>());
 #pragma unroll
-  for (int n = 0; n < OB; ++n)
+  for (int n = 0; n < NC; ++n) {
+    l[n] = four_sum(l[n]);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) ob[(32 * n + 8 * (r / 4) + 4 * hh + r % 4) * 32 + col] = o[n][r];
-  if (hh == 0) {
-    ml[wave * 64 + col] = m;
-    ml[wave * 64 + 32 + col] = l;
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ob[(16 * i + 4 * gg + r) * ROWS + 16 * n + col] = o[n][i][r];
+    if (gg == 0) {
+      ml[wave * 2 * ROWS + 16 * n + col] = m[n];
+      ml[wave * 2 * ROWS + ROWS + 16 * n + col] = l[n];
+    }
   }
   __syncthreads();
   for (int t = tid; t < rows * DP; t += NT) {
@@ -164,13 +290,13 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
     if (d >= a.D) continue;
     float top = -INF;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w * 64 + row]);
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w * 2 * ROWS + row]);
     float sum = 0.0f, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float mw = ml[w * 64 + row], f = mw == -INF ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
-      total += f * ml[w * 64 + 32 + row];
-      const float x = reinterpret_cast<const float*>(smem + w * region<T, DP>())[d * 32 + row];
+      const float mw = ml[w * 2 * ROWS + row], f = mw == -INF ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
+      total += f * ml[w * 2 * ROWS + ROWS + row];
+      const float x = reinterpret_cast<const float*>(smem + w * region<T, DP, NC>())[d * ROWS + row];
       if (mw != -INF) sum += f * x;
     }
     if (splits > 1) {
@@ -198,19 +324,43 @@ __global__ __launch_bounds__(64) void rows_join_kernel(const float* part_o, cons
   const int rows = H / Hk * Lq, row = blockIdx.x % rows, bh = blockIdx.x / rows, hk = bh % Hk, b = bh / Hk;
   const int h = hk * (H / Hk) + row / Lq, i = row % Lq;
   const int64_t first = static_cast<int64_t>(bh) * splits * rows + row;
+  // the splits' maxima and sums, one lane each; then their values, eight reads at once
+  const int lane = threadIdx.x, d0 = lane, d1 = lane + 64;
   float top = -INF;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml[2 * (first + static_cast<int64_t>(s) * rows)]);
+  for (int s = lane; s < splits; s += 64)
+    top = fmaxf(top, part_ml[2 * (first + static_cast<int64_t>(s) * rows)]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   float x0 = 0.0f, x1 = 0.0f, total = 0.0f;
-  const int d0 = threadIdx.x, d1 = threadIdx.x + 64;
-  for (int s = 0; s < splits; ++s) {
-    const int64_t at = first + static_cast<int64_t>(s) * rows;
-    const float ms = part_ml[2 * at];
-    if (ms == -INF) continue;
-    const float f = __builtin_amdgcn_exp2f(ms - top);
-    total += f * part_ml[2 * at + 1];
-    if (d0 < D) x0 += f * part_o[at * D + d0];
-    if (d1 < D) x1 += f * part_o[at * D + d1];
+  for (int s0 = 0; s0 < splits; s0 += 64) {
+    float f = 0.0f;
+    if (s0 + lane < splits) {
+      const int64_t at = first + static_cast<int64_t>(s0 + lane) * rows;
+      const float ms = part_ml[2 * at];
+      if (ms != -INF) {
+        f = __builtin_amdgcn_exp2f(ms - top);
+        total += f * part_ml[2 * at + 1];
+      }
+    }
+    const int here = min(64, splits - s0);
+    for (int s1 = 0; s1 < here; s1 += 8) {
+      float fs[8], y0[8], y1[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        fs[e] = s1 + e < here ? __shfl(f, (s1 + e) & 63, 64) : 0.0f;
+        const float* p = part_o + (first + static_cast<int64_t>(s0 + s1 + e) * rows) * D;
+        // (what a split that saw no key left in part_o is not read)
+        y0[e] = fs[e] != 0.0f && d0 < D ? p[d0] : 0.0f;
+        y1[e] = fs[e] != 0.0f && d1 < D ? p[d1] : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x0 += fs[e] * y0[e];
+        x1 += fs[e] * y1[e];
+      }
+    }
   }
+  total = wave_sum(total);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   T* o = out + b * os.b + h * os.h + i * os.t;
   if (d0 < D) o[d0] = T(x0 * inv);
@@ -219,17 +369,17 @@ __global__ __launch_bounds__(64) void rows_join_kernel(const float* part_o, cons
     lse[(static_cast<int64_t>(b) * H + h) * Lq + i] = total == 0.0f ? INF : top + __builtin_log2f(total);
 }
 
-template <typename T, int DP>
-int launch_dim(const RelAttn& a, T* out, const View& os, float* lse, int splits, float* part_o,
-               float* part_ml, hipStream_t s) {
+template <typename T, int DP, int NC>
+int launch_rows(const RelAttn& a, T* out, const View& os, float* lse, int splits, int per,
+               float* part_o, float* part_ml, hipStream_t s) {
   const int group = a.H / a.Hk, rows = group * a.Lq;
   const int64_t wgs = static_cast<int64_t>(a.B) * a.Hk * splits;
   const int64_t joins = static_cast<int64_t>(a.B) * a.Hk * rows;
   if (wgs > 0x7fffffff || joins > 0x7fffffff) return FA_E_SHAPE;
-  const size_t lds = NW * region<T, DP>() + (NW * 64 + group * (a.pos.n + 2 * PAD)) * sizeof(float);
-  auto kernel = a.vec * sizeof(T) == 16 ? rows_kernel<T, DP, true> : rows_kernel<T, DP, false>;
+  const size_t lds = NW * region<T, DP, NC>() + (NW * 32 * NC + group * (a.pos.n + 2 * PAD)) * sizeof(float);
+  auto kernel = a.vec * sizeof(T) == 16 ? rows_kernel<T, DP, NC, true> : rows_kernel<T, DP, NC, false>;
   if (const int e = launch_lds(kernel, lds)) return e;
-  kernel<<<static_cast<unsigned>(wgs), NT, lds, s>>>(a, out, os, lse, splits, part_o, part_ml);
+  kernel<<<static_cast<unsigned>(wgs), NT, lds, s>>>(a, out, os, lse, splits, per, part_o, part_ml);
   FA_LAUNCH_CHECK();
   if (splits > 1) {
     rows_join_kernel<T><<<static_cast<unsigned>(joins), 64, 0, s>>>(part_o, part_ml, a.H, a.Hk, a.Lq,
@@ -239,16 +389,23 @@ int launch_dim(const RelAttn& a, T* out, const View& os, float* lse, int splits,
   return FA_OK;
 }
 
+template <typename T, int DP>
+int launch_dim(const RelAttn& a, T* out, const View& os, float* lse, int splits, int per, float* part_o,
+               float* part_ml, hipStream_t s) {
+  return a.H / a.Hk * a.Lq <= 16 ? launch_rows<T, DP, 1>(a, out, os, lse, splits, per, part_o, part_ml, s)
+                                 : launch_rows<T, DP, 2>(a, out, os, lse, splits, per, part_o, part_ml, s);
+}
+
 template <typename T>
-int forward(RelAttn a, void* out, const View& os, float* lse, int splits, float* part_o, float* part_ml,
-            hipStream_t s) {
+int forward(RelAttn a, void* out, const View& os, float* lse, int splits, int per, float* part_o,
+            float* part_ml, hipStream_t s) {
   const void* in[3] = {a.q, a.k, a.v};
   const View iv[3] = {a.qs, a.ks, a.vs};
   a.vec = widest_load<T>(in, iv, 3, a.D);
   T* o = static_cast<T*>(out);
-  if (a.D <= 32) return launch_dim<T, 32>(a, o, os, lse, splits, part_o, part_ml, s);
-  if (a.D <= 64) return launch_dim<T, 64>(a, o, os, lse, splits, part_o, part_ml, s);
-  return launch_dim<T, 128>(a, o, os, lse, splits, part_o, part_ml, s);
+  if (a.D <= 32) return launch_dim<T, 32>(a, o, os, lse, splits, per, part_o, part_ml, s);
+  if (a.D <= 64) return launch_dim<T, 64>(a, o, os, lse, splits, per, part_o, part_ml, s);
+  return launch_dim<T, 128>(a, o, os, lse, splits, per, part_o, part_ml, s);
 }
 
 }  // namespace
@@ -275,13 +432,14 @@ int rows_forward(int dtype, const RelAttn& a, void* out, const View& os, float* 
   if (const int e = rows_workspace(a.B, a.H, a.Hk, a.Lq, a.Lk, a.D, device, &need)) return e;
   if (need > 0 && (!ws || ws_bytes < need)) return FA_E_ARG;
   const int splits = splits_of(a.B, a.Hk, a.Lk, device);
+  const int per = per_wave(a.B, a.Hk, a.Lk, device);
   float* part_ml = static_cast<float*>(ws);
   float* part_o = part_ml ? part_ml + static_cast<int64_t>(a.B) * a.Hk * splits * (a.H / a.Hk) * a.Lq * 2
                           : nullptr;
   switch (dtype) {
-    case FA_F16: return forward<_Float16>(a, out, os, lse, splits, part_o, part_ml, s);
-    case FA_BF16: return forward<__bf16>(a, out, os, lse, splits, part_o, part_ml, s);
-    case FA_F32: return forward<float>(a, out, os, lse, splits, part_o, part_ml, s);
+    case FA_F16: return forward<_Float16>(a, out, os, lse, splits, per, part_o, part_ml, s);
+    case FA_BF16: return forward<__bf16>(a, out, os, lse, splits, per, part_o, part_ml, s);
+    case FA_F32: return forward<float>(a, out, os, lse, splits, per, part_o, part_ml, s);
     default: return FA_E_DTYPE;
   }
 }

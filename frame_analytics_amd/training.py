@@ -16,6 +16,7 @@ raises instead of taking it.
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple, Union
@@ -36,6 +37,21 @@ _MOST_SLOTS = 4225
 # --------------------------------------------------------------------------- #
 # positions
 # --------------------------------------------------------------------------- #
+
+
+@functools.lru_cache(maxsize=256)
+def _bucket_starts(n: int, max_distance: int) -> Tuple[int, ...]:
+    """Where rows n // 2 + 1, n // 2 + 2, ... of a direction's n rows start."""
+    half, wide = n // 2, n - n // 2
+    starts, at = [], half
+    for j in range(1, wide):
+        least = half ** (wide - j) * max_distance ** j
+        # the smallest whole number with at ** wide >= least
+        at = max(at, math.floor(math.exp(math.log(least) / wide)) - 1)
+        while at ** wide < least:
+            at += 1
+        starts.append(at)
+    return tuple(starts)
 
 
 @dataclass(frozen=True)
@@ -69,17 +85,9 @@ class LinePositions:
         for name, value in (("num_buckets", int(num_buckets)), ("max_distance", int(max_distance)),
                             ("bidirectional", bool(bidirectional))):
             object.__setattr__(self, name, value)
-        half, wide = n // 2, n - n // 2
-        starts, at = [], half
-        for j in range(1, wide):
-            least = half ** (wide - j) * self.max_distance ** j
-            # the smallest whole number with at ** wide >= least
-            at = max(at, math.floor(math.exp(math.log(least) / wide)) - 1)
-            while at ** wide < least:
-                at += 1
-            starts.append(at)
-        object.__setattr__(self, "_starts", tuple(starts))
-        object.__setattr__(self, "_far", starts[-1] if starts else half)
+        starts = _bucket_starts(n, self.max_distance)
+        object.__setattr__(self, "_starts", starts)
+        object.__setattr__(self, "_far", starts[-1] if starts else n // 2)
         if self.slots > _MOST_SLOTS:
             raise ValueError(f"{self.slots} distances before the last bucket; at most "
                              f"{_MOST_SLOTS} are supported")
@@ -251,12 +259,10 @@ class _RelativeAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, plan):
-        need = any(ctx.needs_input_grad[:4])
-        out, lse, kept = backend_training.rel_attention(q, k, v, table, plan, need)
-        if need:
-            extra = [t for t in (plan.mask, plan.key_lengths, plan.q_starts) if t is not None]
-            ctx.save_for_backward(*kept, out, lse, *extra)
-            ctx.plan = plan
+        out, lse, kept = backend_training.rel_attention(q, k, v, table, plan, True)
+        extra = [t for t in (plan.mask, plan.key_lengths, plan.q_starts) if t is not None]
+        ctx.save_for_backward(*kept, out, lse, *extra)
+        ctx.plan = plan
         return out
 
     @staticmethod
@@ -395,7 +401,10 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
         positions, float(q.shape[3] ** -0.5 if scale is None else scale), bool(causal), mask,
         key_lengths, q_start)
     if _route(q, "relative_attention", backend_hint):
-        return _RelativeAttention.apply(q, k, v, table, plan)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                        or table.requires_grad):
+            return _RelativeAttention.apply(q, k, v, table, plan)
+        return backend_training.rel_attention(q, k, v, table, plan, False)[0]
     return _portable_attention(q, k, v, table, plan)
 
 

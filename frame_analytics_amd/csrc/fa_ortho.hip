@@ -27,7 +27,7 @@ namespace {
 
 typedef _Float16 f16;
 constexpr int NT = 256;
-constexpr int SUMS = 64;                     // partial sums of squares per matrix
+constexpr int SUMS = 512;                    // most partial sums of squares per matrix
 constexpr float SX = 2048.0f, SP = 1024.0f;  // scale of X and A, of the polynomial
 
 template <typename T> __device__ inline float widen(T v) { return static_cast<float>(v); }
@@ -50,13 +50,30 @@ struct Bufs {
 // ---------------------------------------------------------------------------
 // |g|^2, then X and its transpose
 // ---------------------------------------------------------------------------
+// Eight elements a thread, 16 bytes (or twice) at once where the matrix is aligned for
+// it; the sums are float64, in a fixed order.
 template <typename T>
-__global__ __launch_bounds__(NT) void ortho_norm_kernel(const T* g, int64_t count, double* sums) {
+__global__ __launch_bounds__(NT) void ortho_norm_kernel(const T* g, int64_t count, bool wide, double* sums) {
   const T* p = g + blockIdx.y * count;
   double acc = 0.0;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(NT) + threadIdx.x; i < count; i += NT * SUMS) {
-    const double v = static_cast<double>(widen(p[i]));
-    acc += v * v;
+  for (int64_t i = (blockIdx.x * static_cast<int64_t>(NT) + threadIdx.x) * 8; i < count;
+       i += static_cast<int64_t>(gridDim.x) * NT * 8) {
+    float v[8];
+    if (wide && i + 8 <= count) {
+      constexpr int W = 16 / sizeof(T);
+      typedef typename std::conditional<W == 8, typename Mat<T>::V8, typename Mat<T>::V4>::type V;
+#pragma unroll
+      for (int e = 0; e < 8; e += W) {
+        const V x = *reinterpret_cast<const V*>(p + i + e);
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[e + k] = widen(x[k]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = i + e < count ? widen(p[i + e]) : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc += static_cast<double>(v[e]) * v[e];
   }
   __shared__ double smem[WAVES_PER_BLOCK];
   const double s = block_sum(acc, smem);
@@ -69,16 +86,31 @@ __device__ inline void put(f16* hi, f16* lo, int64_t at, float v) {
   if (lo) lo[at] = f16(v - float(h));
 }
 
+// Four neighbours, 8-byte aligned.
+__device__ inline void put4(f16* hi, f16* lo, int64_t at, const float* v) {
+  f16x4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = f16(v[e]);
+    l[e] = f16(v[e] - float(h[e]));
+  }
+  *reinterpret_cast<f16x4*>(hi + at) = h;
+  if (lo) *reinterpret_cast<f16x4*>(lo + at) = l;
+}
+
 constexpr int PT = 64;  // side of a transposed piece
 template <typename T>
 __global__ __launch_bounds__(NT) void ortho_prep_kernel(const T* g, int rows, int cols, int m, int n,
-                                                        int mp, int np, double eps, Bufs w) {
+                                                        int mp, int np, int parts, double eps,
+                                                        Bufs w) {
   __shared__ float tile[PT][PT + 1];
   __shared__ double smem[WAVES_PER_BLOCK];
   __shared__ int exponent;
   const int b = blockIdx.z;
   {
-    const double s = block_sum(threadIdx.x < SUMS ? w.sums[b * SUMS + threadIdx.x] : 0.0, smem);
+    double own = 0.0;
+    for (int t = threadIdx.x; t < parts; t += NT) own += w.sums[b * SUMS + t];
+    const double s = block_sum(own, smem);
     if (threadIdx.x == 0) {
       const double norm = sqrt(s) + eps;
       int ex = 0;
@@ -139,15 +171,20 @@ __device__ inline void upper(int t, int k, int* ti, int* tj) {
   *tj = i + t - before(i);
 }
 
-template <int TM, bool PAIR, int MODE, typename T>
-__global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* out) {
+// The KG groups of four waves of a workgroup take every KG-th piece of k, each with LDS
+// of its own; their sums are added in order of the groups.
+template <int TM, int KG, bool PAIR, int MODE, typename T>
+__global__ __launch_bounds__(NT * KG) void ortho_product_kernel(Bufs w, Step st, T* out) {
   constexpr int BK = PAIR ? 32 : 64, PARTS = PAIR ? 2 : 1, WT = TM / 2, NB = WT / 32;
+  constexpr int BUFS = KG > 1 ? 1 : 2;
   using TL = Tile<f16, BK>;
   using M = Mat<f16>;
   constexpr int PIECE = TM * TL::LD;
   extern __shared__ __align__(16) unsigned char smem[];
-  f16* lds = reinterpret_cast<f16*>(smem);  // [2][A, B][PARTS][TM][LD]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+  // [KG][BUFS][A, B][PARTS][TM][LD]
+  f16* lds = reinterpret_cast<f16*>(smem) + kg * BUFS * 2 * PARTS * PIECE;
+  const int tid = threadIdx.x & (NT - 1), lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
   const int per = MODE == STEP ? st.tiles_i * st.tiles_j : st.tiles_i * (st.tiles_i + 1) / 2;
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int b = wg / per, t = wg % per;
@@ -170,11 +207,12 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* o
     bp[s] = B[s] + bbase + static_cast<int64_t>(tj) * TM * K;
   }
   TileLoad<f16, BK, TM, NT, true> al[PARTS], bl[PARTS];
-  auto load = [&](int k) {
+  auto load = [&](int piece) {  // past the end: zeros
+    const int rows = piece * BK < K ? TM : 0, k = rows ? piece * BK : 0;
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) {
-      al[s].load(ap[s] + k, K, TM, BK, 8, tid);
-      bl[s].load(bp[s] + k, K, TM, BK, 8, tid);
+      al[s].load(ap[s] + k, K, rows, BK, 8, tid);
+      bl[s].load(bp[s] + k, K, rows, BK, 8, tid);
     }
   };
   auto store = [&](int buf) {
@@ -192,14 +230,14 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* o
     for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  load(0);
+  const int rounds = (K / BK + KG - 1) / KG;
+  load(kg);
   store(0);
-  const int steps = K / BK;
-  for (int k = 0; k < steps; ++k) {
+  for (int k = 0; k < rounds; ++k) {
     __syncthreads();
-    if (k + 1 < steps) load((k + 1) * BK);
-    const f16* la = lds + ((k & 1) * 2 + 0) * PARTS * PIECE;
-    const f16* lb = lds + ((k & 1) * 2 + 1) * PARTS * PIECE;
+    if (k + 1 < rounds) load((k + 1) * KG + kg);
+    const f16* la = lds + ((k % BUFS) * 2 + 0) * PARTS * PIECE;
+    const f16* lb = lds + ((k % BUFS) * 2 + 1) * PARTS * PIECE;
 #pragma unroll
     for (int c = 0; c < BK / 16; ++c) {
       f16x8 af[PARTS][NB], bf[PARTS][NB];
@@ -221,7 +259,41 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* o
           }
         }
     }
-    if (k + 1 < steps) store((k + 1) & 1);
+    if (k + 1 < rounds) {
+      if (BUFS == 1) __syncthreads();
+      store((k + 1) % BUFS);
+    }
+  }
+  if constexpr (KG > 1) {
+    // group g finishes the registers r with (r / 4) % KG = g
+    static_assert(KG == 4, "a group for each four registers");
+    float* part = reinterpret_cast<float*>(smem);  // [KG][4 waves][NB * NB][64 lanes][16]
+    constexpr int GROUP = 4 * NB * NB * 1024;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4)
+          *reinterpret_cast<f32x4*>(part + kg * GROUP + ((wave * NB + i) * NB + j) * 1024 + r4 * 256 + lane * 4) =
+              f32x4{acc[i][j][4 * r4], acc[i][j][4 * r4 + 1], acc[i][j][4 * r4 + 2], acc[i][j][4 * r4 + 3]};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(part + g * GROUP + ((wave * NB + i) * NB + j) * 1024 +
+                                                          kg * 256 + lane * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = v[e];  // (read below as register 4 r4 + e, r4 = 0)
+      }
   }
 
   const float f = st.first ? w.f[b] : 1.0f;
@@ -231,11 +303,12 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* o
     for (int bj = 0; bj < NB; ++bj) {
       const int j = tj * TM + wj + 32 * bj + col;
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
+      for (int q4 = 0; q4 < (KG > 1 ? 1 : 4); ++q4) {
+        const int r4 = KG > 1 ? kg : q4;
         const int i = ti * TM + wi + 32 * bi + 8 * r4 + 4 * hh;  // four rows from here
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[bi][bj][4 * r4 + e];
+        for (int e = 0; e < 4; ++e) v[e] = acc[bi][bj][4 * q4 + e];
         if constexpr (MODE == GRAM || MODE == SQUARE) {
           f16* const* dst = MODE == GRAM ? w.a : w.p;
           const int64_t o = b * as;
@@ -251,11 +324,7 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* o
             }
             put(dst[0], PAIR ? dst[1] : nullptr, at, v[e]);
           }
-          if (ti != tj) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              put(dst[0], PAIR ? dst[1] : nullptr, o + static_cast<int64_t>(j) * st.mp + i + e, v[e]);
-          }
+          if (ti != tj) put4(dst[0], PAIR ? dst[1] : nullptr, o + static_cast<int64_t>(j) * st.mp + i, v);
         } else {
           const int64_t o = b * xs;
 #pragma unroll
@@ -283,9 +352,9 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(Bufs w, Step st, T* o
             for (int e = 0; e < 4; ++e) {
               const int64_t at = o + static_cast<int64_t>(i + e) * st.np + j;
               put(w.x[0], PAIR ? w.x[1] : nullptr, at, v[e]);
-              put(w.xt_out[0], PAIR ? w.xt_out[1] : nullptr, o + static_cast<int64_t>(j) * st.mp + i + e, v[e]);
               if (!PAIR && st.write_f) w.xf[at] = v[e];
             }
+            put4(w.xt_out[0], PAIR ? w.xt_out[1] : nullptr, o + static_cast<int64_t>(j) * st.mp + i, v);
           }
         }
       }
@@ -308,7 +377,10 @@ inline int plan(int dtype, int batch, int rows, int cols, Plan* p) {
   // up to 64 rows a product is a launch's time whatever its precision, and little
   // averages the noise of single float16
   p->parts = dtype == FA_BF16 && p->m > 64 ? 1 : 2;
-  p->tile = 128;
+  // 128 x 128 tiles where they make two workgroups for every compute unit of the card
+  // (its 256 are assumed here: the workspace's size depends on the tile)
+  const int64_t tiles = static_cast<int64_t>(batch) * ((p->m + 127) / 128) * ((p->n + 127) / 128);
+  p->tile = tiles >= 512 ? 128 : 64;
   p->mp = (p->m + p->tile - 1) / p->tile * p->tile;
   p->np = (p->n + p->tile - 1) / p->tile * p->tile;
   const int64_t xs = static_cast<int64_t>(batch) * p->mp * p->np, as = static_cast<int64_t>(batch) * p->mp * p->mp;
@@ -330,25 +402,36 @@ inline int plan(int dtype, int batch, int rows, int cols, Plan* p) {
   return FA_OK;
 }
 
-template <int TM, bool PAIR, int MODE, typename T>
-int launch_product(const Bufs& w, const Step& st, int batch, T* out, hipStream_t s) {
-  constexpr int BK = PAIR ? 32 : 64, PARTS = PAIR ? 2 : 1;
-  constexpr size_t lds = size_t(4) * PARTS * TM * Tile<f16, BK>::LD * sizeof(f16);
-  const int64_t per = MODE == STEP ? static_cast<int64_t>(st.tiles_i) * st.tiles_j
-                                   : static_cast<int64_t>(st.tiles_i) * (st.tiles_i + 1) / 2;
-  if (per * batch > 0x7fffffff) return FA_E_SHAPE;
-  auto kernel = ortho_product_kernel<TM, PAIR, MODE, T>;
+template <int TM, int KG, bool PAIR, int MODE, typename T>
+int launch_tiles(const Bufs& w, const Step& st, int64_t wgs, T* out, hipStream_t s) {
+  constexpr int BK = PAIR ? 32 : 64, PARTS = PAIR ? 2 : 1, BUFS = KG > 1 ? 1 : 2;
+  constexpr size_t tiles = size_t(KG) * BUFS * 2 * PARTS * TM * Tile<f16, BK>::LD * sizeof(f16);
+  constexpr size_t sums = KG > 1 ? size_t(KG) * TM * TM * sizeof(float) : 0;
+  constexpr size_t lds = tiles > sums ? tiles : sums;
+  auto kernel = ortho_product_kernel<TM, KG, PAIR, MODE, T>;
   if (lds > 64 * 1024)
     FA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                    hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-  kernel<<<static_cast<unsigned>(per * batch), NT, lds, s>>>(w, st, out);
+  kernel<<<static_cast<unsigned>(wgs), NT * KG, lds, s>>>(w, st, out);
   FA_LAUNCH_CHECK();
   return FA_OK;
 }
 
+template <bool PAIR, int MODE, typename T>
+int launch_product(const Bufs& w, const Step& st, int tile, int batch, int device, T* out, hipStream_t s) {
+  const int64_t per = MODE == STEP ? static_cast<int64_t>(st.tiles_i) * st.tiles_j
+                                   : static_cast<int64_t>(st.tiles_i) * (st.tiles_i + 1) / 2;
+  const int64_t wgs = per * batch;
+  if (wgs > 0x7fffffff) return FA_E_SHAPE;
+  if (tile == 128) return launch_tiles<128, 1, PAIR, MODE, T>(w, st, wgs, out, s);
+  // few workgroups: k is split between four groups of waves
+  if (wgs < cu_count(device)) return launch_tiles<64, 4, PAIR, MODE, T>(w, st, wgs, out, s);
+  return launch_tiles<64, 1, PAIR, MODE, T>(w, st, wgs, out, s);
+}
+
 template <typename T, bool PAIR>
 int orthogonalize(const void* g, int batch, int rows, int cols, int steps, const Poly& poly, double eps,
-                  void* out, char* ws, const Plan& p, hipStream_t s) {
+                  void* out, char* ws, const Plan& p, int device, hipStream_t s) {
   const int64_t xs = static_cast<int64_t>(batch) * p.mp * p.np, as = static_cast<int64_t>(batch) * p.mp * p.mp;
   auto set = [&](f16** dst, int64_t off, int64_t count) {
     dst[0] = reinterpret_cast<f16*>(ws + off);
@@ -362,11 +445,14 @@ int orthogonalize(const void* g, int batch, int rows, int cols, int steps, const
   w.xf = PAIR ? nullptr : reinterpret_cast<float*>(ws + p.off_xf);
   w.f = reinterpret_cast<float*>(ws + p.off_f);
   w.sums = reinterpret_cast<double*>(ws + p.off_sums);
-  ortho_norm_kernel<T><<<dim3(SUMS, batch), NT, 0, s>>>(static_cast<const T*>(g),
-                                                        static_cast<int64_t>(rows) * cols, w.sums);
+  const int64_t count = static_cast<int64_t>(rows) * cols;
+  const int64_t want = (count + 8 * NT - 1) / (8 * NT);
+  const int parts = static_cast<int>(want < SUMS ? want : SUMS);
+  const bool wide = reinterpret_cast<uintptr_t>(g) % 16 == 0 && count * sizeof(T) % 16 == 0;
+  ortho_norm_kernel<T><<<dim3(parts, batch), NT, 0, s>>>(static_cast<const T*>(g), count, wide, w.sums);
   FA_LAUNCH_CHECK();
   ortho_prep_kernel<T><<<dim3(p.np / PT, p.mp / PT, batch), NT, 0, s>>>(
-      static_cast<const T*>(g), rows, cols, p.m, p.n, p.mp, p.np, eps, w);
+      static_cast<const T*>(g), rows, cols, p.m, p.n, p.mp, p.np, parts, eps, w);
   FA_LAUNCH_CHECK();
   Step st{};
   st.m = p.m;
@@ -384,9 +470,9 @@ int orthogonalize(const void* g, int batch, int rows, int cols, int steps, const
     st.last = k == steps - 1;
     st.read_f = k >= 1 && steps - k >= 3;
     st.write_f = steps - (k + 1) >= 3;
-    if (const int e = launch_product<128, PAIR, GRAM, T>(w, st, batch, o, s)) return e;
-    if (const int e = launch_product<128, PAIR, SQUARE, T>(w, st, batch, o, s)) return e;
-    if (const int e = launch_product<128, PAIR, STEP, T>(w, st, batch, o, s)) return e;
+    if (const int e = launch_product<PAIR, GRAM, T>(w, st, p.tile, batch, device, o, s)) return e;
+    if (const int e = launch_product<PAIR, SQUARE, T>(w, st, p.tile, batch, device, o, s)) return e;
+    if (const int e = launch_product<PAIR, STEP, T>(w, st, p.tile, batch, device, o, s)) return e;
     std::swap(w.xt, w.xt_out);
   }
   return FA_OK;
@@ -423,10 +509,10 @@ FA_API int fa_gpu_orthogonalize(const void* g, int dtype, int batch, int rows, i
   switch (dtype) {
     case FA_BF16:
       return p.parts == 1
-                 ? orthogonalize<__bf16, false>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s)
-                 : orthogonalize<__bf16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s);
-    case FA_F16: return orthogonalize<f16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s);
-    default: return orthogonalize<float, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, s);
+                 ? orthogonalize<__bf16, false>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s)
+                 : orthogonalize<__bf16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s);
+    case FA_F16: return orthogonalize<f16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s);
+    default: return orthogonalize<float, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s);
   }
 }
 

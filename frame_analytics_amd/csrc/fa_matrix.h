@@ -159,6 +159,13 @@ __device__ inline float both_sum(float v) {
   return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
 
+// LDS that one wave wrote is read by its other lanes after this.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // A tile of ROWS rows of DP elements in LDS, rows LD apart: 16 bytes of padding put
 // the rows that one instruction reads on different banks.
 template <typename T, int DP> struct Tile {
@@ -204,6 +211,13 @@ template <typename T, int DP> struct Tile {
   }
 };
 
+// A value that the compiler takes as new each time: offsets made from it are computed
+// where they are used, not kept in registers through a loop (there is one for each load).
+__device__ inline int afresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // A tile of ROWS rows on its way from memory to LDS: read into registers while the
 // tile before is worked on, stored after.  The first `valid` rows are read, the rest
 // and elements from D on are zeros.
@@ -212,21 +226,22 @@ template <typename T, int DP, int ROWS, int NT, bool WIDE> struct TileLoad {
   static constexpr int N = (ROWS * PER_ROW + NT - 1) / NT;
   typename Mat<T>::V8 r[N];
   __device__ inline void load(const T* base, int64_t stride, int valid, int D, int vec, int tid) {
-    const Rows<T> rows(base, stride);
+    static_assert(NT % PER_ROW == 0, "a thread keeps its columns");
+    constexpr int STEP = NT / PER_ROW;  // rows between a thread's pieces
     valid = min(valid, ROWS);
+    tid = afresh(tid);
+    const int row = tid / PER_ROW, d = (tid % PER_ROW) * 8;
     auto each = [&](auto read) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = tid + i * NT, row = c / PER_ROW;
-        r[i] = read(row, (c % PER_ROW) * 8, row < valid);
-      }
+      for (int i = 0; i < N; ++i)
+        r[i] = read(Rows<T>(base + i * STEP * stride, stride), row + i * STEP < valid);
     };
     if constexpr (WIDE)
-      each([&](int row, int d, bool on) { return rows.wide(row, d, D, on); });
+      each([&](const Rows<T>& rows, bool on) { return rows.wide(row, d, D, on); });
     else if (sizeof(T) == 2 && vec == 2)
-      each([&](int row, int d, bool on) { return rows.pairs(row, d, D, on); });
+      each([&](const Rows<T>& rows, bool on) { return rows.pairs(row, d, D, on); });
     else
-      each([&](int row, int d, bool on) { return rows.single(row, d, D, on); });
+      each([&](const Rows<T>& rows, bool on) { return rows.single(row, d, D, on); });
   }
   __device__ inline void store(T* lds, int tid) const {
 #pragma unroll
@@ -240,6 +255,36 @@ template <typename T, int DP, int ROWS, int NT, bool WIDE> struct TileLoad {
         *reinterpret_cast<f32x4*>(p) = f32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
         *reinterpret_cast<f32x4*>(p + 4) = f32x4{r[i][4], r[i][5], r[i][6], r[i][7]};
       }
+    }
+  }
+};
+
+// The same for 16-bit rows of an even number of elements on 4-byte boundaries: each
+// thread takes pairs, neighbouring threads neighbouring pairs, so an instruction covers
+// whole rows (TileLoad's 16-byte pieces, read 4 bytes at a time, cover each line four times).
+template <typename T, int DP, int ROWS, int NT> struct PairLoad {
+  static constexpr int PER_ROW = DP / 2;
+  static constexpr int N = ROWS * PER_ROW / NT;
+  static_assert(ROWS * PER_ROW % NT == 0, "whole rounds");
+  unsigned r[N];
+  __device__ inline void load(const T* base, int64_t stride, int valid, int D, int, int tid) {
+    static_assert(NT % PER_ROW == 0, "a thread keeps its columns");
+    constexpr int STEP = NT / PER_ROW;
+    tid = afresh(tid);
+    const int row = tid / PER_ROW, d = (tid % PER_ROW) * 2;
+    valid = d < D ? valid : 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const Rows<T> rows(base + i * STEP * stride, stride);
+      r[i] = __builtin_amdgcn_raw_buffer_load_b32(
+          rows.rsrc, row + i * STEP < valid ? row * rows.stride + d * int(sizeof(T)) : OUTSIDE, 0, 0);
+    }
+  }
+  __device__ inline void store(T* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + i * NT, row = c / PER_ROW, d = (c % PER_ROW) * 2;
+      *reinterpret_cast<unsigned*>(lds + row * Tile<T, DP>::LD + d) = r[i];
     }
   }
 };

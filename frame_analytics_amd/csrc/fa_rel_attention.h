@@ -24,6 +24,7 @@ struct RelAttn {
   const uint8_t* mask;
   int mask_b;
   int64_t mb, mh, mq, mk;
+  int mask4;  // four neighbouring keys' bytes of the mask are one aligned word
   int causal;
   float scale;
   __device__ inline int start(int b) const {
@@ -179,6 +180,8 @@ inline RelAttn rel_attn_args(const void* q, const void* k, const void* v, int B,
     a.mh = ms[1];
     a.mq = ms[2];
     a.mk = ms[3];
+    a.mask4 = a.mk == 1 && a.mq < (1 << 22) && (a.mb | a.mh | a.mq | Lk) % 4 == 0 &&
+              reinterpret_cast<uintptr_t>(mask) % 4 == 0;
   }
   a.causal = causal;
   a.scale = static_cast<float>(scale);
@@ -194,5 +197,31 @@ template <typename K> inline int launch_lds(K kernel, size_t bytes) {
                                    static_cast<int>(bytes)));
   return FA_OK;
 }
+
+// fa_rel_bias.hip: dtable from `parts` rows of n sums by slot for each head
+template <typename T>
+void launch_table_sum(const float* partial, int parts, int n, const int* row_of, int rows, int H,
+                      T* dtable, hipStream_t s);
+
+// fa_rel_attention_rows.hip: few queries against many keys
+int rows_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int device, int64_t* bytes);
+bool rows_serve(const RelAttn& a);
+int rows_forward(int dtype, const RelAttn& a, void* out, const View& os, float* lse, void* ws,
+                 int64_t ws_bytes, int device, hipStream_t s);
+
+// fa_rel_attention_window.hip: windows of up to 64 tokens
+struct WindowGrads {
+  const void* dout;
+  View gs;
+  void *dq, *dk, *dv;
+  View dqs, dks, dvs;
+  float* parts;  // [H][window_parts][n], or null: the table needs no gradient
+};
+bool window_serve(const RelAttn& a);
+int window_parts(int B, int H, int device);
+int window_forward(int dtype, const RelAttn& a, void* out, const View& os, float* lse, int device,
+                   hipStream_t s);
+int window_backward(int dtype, const RelAttn& a, const WindowGrads& g, int rows, void* dtable, int device,
+                    hipStream_t s);
 
 }  // namespace fa

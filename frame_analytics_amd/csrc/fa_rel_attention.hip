@@ -10,12 +10,6 @@
 
 namespace fa {
 
-// fa_rel_attention_rows.hip: few queries against many keys
-int rows_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int device, int64_t* bytes);
-bool rows_serve(const RelAttn& a);
-int rows_forward(int dtype, const RelAttn& a, void* out, const View& os, float* lse, void* ws,
-                 int64_t ws_bytes, int device, hipStream_t s);
-
 namespace {
 
 template <typename T, int DP> struct Shape {
@@ -247,6 +241,7 @@ FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int
                                   mask, mask_b, mask_strides, causal, scale);
   const View os{strides[9], strides[10], strides[11]};
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (window_serve(a)) return window_forward(dtype, a, out, os, lse, device, s);
   if (rows_serve(a)) return rows_forward(dtype, a, out, os, lse, workspace, workspace_bytes, device, s);
   switch (dtype) {
     case FA_F16: return forward<_Float16>(a, out, os, lse, s);

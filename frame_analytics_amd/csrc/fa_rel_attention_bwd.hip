@@ -12,10 +12,6 @@
 
 namespace fa {
 
-template <typename T>
-void launch_table_sum(const float* partial, int parts, int n, const int* row_of, int rows, int H,
-                      T* dtable, hipStream_t s);
-
 namespace {
 
 struct Grads {
@@ -563,6 +559,11 @@ FA_API int fa_gpu_rel_attention_backward(
   g.dk = dk;
   g.dv = dv;
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (window_serve(a)) {
+    // (its parts are no more than the workspace's: one for each batch entry at most)
+    const WindowGrads w{dout, g.gs, dq, dk, dv, g.dqs, g.dks, g.dvs, g.parts};
+    return window_backward(dtype, a, w, rows, dtable, device, s);
+  }
   switch (dtype) {
     case FA_F16: return backward<_Float16>(a, g, rows, dtable, s);
     case FA_BF16: return backward<__bf16>(a, g, rows, dtable, s);

@@ -18,8 +18,6 @@
 
 namespace fa {
 
-int rows_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int device, int64_t* bytes);
-
 namespace {
 
 constexpr int NW = 4, NT = NW * 64, BN = 32;
@@ -211,9 +209,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
 #pragma unroll
         for (int i = 0; i < CH; ++i) s[n][w] = mma16<T>(kf[w][i], qf[n][i], s[n][w]);
       }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_sync();
     if (k0 + stride < end) load(k0 + stride);
     const int kind = block_kind(a.pos, s0 - (k0 + 31), s0 + a.Lq - 1 - k0);
     const bool partial = a.mask || k0 + 32 > len || (a.causal && k0 + 31 > s0);
@@ -265,9 +261,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
       for (int n = 0; n < NC; ++n)
         o[n][i] = partial ? guarded16<T>(vf, p[n], o[n][i]) : mma16<T>(vf, p[n], o[n][i]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_sync();
   }
 
   // join the waves: O^T in LDS as [d][row], each wave's in its own region

@@ -50,7 +50,7 @@ FA_API int fa_gpu_rel_bias_backward(const void* up, const int64_t* up_strides, i
 /*
  * out = softmax(scale * q k^T + bias) v over the keys that query i of batch entry
  * b may see: j < key_lengths[b] (null: Lk), j <= start + i where causal, and
- * mask[b % mask_b, h, i, j] != 0 (null: all).  A row that sees none is 0.
+ * mask[b % mask_b, h, i, j] is 1 (bytes, 0 or 1; null: all).  A row that sees none is 0.
  *
  * q, out: [B, H, Lq, D]; k, v: [B, Hk, Lk, D], H a multiple of Hk: query head h
  * reads key head h / (H / Hk).  strides: 12 int64 in elements, {batch, head, token}

@@ -180,7 +180,7 @@ inline RelAttn rel_attn_args(const void* q, const void* k, const void* v, int B,
     a.mh = ms[1];
     a.mq = ms[2];
     a.mk = ms[3];
-    a.mask4 = a.mk == 1 && a.mq < (1 << 22) && (a.mb | a.mh | a.mq | Lk) % 4 == 0 &&
+    a.mask4 = mask && a.mk == 1 && a.mq < (1 << 22) && (a.mb | a.mh | a.mq | Lk) % 4 == 0 &&
               reinterpret_cast<uintptr_t>(mask) % 4 == 0;
   }
   a.causal = causal;

@@ -44,40 +44,46 @@ __device__ inline uint32_t reachable(const RelAttn& a, const Pairs& p, int len) 
   return bits;
 }
 
-// ... and by the mask.  Its bytes are 0 or 1: a product gathers four into four bits.
-__device__ inline uint32_t allowed(const RelAttn& a, const Pairs& p, int b, int h) {
-  const uint8_t* mask = a.mask_of(b, h);
-  uint32_t bits = 0;
-  if (a.mask4) {
+// ... and by the mask.  Its bytes are 0 or 1.  Where four are a word, the words of the
+// next window are read with its tiles (memory answers in order: a read made later would
+// wait for them), and a product gathers a word into four bits.
+struct MaskWords {
+  uint32_t word[8];
+  __device__ inline void load(const RelAttn& a, const Pairs& p, int b, int h) {
     const __amdgpu_buffer_rsrc_t rsrc =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(mask), 0, 0x7fffffff, 0x00020000);
-    const int at = p.qc * static_cast<int>(a.mq) + 4 * p.hh;
-    uint32_t word[8];
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.mask_of(b, h)), 0, 0x7fffffff, 0x00020000);
+    const int hh = afresh(p.hh), at = p.qc * static_cast<int>(a.mq) + 4 * hh;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const int k = 32 * (t >> 2) + 8 * (t & 3);
-      word[t] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, k + 4 * p.hh < a.Lk ? at + k : OUTSIDE, 0, 0);
+      word[t] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, k + 4 * hh < a.Lk ? at + k : OUTSIDE, 0, 0);
     }
+  }
+  __device__ inline uint32_t bits() const {
+    uint32_t r = 0;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) bits |= (word[t] * 0x01020408u >> 24 & 15u) << (4 * t);
-  } else {
+    for (int t = 0; t < 8; ++t) r |= (word[t] * 0x01020408u >> 24 & 15u) << (4 * t);
+    return r;
+  }
+};
+__device__ inline uint32_t allowed(const RelAttn& a, const Pairs& p, int b, int h) {
+  const uint8_t* mask = a.mask_of(b, h);
+  uint32_t bits = 0;
 #pragma unroll 1
-    for (int t = 0; t < 32; ++t) {
-      const int k = p.key(t >> 4, t & 15);
-      if (k < a.Lk && mask[p.qc * a.mq + k * a.mk]) bits |= 1u << t;
-    }
+  for (int t = 0; t < 32; ++t) {
+    const int k = p.key(t >> 4, t & 15);
+    if (k < a.Lk && mask[p.qc * a.mq + k * a.mk]) bits |= 1u << t;
   }
   return bits;
 }
 
 // The wave's 32 rows of a block (C layout, transposed: lane l's row is l % 32) to memory by
-// way of the wave's rows of an LDS tile, so that neighbouring lanes write neighbouring
+// way of LDS of the wave's own, so that neighbouring lanes write neighbouring
 // elements; rows from `valid` on and elements from D on are dropped.
 template <typename T, int DP, int ACCESS>
-__device__ inline void store_rows(T* tile, const f32x16 (&acc)[DP / 32], float f, T* base, int64_t stride,
+__device__ inline void store_rows(T* own, const f32x16 (&acc)[DP / 32], float f, T* base, int64_t stride,
                                   int row0, int valid, int D, int lane) {
   constexpr int LD = Tile<T, DP>::LD;
-  T* own = tile + row0 * LD;
   const int hh = lane >> 5, col = lane & 31;
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i)
@@ -156,6 +162,7 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
   T* qt = reinterpret_cast<T*>(smem);
   T* kt = qt + L * TL::LD;
   T* vt = kt + L * TL::LD;
+  T* ot = vt + L * TL::LD;
   const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
@@ -166,24 +173,31 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
   load_pair_bias<T>(bias, a, p, h);
   const uint32_t reach = reachable(a, p, a.Lk);
   Load<T, DP, ACCESS> ql, kl, vl;
+  MaskWords words;
   auto load = [&](int b) {
     const int len = a.keys(b);
+    if (a.mask4) words.load(a, p, b, h);
     ql.load(static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h, a.qs.t, a.Lq, a.D, a.vec, tid);
     kl.load(static_cast<const T*>(a.k) + b * a.ks.b + h * a.ks.h, a.ks.t, len, a.D, a.vec, tid);
     vl.load(static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h, a.vs.t, len, a.D, a.vec, tid);
   };
-  load(chunk);
-  for (int b = chunk; b < a.B; b += chunks) {
-    __syncthreads();  // the window before is done with the tiles
+  int len;
+  uint32_t seen;
+  auto store = [&](int b) {
+    len = a.keys(b);
+    seen = len == a.Lk ? reach : reachable(a, p, len);
+    if (a.mask) seen &= a.mask4 ? words.bits() : allowed(a, p, b, h);
     ql.store(qt, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
+  };
+  load(chunk);
+  store(chunk);
+  for (int b = chunk; b < a.B; b += chunks) {
     __syncthreads();
-    if (b + chunks < a.B) load(b + chunks);
-    const int len = a.keys(b);
+    const bool more = b + chunks < a.B;
+    if (more) load(b + chunks);
     const bool all = !a.mask && len == L && !a.causal;
-    uint32_t seen = len == a.Lk ? reach : reachable(a, p, len);
-    if (a.mask) seen &= allowed(a, p, b, h);
     typename M::V8 qf[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) qf[i] = TL::straight(qt, wave * 32 + col, 16 * i + 8 * hh);
@@ -216,8 +230,11 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
       }
     }
     l = both_sum(l);
-    // the wave's rows of the queries' tile have been read, by it alone
-    store_rows<T, DP, ACCESS>(qt, o, l == 0.0f ? 0.0f : 1.0f / l, out + b * os.b + h * os.h, os.t, wave * 32,
+    // the next window goes to LDS before this one's results go to memory: a wait for the
+    // reads would wait for writes made before it
+    __syncthreads();
+    if (more) store(b + chunks);
+    store_rows<T, DP, ACCESS>(ot + wave * 32 * TL::LD, o, l == 0.0f ? 0.0f : 1.0f / l, out + b * os.b + h * os.h, os.t, wave * 32,
                               a.Lq, a.D, lane);
     if (lse && p.q < a.Lq) {
       if (hh == 0)
@@ -256,26 +273,33 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
 #pragma unroll
     for (int r = 0; r < 16; ++r) total[nb][r] = 0.0f;
   Load<T, DP, ACCESS> ql, gl, kl, vl;
+  MaskWords words;
   auto load = [&](int b) {
     const int len = a.keys(b);
+    if (a.mask4) words.load(a, p, b, h);
     ql.load(static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h, a.qs.t, a.Lq, a.D, a.vec, tid);
     gl.load(dout + b * gs.b + h * gs.h, gs.t, a.Lq, a.D, a.vec, tid);
     kl.load(static_cast<const T*>(a.k) + b * a.ks.b + h * a.ks.h, a.ks.t, len, a.D, a.vec, tid);
     vl.load(static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h, a.vs.t, len, a.D, a.vec, tid);
   };
-  load(chunk);
-  for (int b = chunk; b < a.B; b += chunks) {
-    __syncthreads();
+  int len;
+  uint32_t seen;
+  auto store = [&](int b) {
+    len = a.keys(b);
+    seen = len == a.Lk ? reach : reachable(a, p, len);
+    if (a.mask) seen &= a.mask4 ? words.bits() : allowed(a, p, b, h);
     ql.store(qt, tid);
     gl.store(gt, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
+  };
+  load(chunk);
+  store(chunk);
+  for (int b = chunk; b < a.B; b += chunks) {
     __syncthreads();
-    if (b + chunks < a.B) load(b + chunks);
-    const int len = a.keys(b);
+    const bool more = b + chunks < a.B;
+    if (more) load(b + chunks);
     const bool all = !a.mask && len == L && !a.causal;
-    uint32_t seen = len == a.Lk ? reach : reachable(a, p, len);
-    if (a.mask) seen &= allowed(a, p, b, h);
     f32x16 s[2], dp[2];
     {
       typename M::V8 qf[CH];
@@ -366,28 +390,31 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
           acc[i] = M::mma(kf, df, acc[i]);
         }
       }
-    __syncthreads();  // P and dS of all queries; the tiles of K and V have been read
-    store_rows<T, DP, ACCESS>(vt, acc, a.scale, dq + b * dqs.b + h * dqs.h, dqs.t, wave * 32, a.Lq, a.D, lane);
+    __syncthreads();  // P and dS of all queries
     // the wave's keys: 32 wave + col
+    f32x16 acc_v[OB], acc_k[OB];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const T* left = which ? qt : gt;
-      const T* right = which ? dt : pt;
+    for (int i = 0; i < OB; ++i)
 #pragma unroll
-      for (int i = 0; i < OB; ++i)
+      for (int r = 0; r < 16; ++r) acc_v[i][r] = acc_k[i][r] = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
+    for (int k = 0; k < L / 16; ++k) {
+      const typename M::V8 pf = PL::transposed(pt, 16 * k, 32 * wave, lane);
+      const typename M::V8 df = PL::transposed(dt, 16 * k, 32 * wave, lane);
 #pragma unroll
-      for (int k = 0; k < L / 16; ++k) {
-        const typename M::V8 rf = PL::transposed(right, 16 * k, 32 * wave, lane);
-#pragma unroll
-        for (int i = 0; i < OB; ++i) acc[i] = M::mma(TL::transposed(left, 16 * k, 32 * i, lane), rf, acc[i]);
+      for (int i = 0; i < OB; ++i) {
+        acc_v[i] = M::mma(TL::transposed(gt, 16 * k, 32 * i, lane), pf, acc_v[i]);
+        acc_k[i] = M::mma(TL::transposed(qt, 16 * k, 32 * i, lane), df, acc_k[i]);
       }
-      if (which)
-        store_rows<T, DP, ACCESS>(kt, acc, a.scale, dk + b * dks.b + h * dks.h, dks.t, wave * 32, a.Lk, a.D, lane);
-      else
-        store_rows<T, DP, ACCESS>(kt, acc, 1.0f, dv + b * dvs.b + h * dvs.h, dvs.t, wave * 32, a.Lk, a.D, lane);
     }
+    // the next window goes to LDS before this one's results go to memory: a wait for the
+    // reads would wait for writes made before it
+    __syncthreads();
+    if (more) store(b + chunks);
+    T* own = pt + wave * 32 * PL::LD;
+    store_rows<T, DP, ACCESS>(own, acc, a.scale, dq + b * dqs.b + h * dqs.h, dqs.t, wave * 32, a.Lq, a.D, lane);
+    store_rows<T, DP, ACCESS>(own, acc_v, 1.0f, dv + b * dvs.b + h * dvs.h, dvs.t, wave * 32, a.Lk, a.D, lane);
+    store_rows<T, DP, ACCESS>(own, acc_k, a.scale, dk + b * dks.b + h * dks.h, dks.t, wave * 32, a.Lk, a.D, lane);
   }
   if (TABLE) {
     const int n = a.pos.n;
@@ -423,7 +450,7 @@ inline int chunks_of(int B, int H, int device) {
 
 template <typename T, int DP, int ACCESS>
 int launch_forward(const RelAttn& a, T* out, const View& os, float* lse, int chunks, hipStream_t s) {
-  const size_t lds = 3 * tile_bytes<T, DP>();
+  const size_t lds = 4 * tile_bytes<T, DP>();
   auto kernel = window_kernel<T, DP, ACCESS>;
   if (const int e = launch_lds(kernel, lds)) return e;
   kernel<<<static_cast<unsigned>(chunks * a.H), NT, lds, s>>>(a, out, os, lse, chunks);

@@ -218,6 +218,14 @@ __device__ inline int afresh(int v) {
   return v;
 }
 
+// Whether any element of a register of T is not finite: its exponent is all ones.
+template <typename T> __device__ inline bool not_finite(unsigned x) {
+  if constexpr (sizeof(T) == 4) return (x & 0x7f800000u) == 0x7f800000u;
+  constexpr unsigned E = std::is_same<T, _Float16>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr unsigned ONE = E & (~E << 1);  // an exponent's lowest bit: all ones carry into the sign
+  return (((x & E) + ONE) & 0x80008000u) != 0;
+}
+
 // A tile of ROWS rows on its way from memory to LDS: read into registers while the
 // tile before is worked on, stored after.  The first `valid` rows are read, the rest
 // and elements from D on are zeros.
@@ -225,6 +233,18 @@ template <typename T, int DP, int ROWS, int NT, bool WIDE> struct TileLoad {
   static constexpr int PER_ROW = DP / 8;
   static constexpr int N = (ROWS * PER_ROW + NT - 1) / NT;
   typename Mat<T>::V8 r[N];
+  __device__ inline bool not_finite() const {
+    constexpr int W = sizeof(T) * 2;
+    typedef unsigned words __attribute__((ext_vector_type(W)));
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const words w = __builtin_bit_cast(words, r[i]);
+#pragma unroll
+      for (int e = 0; e < W; ++e) bad |= fa::not_finite<T>(w[e]);
+    }
+    return bad;
+  }
   __device__ inline void load(const T* base, int64_t stride, int valid, int D, int vec, int tid) {
     static_assert(NT % PER_ROW == 0, "a thread keeps its columns");
     constexpr int STEP = NT / PER_ROW;  // rows between a thread's pieces
@@ -267,6 +287,12 @@ template <typename T, int DP, int ROWS, int NT> struct PairLoad {
   static constexpr int N = ROWS * PER_ROW / NT;
   static_assert(ROWS * PER_ROW % NT == 0, "whole rounds");
   unsigned r[N];
+  __device__ inline bool not_finite() const {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) bad |= fa::not_finite<T>(r[i]);
+    return bad;
+  }
   __device__ inline void load(const T* base, int64_t stride, int valid, int D, int, int tid) {
     static_assert(NT % PER_ROW == 0, "a thread keeps its columns");
     constexpr int STEP = NT / PER_ROW;

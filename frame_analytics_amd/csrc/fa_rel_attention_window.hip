@@ -135,7 +135,8 @@ __device__ inline void load_pair_bias(float (&bias)[2][16], const RelAttn& a, co
 // Scores of the wave's queries, hidden ones -inf; their maximum (0 where there is none).
 template <typename T, int DP>
 __device__ inline float scores(f32x16 (&s)[2], const T* kt, const typename Mat<T>::V8 (&qf)[DP / 16],
-                               const float (&bias)[2][16], float c, uint32_t seen, int col, int hh) {
+                               const float (&bias)[2][16], float c, bool all, uint32_t seen, int col,
+                               int hh) {
   float top = -INF;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb) {
@@ -145,16 +146,19 @@ __device__ inline float scores(f32x16 (&s)[2], const T* kt, const typename Mat<T
     for (int i = 0; i < DP / 16; ++i)
       s[nb] = Mat<T>::mma(Tile<T, DP>::straight(kt, 32 * nb + col, 16 * i + 8 * hh), qf[i], s[nb]);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[nb][r] = seen >> (16 * nb + r) & 1 ? s[nb][r] * c + bias[nb][r] : -INF;
-      top = fmaxf(top, s[nb][r]);
+    for (int r = 0; r < 16; ++r) s[nb][r] = s[nb][r] * c + bias[nb][r];
+    if (!all) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[nb][r] = seen >> (16 * nb + r) & 1 ? s[nb][r] : -INF;
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
   }
   return both_max(top);
 }
 
 template <typename T, int DP, int ACCESS>
-__global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View os, float* lse, int chunks) {
+__global__ __launch_bounds__(NT, sizeof(T) == 2 && DP == 32 ? 3 : 2) void window_kernel(RelAttn a, T* out, View os, float* lse, int chunks) {
   using M = Mat<T>;
   using TL = Tile<T, DP>;
   constexpr int CH = DP / 16, OB = DP / 32;
@@ -163,6 +167,7 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
   T* kt = qt + L * TL::LD;
   T* vt = kt + L * TL::LD;
   T* ot = vt + L * TL::LD;
+  __shared__ int wild[NW];  // whether a wave brought a value that is not finite
   const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
@@ -190,19 +195,22 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
     ql.store(qt, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
+    const bool bad = __ballot(vl.not_finite()) != 0;
+    if (lane == 0) wild[wave] = bad;
   };
   load(chunk);
   store(chunk);
   for (int b = chunk; b < a.B; b += chunks) {
     __syncthreads();
+    const bool tame = (wild[0] | wild[1]) == 0;
     const bool more = b + chunks < a.B;
     if (more) load(b + chunks);
-    const bool all = !a.mask && len == L && !a.causal;
+    const bool all = __ballot(seen != ~0u) == 0;  // of the wave's queries
     typename M::V8 qf[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) qf[i] = TL::straight(qt, wave * 32 + col, 16 * i + 8 * hh);
     f32x16 s[2];
-    const float m = scores<T, DP>(s, kt, qf, bias, c, seen, col, hh);
+    const float m = scores<T, DP>(s, kt, qf, bias, c, all, seen, col, hh);
     const float sub = m == -INF ? 0.0f : m;
     float l = 0.0f;
     f32x16 o[OB];
@@ -225,7 +233,7 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
 #pragma unroll
         for (int i = 0; i < OB; ++i) {
           const typename M::V8 vf = TL::transposed(vt, 32 * nb + 16 * half, 32 * i, lane);
-          o[i] = all ? M::mma(vf, pf, o[i]) : guarded<T>(vf, pf, o[i]);
+          o[i] = all || tame ? M::mma(vf, pf, o[i]) : guarded<T>(vf, pf, o[i]);
         }
       }
     }
@@ -259,6 +267,7 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
   T* pt = vt + L * TL::LD;
   T* dt = pt + L * PL::LD;
   float* sums = reinterpret_cast<float*>(smem);  // [NW][n], over the tiles at the end
+  __shared__ int wild[NW];  // whether a wave brought a key that is not finite
   const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
@@ -292,20 +301,23 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
     gl.store(gt, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
+    const bool bad = __ballot(kl.not_finite()) != 0;
+    if (lane == 0) wild[wave] = bad;
   };
   load(chunk);
   store(chunk);
   for (int b = chunk; b < a.B; b += chunks) {
     __syncthreads();
+    const bool tame = (wild[0] | wild[1]) == 0;
     const bool more = b + chunks < a.B;
     if (more) load(b + chunks);
-    const bool all = !a.mask && len == L && !a.causal;
+    const bool all = __ballot(seen != ~0u) == 0;  // of the wave's queries
     f32x16 s[2], dp[2];
     {
       typename M::V8 qf[CH];
 #pragma unroll
       for (int i = 0; i < CH; ++i) qf[i] = TL::straight(qt, wave * 32 + col, 16 * i + 8 * hh);
-      const float m = scores<T, DP>(s, kt, qf, bias, c, seen, col, hh);
+      const float m = scores<T, DP>(s, kt, qf, bias, c, all, seen, col, hh);
       const float sub = m == -INF ? 0.0f : m;
       float l = 0.0f;
 #pragma unroll
@@ -383,7 +395,7 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
 #pragma unroll
         for (int i = 0; i < OB; ++i) {
           typename M::V8 kf = TL::transposed(kt, 32 * nb + 16 * half, 32 * i, lane);
-          if (!all) {
+          if (!all && !tame) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) kf[e] = __builtin_fabsf(widen(kf[e])) < INF ? kf[e] : T(0);
           }
@@ -442,9 +454,9 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
   }
 }
 
-// Workgroups that share a head's windows: four for every compute unit over all heads.
-inline int chunks_of(int B, int H, int device) {
-  const int want = (4 * cu_count(device) + H - 1) / H;
+// Workgroups that share a head's windows: `fit` for every compute unit over all heads.
+inline int chunks_of(int B, int H, int device, int fit) {
+  const int want = (fit * cu_count(device) + H - 1) / H;
   return want < B ? want : B;
 }
 
@@ -483,7 +495,7 @@ int forward(RelAttn a, void* out, const View& os, float* lse, int device, hipStr
   const void* views[4] = {a.q, a.k, a.v, out};
   const View vs[4] = {a.qs, a.ks, a.vs, os};
   a.vec = widest_load<T>(views, vs, 4, a.D);
-  const int chunks = chunks_of(a.B, a.H, device);
+  const int chunks = chunks_of(a.B, a.H, device, sizeof(T) == 2 && a.D <= 32 ? 6 : 4);
   T* o = static_cast<T*>(out);
   auto go = [&](auto access) {
     constexpr int ACCESS = decltype(access)::value;
@@ -498,7 +510,7 @@ int backward(RelAttn a, const WindowGrads& g, int rows, void* dtable, int device
   const void* views[7] = {a.q, a.k, a.v, g.dout, g.dq, g.dk, g.dv};
   const View vs[7] = {a.qs, a.ks, a.vs, g.gs, g.dqs, g.dks, g.dvs};
   a.vec = widest_load<T>(views, vs, 7, a.D);
-  const int chunks = chunks_of(a.B, a.H, device);
+  const int chunks = chunks_of(a.B, a.H, device, 4);
   auto go = [&](auto access) {
     constexpr int ACCESS = decltype(access)::value;
     return a.D <= 32 ? launch_backward<T, 32, ACCESS>(a, g, chunks, s)
@@ -519,7 +531,7 @@ bool window_serve(const RelAttn& a) {
   return a.pos.grid_w > 0 && a.Lq <= L && a.H == a.Hk && a.D <= 64;
 }
 
-int window_parts(int B, int H, int device) { return chunks_of(B, H, device); }
+int window_parts(int B, int H, int device) { return chunks_of(B, H, device, 4); }
 
 int window_forward(int dtype, const RelAttn& a, void* out, const View& os, float* lse, int device,
                    hipStream_t s) {

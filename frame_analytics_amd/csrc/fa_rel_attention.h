@@ -24,7 +24,7 @@ struct RelAttn {
   const uint8_t* mask;
   int mask_b;
   int64_t mb, mh, mq, mk;
-  int mask4;  // four neighbouring keys' bytes of the mask are one aligned word
+  int mask64;  // the mask's rows are 64 bytes on 16-byte boundaries
   int causal;
   float scale;
   __device__ inline int start(int b) const {
@@ -180,8 +180,8 @@ inline RelAttn rel_attn_args(const void* q, const void* k, const void* v, int B,
     a.mh = ms[1];
     a.mq = ms[2];
     a.mk = ms[3];
-    a.mask4 = mask && a.mk == 1 && a.mq < (1 << 22) && (a.mb | a.mh | a.mq | Lk) % 4 == 0 &&
-              reinterpret_cast<uintptr_t>(mask) % 4 == 0;
+    a.mask64 = a.mk == 1 && Lk == 64 && a.mq >= 0 && a.mq < (1 << 22) && (a.mb | a.mh | a.mq) % 16 == 0 &&
+               reinterpret_cast<uintptr_t>(mask) % 16 == 0;
   }
   a.causal = causal;
   a.scale = static_cast<float>(scale);

@@ -44,25 +44,32 @@ __device__ inline uint32_t reachable(const RelAttn& a, const Pairs& p, int len) 
   return bits;
 }
 
-// ... and by the mask.  Its bytes are 0 or 1.  Where four are a word, the words of the
-// next window are read with its tiles (memory answers in order: a read made later would
-// wait for them), and a product gathers a word into four bits.
+// ... and by the mask.  Its bytes are 0 or 1.  Where its rows are 64 aligned bytes a lane
+// reads half of its query's row, 32 bytes in two reads (four bytes at a time, the bits
+// that it needs, cost 65 us of 208 in 24576 windows: each read touches 32 rows), and the
+// halves of the wave exchange every other word.  The words of the next window are read
+// with its tiles: memory answers in order, and a read made later would wait for them.
 struct MaskWords {
-  uint32_t word[8];
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 row[2];
   __device__ inline void load(const RelAttn& a, const Pairs& p, int b, int h) {
     const __amdgpu_buffer_rsrc_t rsrc =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.mask_of(b, h)), 0, 0x7fffffff, 0x00020000);
-    const int hh = afresh(p.hh), at = p.qc * static_cast<int>(a.mq) + 4 * hh;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const int k = 32 * (t >> 2) + 8 * (t & 3);
-      word[t] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, k + 4 * hh < a.Lk ? at + k : OUTSIDE, 0, 0);
-    }
+    const int at = p.qc * static_cast<int>(a.mq) + 32 * p.hh;
+    row[0] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0);
+    row[1] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16, 0, 0);
   }
+  // word w of the row is keys 4 w ..; group t of a lane's bits is word 2 t + h.  A product
+  // gathers a word's bytes into four bits.
   __device__ inline uint32_t bits() const {
     uint32_t r = 0;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) r |= (word[t] * 0x01020408u >> 24 & 15u) << (4 * t);
+    for (int t = 0; t < 4; ++t) {
+      const auto w = __builtin_amdgcn_permlane32_swap(row[t >> 1][2 * (t & 1)], row[t >> 1][2 * (t & 1) + 1],
+                                                      false, false);
+      r |= (w[0] * 0x01020408u >> 24 & 15u) << (4 * t);
+      r |= (w[1] * 0x01020408u >> 24 & 15u) << (16 + 4 * t);
+    }
     return r;
   }
 };
@@ -158,7 +165,7 @@ __device__ inline float scores(f32x16 (&s)[2], const T* kt, const typename Mat<T
 }
 
 template <typename T, int DP, int ACCESS>
-__global__ __launch_bounds__(NT, sizeof(T) == 2 && DP == 32 ? 3 : 2) void window_kernel(RelAttn a, T* out, View os, float* lse, int chunks) {
+__global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View os, float* lse, int chunks) {
   using M = Mat<T>;
   using TL = Tile<T, DP>;
   constexpr int CH = DP / 16, OB = DP / 32;
@@ -181,7 +188,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 && DP == 32 ? 3 : 2) void window
   MaskWords words;
   auto load = [&](int b) {
     const int len = a.keys(b);
-    if (a.mask4) words.load(a, p, b, h);
+    if (a.mask64) words.load(a, p, b, h);
     ql.load(static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h, a.qs.t, a.Lq, a.D, a.vec, tid);
     kl.load(static_cast<const T*>(a.k) + b * a.ks.b + h * a.ks.h, a.ks.t, len, a.D, a.vec, tid);
     vl.load(static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h, a.vs.t, len, a.D, a.vec, tid);
@@ -191,7 +198,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 && DP == 32 ? 3 : 2) void window
   auto store = [&](int b) {
     len = a.keys(b);
     seen = len == a.Lk ? reach : reachable(a, p, len);
-    if (a.mask) seen &= a.mask4 ? words.bits() : allowed(a, p, b, h);
+    if (a.mask) seen &= a.mask64 ? words.bits() : allowed(a, p, b, h);
     ql.store(qt, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
@@ -285,7 +292,7 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
   MaskWords words;
   auto load = [&](int b) {
     const int len = a.keys(b);
-    if (a.mask4) words.load(a, p, b, h);
+    if (a.mask64) words.load(a, p, b, h);
     ql.load(static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h, a.qs.t, a.Lq, a.D, a.vec, tid);
     gl.load(dout + b * gs.b + h * gs.h, gs.t, a.Lq, a.D, a.vec, tid);
     kl.load(static_cast<const T*>(a.k) + b * a.ks.b + h * a.ks.h, a.ks.t, len, a.D, a.vec, tid);
@@ -296,7 +303,7 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
   auto store = [&](int b) {
     len = a.keys(b);
     seen = len == a.Lk ? reach : reachable(a, p, len);
-    if (a.mask) seen &= a.mask4 ? words.bits() : allowed(a, p, b, h);
+    if (a.mask) seen &= a.mask64 ? words.bits() : allowed(a, p, b, h);
     ql.store(qt, tid);
     gl.store(gt, tid);
     kl.store(kt, tid);
@@ -434,7 +441,8 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
     for (int t = tid; t < NW * n; t += NT) sums[t] = 0.0f;
     __syncthreads();
     float* mine = sums + wave * n;
-    const int cq = a.pos.code(p.qc);
+    const Pairs p2{p.q, afresh(p.qc), afresh(hh)};  // (its slots are not kept from the start)
+    const int cq = a.pos.code(p2.qc);
     // within one half of the lanes one key meets 32 queries: 32 slots.  The halves add
     // one after the other, so the order of every slot's sum is fixed.
     for (int turn = 0; turn < 2; ++turn) {
@@ -443,8 +451,8 @@ __global__ __launch_bounds__(NT, 2) void window_backward_kernel(RelAttn a, const
         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (p.key(nb, r) < a.Lk)
-              unsafeAtomicAdd(mine + a.pos.slot(cq - a.pos.code(p.key(nb, r))), total[nb][r]);
+            if (p2.key(nb, r) < a.Lk)
+              unsafeAtomicAdd(mine + a.pos.slot(cq - a.pos.code(p2.key(nb, r))), total[nb][r]);
       }
       __builtin_amdgcn_wave_barrier();
     }
@@ -495,7 +503,7 @@ int forward(RelAttn a, void* out, const View& os, float* lse, int device, hipStr
   const void* views[4] = {a.q, a.k, a.v, out};
   const View vs[4] = {a.qs, a.ks, a.vs, os};
   a.vec = widest_load<T>(views, vs, 4, a.D);
-  const int chunks = chunks_of(a.B, a.H, device, sizeof(T) == 2 && a.D <= 32 ? 6 : 4);
+  const int chunks = chunks_of(a.B, a.H, device, 4);
   T* o = static_cast<T*>(out);
   auto go = [&](auto access) {
     constexpr int ACCESS = decltype(access)::value;

@@ -67,23 +67,56 @@ __device__ inline void load_bias(float* eb, const T* table, int H, int h, int he
   }
 }
 
+// The codes of a window's tokens in LDS, the last one's repeated to a whole tile (a
+// division for each token here, in place of one for each pair).
+inline __host__ __device__ int codes_room(int n) { return (n + 63) / 64 * 64; }
+__device__ inline void load_codes(int* codes, const RelPos& pos, int n, int tid, int nt) {
+  for (int t = tid; t < codes_room(n); t += nt) codes[t] = pos.code(min(t, n - 1));
+}
+
 // How the pairs of a 32 x 32 block stand to the bias table.
 enum : int { NEAR = 0, ALL_BELOW = 1, ALL_ABOVE = 2 };
 __device__ inline int block_kind(const RelPos& pos, int dmin, int dmax) {
   return dmax <= pos.lo ? ALL_BELOW : dmin >= pos.lo + pos.n - 1 ? ALL_ABOVE : NEAR;
 }
 
-// 16 scores of a block whose pairs may be hidden: those are -inf.  k: the key of
-// register 0 of this lane, q: its query (row q of the mask, position qpos).
-__device__ inline void hide(f32x16& s, const RelAttn& a, const uint8_t* mask, int q, int qpos, int k,
-                            int len) {
+// Bit r: whether pair r of a lane's 16 counts, steps 8 (r / 4) + r % 4 from its first
+// along the keys (or the queries): the first `count` steps may, and where there is a mask
+// its byte `step` bytes further on each step.
+__device__ inline uint32_t mask_bits(const uint8_t* p, int64_t step, int count) {
+  uint32_t bits = 0;
+  if (count > 27) {  // the last step is 27
+    uint8_t v[16];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int key = k + 8 * (r / 4) + r % 4;
-    bool on = key < len && (!a.causal || key <= qpos);
-    if (mask && on) on = mask[q * a.mq + key * a.mk] != 0;
-    if (!on) s[r] = -INF;
+    for (int r = 0; r < 16; ++r) v[r] = p[(8 * (r / 4) + r % 4) * step];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bits |= (v[r] != 0 ? 1u : 0u) << r;
+  } else {
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r) {
+      const int s = 8 * (r / 4) + r % 4;
+      if (s < count && p[s * step]) bits |= 1u << r;
+    }
   }
+  return bits;
+}
+// Steps below `to`.
+__device__ inline uint32_t first_bits(int to) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) bits |= (15u >> (4 - min(max(to - 8 * g, 0), 4))) << (4 * g);
+  return bits;
+}
+// The pairs of query q (position qpos) with the keys from k on.
+__device__ inline uint32_t seen_keys(const RelAttn& a, const uint8_t* mask, int q, int qpos, int k, int len) {
+  uint32_t bits = first_bits(min(len, a.causal ? max(qpos, -1) + 1 : len) - k);
+  if (mask) bits &= mask_bits(mask + afresh(q) * a.mq + k * a.mk, a.mk, len - k);
+  return bits;
+}
+// 16 scores of which some may be hidden: those are -inf.
+__device__ inline void hide(f32x16& s, uint32_t seen) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = seen >> r & 1 ? s[r] : -INF;
 }
 
 // acc += V^T P^T over 16 keys of which some are hidden from some queries: a value

@@ -38,7 +38,9 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   const uint8_t* mask = a.mask_of(b, h);
   const float c = a.scale * LOG2E;
 
+  int* codes = reinterpret_cast<int*>(eb + (a.pos.n + 2 * PAD + 3) / 4 * 4);  // of a window's keys
   load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
+  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, tid, NT);
 
   typename M::V8 qf[CH];
   const int q_first = tile * (NW * 32);
@@ -106,13 +108,17 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
         }
       } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = min(k0 + 4 * hh + 8 * (r / 4) + r % 4, a.Lk - 1);
-          s[nb][r] = s[nb][r] * c + eb[cq - a.pos.code(key) - a.pos.lo + PAD];
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int4 ck = *reinterpret_cast<const int4*>(codes + k0 + 4 * hh + 8 * r4);
+          const float* e = eb + cq - a.pos.lo + PAD;
+          s[nb][4 * r4] = s[nb][4 * r4] * c + e[-ck.x];
+          s[nb][4 * r4 + 1] = s[nb][4 * r4 + 1] * c + e[-ck.y];
+          s[nb][4 * r4 + 2] = s[nb][4 * r4 + 2] * c + e[-ck.z];
+          s[nb][4 * r4 + 3] = s[nb][4 * r4 + 3] * c + e[-ck.w];
         }
       }
       partial[nb] = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
-      if (partial[nb]) hide(s[nb], a, mask, qc, qpos, k0 + 4 * hh, len);
+      if (partial[nb]) hide(s[nb], seen_keys(a, mask, qc, qpos, k0 + 4 * hh, len));
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
     }
@@ -177,7 +183,8 @@ int launch_one(const RelAttn& a, T* out, const View& os, int ovec, float* lse, h
   const int q_tiles = (a.Lq + NW * 32 - 1) / (NW * 32);
   const int64_t wgs = static_cast<int64_t>(a.B) * a.H * q_tiles;
   if (wgs > 0x7fffffff) return FA_E_SHAPE;
-  const size_t lds = 4 * Shape<T, DP>::TILE + (a.pos.n + 2 * PAD) * sizeof(float);
+  const size_t lds = 4 * Shape<T, DP>::TILE + (a.pos.n + 2 * PAD + 3) / 4 * 16 +
+                     (a.pos.grid_w ? codes_room(a.Lk) * sizeof(int) : 0);
   auto kernel = rel_attention_kernel<T, DP, NW, WIDE>;
   if (const int e = launch_lds(kernel, lds)) return e;
   kernel<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, out, os, ovec, lse, q_tiles);

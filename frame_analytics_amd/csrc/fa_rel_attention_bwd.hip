@@ -44,8 +44,13 @@ template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<
 // ---------------------------------------------------------------------------
 // dQ and the table
 // ---------------------------------------------------------------------------
-template <typename T, int DP, bool TABLE, bool WIDE>
-__global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g, int q_tiles) {
+// Windows of up to 256 tokens (KEYS blocks of 32 keys, KEYS > 0): a workgroup takes one
+// tile of queries of every `chunks`-th batch entry, and its dS by pair is summed over
+// them in registers, to reach the table's differences once at the end.  (By LDS atomics
+// for each window: 1617 us of 2270 for 512 windows of 16 x 16, 8 heads.)  On a line most
+// blocks are far from the wave's queries and are one sum.
+template <typename T, int DP, bool TABLE, bool WIDE, int KEYS>
+__global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g, int q_tiles, int chunks) {
   using M = Mat<T>;
   using TL = Tile<T, DP>;
   constexpr int BN = Shape<T, DP>::BN, NB = BN / 32, CH = DP / 16, OB = DP / 32;
@@ -56,22 +61,31 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
   float* eb = reinterpret_cast<float*>(vt + BUFS * BN * TL::LD);
   const int np = a.pos.n + 2 * PAD;
   float* sums = eb + np;  // [NW][np]: the table's sums by slot, one copy for each wave
+  int* codes = reinterpret_cast<int*>(eb + ((TABLE ? 1 + NW : 1) * np + 3) / 4 * 4);  // of a window's keys
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = q_tiles - 1 - int(wg % q_tiles);
-  const int h = int(wg / q_tiles) % a.H, b = int(wg / q_tiles) / a.H, hk = h / (a.H / a.Hk);
+  const int h = int(wg / q_tiles) % a.H, chunk = int(wg / q_tiles) / a.H, hk = h / (a.H / a.Hk);
   const int qw = tile * (NW * 32) + wave * 32;
-  const int q = qw + col, qc = min(q, a.Lq - 1), s0 = a.start(b), len = a.keys(b);
-  const int qpos = s0 + q, cq = s0 + a.pos.code(qc);
-  const uint8_t* mask = a.mask_of(b, h);
+  const int q = qw + col, qc = min(q, a.Lq - 1);
   const float c = a.scale * LOG2E;
 
   load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
-  if (TABLE)
+  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, tid, NT);
+  constexpr int TOTALS = KEYS > 0 ? KEYS : 1;
+  f32x16 total[TOTALS];
+#pragma unroll
+  for (int i = 0; i < TOTALS; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) total[i][r] = 0.0f;
+  if (TABLE && KEYS == 0)
     for (int t = tid; t < NW * np; t += NT) sums[t] = 0.0f;
   float* mine = sums + wave * np;
   float far_lo = 0.0f, far_hi = 0.0f;
 
+  for (int b = chunk; b < a.B; b += chunks) {
+  const int s0 = a.start(b), len = a.keys(b), qpos = s0 + q, cq = s0 + a.pos.code(qc);
+  const uint8_t* mask = a.mask_of(b, h);
   typename M::V8 qf[CH], gf[CH];
   const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.Lq + qc;
   // a row that sees no key: its weights are 2^(s - inf) = 0 whatever dout holds
@@ -116,13 +130,14 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
   TileLoad<T, DP, BN, NT, WIDE> kl, vl;
   const int tiles = (end + BN - 1) / BN;
+  if (KEYS > 0) __syncthreads();  // the window before is done with the tiles
   if (tiles > 0) {
     kl.load(kb, a.ks.t, len, a.D, a.vec, tid);
     vl.load(vb, a.vs.t, len, a.D, a.vec, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
   }
-  for (int t = 0; t < tiles; ++t) {
+  auto work = [&](int t, f32x16* pairs) {
     __syncthreads();
     const T* kk = kt + (t % BUFS) * BN * TL::LD;
     const T* vv = vt + (t % BUFS) * BN * TL::LD;
@@ -136,7 +151,7 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
     for (int nb = 0; nb < NB; ++nb) {
       const int k0 = t * BN + nb * 32;
       const bool hidden = a.causal && k0 > s0 + qw + 31;  // nothing for this wave
-      if (hidden || k0 >= len) continue;
+      if (hidden || k0 >= len || qw >= a.Lq) continue;
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
@@ -148,19 +163,24 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
       const bool partial = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
       int kind = NEAR;
       int slot[16];  // of each pair, where it has one of its own
-      if (a.pos.grid_w == 0) {
+      if (KEYS == 0 && a.pos.grid_w == 0) {
         kind = block_kind(a.pos, s0 + qw - (k0 + 31), s0 + qw + 31 - k0);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           slot[r] = s0 + q - k0 - 4 * hh - a.pos.lo + PAD - (8 * (r / 4) + r % 4);
       } else {
+        // (codes are those of the window's keys, the last one's past its end)
+        const int at = afresh(cq - a.pos.lo + PAD);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = min(k0 + 4 * hh + 8 * (r / 4) + r % 4, a.Lk - 1);
-          slot[r] = cq - a.pos.code(key) - a.pos.lo + PAD;
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int4 ck = *reinterpret_cast<const int4*>(codes + k0 + 4 * hh + 8 * r4);
+          slot[4 * r4] = at - ck.x;
+          slot[4 * r4 + 1] = at - ck.y;
+          slot[4 * r4 + 2] = at - ck.z;
+          slot[4 * r4 + 3] = at - ck.w;
         }
       }
-      if (kind == NEAR) {
+      if (KEYS > 0 || kind == NEAR) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = s[r] * c + eb[slot[r]];
       } else {
@@ -174,15 +194,14 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
         s[r] = p * (dp[r] - dsum);
       }
       if (partial) {
+        const uint32_t seen = seen_keys(a, mask, qc, qpos, k0 + 4 * hh, len);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 4 * hh + 8 * (r / 4) + r % 4;
-          bool seen = key < len && (!a.causal || key <= qpos);
-          if (mask && seen) seen = mask[qc * a.mq + key * a.mk] != 0;
-          if (!seen) s[r] = 0.0f;
-        }
+        for (int r = 0; r < 16; ++r) s[r] = seen >> r & 1 ? s[r] : 0.0f;
       }
-      if (TABLE) {
+      if (TABLE && KEYS > 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) pairs[nb][r] += s[r];
+      } else if (TABLE) {
         if (kind == NEAR) {
           // within one half of the lanes one key meets 32 queries: 32 slots.  The
           // halves add one after the other, so the order of every slot's sum is fixed.
@@ -225,6 +244,13 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
       kl.store(kt + ((t + 1) % BUFS) * BN * TL::LD, tid);
       vl.store(vt + ((t + 1) % BUFS) * BN * TL::LD, tid);
     }
+  };
+  if constexpr (KEYS > 0) {
+#pragma unroll
+    for (int t = 0; t < KEYS / NB; ++t)
+      if (t < tiles) work(t, total + t * NB);
+  } else {
+    for (int t = 0; t < tiles; ++t) work(t, total);
   }
   if (q < a.Lq) {
     T* drow = static_cast<T*>(g.dq) + b * g.dqs.b + h * g.dqs.h + q * g.dqs.t;
@@ -238,6 +264,25 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
         store4<T>(drow, 32 * i + 8 * e4 + 4 * hh, a.D, g.dqvec, w);
       }
   }
+  }
+  if (TABLE && KEYS > 0) {
+    __syncthreads();
+    for (int t = tid; t < NW * np; t += NT) sums[t] = 0.0f;
+    __syncthreads();
+    const int at = a.pos.code(qc) - a.pos.lo + PAD;
+    for (int turn = 0; turn < 2; ++turn) {  // the halves one after the other, as above
+      if (hh == turn && q < a.Lq) {
+#pragma unroll
+        for (int i = 0; i < TOTALS; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = 32 * i + 4 * hh + 8 * (r / 4) + r % 4;
+            if (key < a.Lk) unsafeAtomicAdd(mine + at - codes[key], total[i][r]);
+          }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
   if (TABLE) {
     // what the padding holds belongs to the ends
     far_lo += mine[lane];  // slots 0 .. PAD - 1
@@ -249,7 +294,7 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
       mine[PAD + a.pos.n - 1] += far_hi;
     }
     __syncthreads();
-    float* dst = g.parts + (static_cast<int64_t>(h) * a.B * q_tiles + b * q_tiles + tile) * a.pos.n;
+    float* dst = g.parts + (static_cast<int64_t>(h) * chunks * q_tiles + chunk * q_tiles + tile) * a.pos.n;
     for (int t = tid; t < a.pos.n; t += NT) {
       float v = 0.0f;
 #pragma unroll
@@ -275,6 +320,7 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
   const int np = a.pos.n + 2 * PAD;
   float* ls = eb + (np + 3) / 4 * 4;  // [2][BM]: each query's log-sum
   float* dd = ls + 2 * BM;            // [2][BM]: and D_i
+  int* codes = reinterpret_cast<int*>(dd + 2 * BM);  // of a window's queries
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = int(wg % k_tiles), hk = int(wg / k_tiles) % a.Hk, b = int(wg / k_tiles) / a.Hk;
@@ -284,6 +330,7 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
   const int ck = a.pos.code(kc);
   const float c = a.scale * LOG2E;
   const int k_first = tile * (NW * 32);
+  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lq, tid, NT);
 
   typename M::V8 kf[CH], vf[CH];
   load_row<T, WIDE>(kf, Rows<T>(static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + k_first * a.ks.t, a.ks.t),
@@ -384,9 +431,13 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
           }
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int i = min(i0 + 4 * hh + 8 * (r / 4) + r % 4, a.Lq - 1);
-            s[r] = s[r] * c + eb[a.pos.code(i) - ck - a.pos.lo + PAD];
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const int4 cq = *reinterpret_cast<const int4*>(codes + i0 + 4 * hh + 8 * r4);
+            const float* e = eb + PAD - ck - a.pos.lo;
+            s[4 * r4] = s[4 * r4] * c + e[cq.x];
+            s[4 * r4 + 1] = s[4 * r4 + 1] * c + e[cq.y];
+            s[4 * r4 + 2] = s[4 * r4 + 2] * c + e[cq.z];
+            s[4 * r4 + 3] = s[4 * r4 + 3] * c + e[cq.w];
           }
         }
 #pragma unroll
@@ -403,13 +454,13 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
           }
         }
         if (partial) {
+          // queries from the key's position on, those before Lq
+          const int i = i0 + 4 * hh, from = a.causal ? key - s0 - i : 0;
+          uint32_t seen = key < len ? ~first_bits(from) & first_bits(a.Lq - i) : 0;
+          if (mask && key < len) seen &= mask_bits(mask + i * a.mq + afresh(key) * a.mk, a.mq, a.Lq - i);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int i = i0 + 4 * hh + 8 * (r / 4) + r % 4;
-            bool seen = key < len && (!a.causal || key <= s0 + i);
-            if (mask && seen && i < a.Lq) seen = mask[i * a.mq + key * a.mk] != 0;
-            if (!seen) s[r] = dp[r] = 0.0f;
-          }
+          for (int r = 0; r < 16; ++r)
+            if (!(seen >> r & 1)) s[r] = dp[r] = 0.0f;
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -455,19 +506,32 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
 
 inline int tiles_of(int n) { return (n + NW * 32 - 1) / (NW * 32); }
 
+// Batch entries that a workgroup of dQ leaves to others: all, except where windows'
+// sums stay in its registers (two workgroups for every compute unit then).
+inline bool sums_in_registers(int Lq, int D, int grid_w) { return grid_w > 0 && Lq <= 256 && D <= 64; }
+inline int chunks_of(int B, int H, int Lq, int D, int grid_w, int device) {
+  if (!sums_in_registers(Lq, D, grid_w)) return B;
+  const int each = H * tiles_of(Lq), want = (2 * cu_count(device) + each - 1) / each;
+  return want < B ? want : B;
+}
+
 template <typename T, int DP, bool WIDE>
-int launch_wide(const RelAttn& a, const Grads& g, hipStream_t s) {
+int launch_wide(const RelAttn& a, const Grads& g, int chunks, hipStream_t s) {
   const int qt = tiles_of(a.Lq), kt = tiles_of(a.Lk);
-  const int64_t wq = static_cast<int64_t>(a.B) * a.H * qt, wk = static_cast<int64_t>(a.B) * a.Hk * kt;
+  const int64_t wq = static_cast<int64_t>(chunks) * a.H * qt, wk = static_cast<int64_t>(a.B) * a.Hk * kt;
   if (wq > 0x7fffffff || wk > 0x7fffffff) return FA_E_SHAPE;
   const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
-  const size_t lds_q = tiles + (g.parts ? 1 + NW : 1) * np * sizeof(float);
-  const size_t lds_k = tiles + ((np + 3) / 4 * 4 + 4 * Shape<T, DP>::BN) * sizeof(float);
-  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, true, WIDE> : rel_attention_dq_kernel<T, DP, false, WIDE>;
+  const size_t code = a.pos.grid_w ? codes_room(a.Lk) * sizeof(int) : 0;
+  const size_t lds_q = tiles + ((g.parts ? 1 + NW : 1) * np + 3) / 4 * 16 + code;
+  const size_t lds_k = tiles + ((np + 3) / 4 * 4 + 4 * Shape<T, DP>::BN) * sizeof(float) + code;
+  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, true, WIDE, 0> : rel_attention_dq_kernel<T, DP, false, WIDE, 0>;
+  if constexpr (DP <= 64)
+    if (g.parts && sums_in_registers(a.Lq, a.D, a.pos.grid_w))
+      dq = a.Lq <= 128 ? rel_attention_dq_kernel<T, DP, true, WIDE, 4> : rel_attention_dq_kernel<T, DP, true, WIDE, 8>;
   auto dkv = rel_attention_dkv_kernel<T, DP, WIDE>;
   if (const int e = launch_lds(dq, lds_q)) return e;
   if (const int e = launch_lds(dkv, lds_k)) return e;
-  dq<<<static_cast<unsigned>(wq), NT, lds_q, s>>>(a, g, qt);
+  dq<<<static_cast<unsigned>(wq), NT, lds_q, s>>>(a, g, qt, chunks);
   FA_LAUNCH_CHECK();
   dkv<<<static_cast<unsigned>(wk), NT, lds_k, s>>>(a, g, kt);
   FA_LAUNCH_CHECK();
@@ -475,12 +539,14 @@ int launch_wide(const RelAttn& a, const Grads& g, hipStream_t s) {
 }
 
 template <typename T, int DP>
-int launch_dim(const RelAttn& a, const Grads& g, hipStream_t s) {
-  return a.vec * sizeof(T) == 16 ? launch_wide<T, DP, true>(a, g, s) : launch_wide<T, DP, false>(a, g, s);
+int launch_dim(const RelAttn& a, const Grads& g, int chunks, hipStream_t s) {
+  return a.vec * sizeof(T) == 16 ? launch_wide<T, DP, true>(a, g, chunks, s)
+                                 : launch_wide<T, DP, false>(a, g, chunks, s);
 }
 
 template <typename T>
-int backward(RelAttn a, Grads g, int rows, void* dtable, hipStream_t s) {
+int backward(RelAttn a, Grads g, int rows, void* dtable, int device, hipStream_t s) {
+  const int chunks = g.parts ? chunks_of(a.B, a.H, a.Lq, a.D, a.pos.grid_w, device) : a.B;
   const void* in[5] = {a.q, a.k, a.v, g.out, g.dout};
   const View iv[5] = {a.qs, a.ks, a.vs, g.os, g.gs};
   a.vec = widest_load<T>(in, iv, 5, a.D);
@@ -490,12 +556,12 @@ int backward(RelAttn a, Grads g, int rows, void* dtable, hipStream_t s) {
   const View dkv[2] = {g.dks, g.dvs};
   g.dkvec = widest_load<T>(dkp, dkv, 2, a.D);
   int e;
-  if (a.D <= 32) e = launch_dim<T, 32>(a, g, s);
-  else if (a.D <= 64) e = launch_dim<T, 64>(a, g, s);
-  else e = launch_dim<T, 128>(a, g, s);
+  if (a.D <= 32) e = launch_dim<T, 32>(a, g, chunks, s);
+  else if (a.D <= 64) e = launch_dim<T, 64>(a, g, chunks, s);
+  else e = launch_dim<T, 128>(a, g, chunks, s);
   if (e) return e;
   if (dtable) {
-    launch_table_sum<T>(g.parts, a.B * tiles_of(a.Lq), a.pos.n, a.pos.row_of, rows, a.H,
+    launch_table_sum<T>(g.parts, chunks * tiles_of(a.Lq), a.pos.n, a.pos.row_of, rows, a.H,
                         static_cast<T*>(dtable), s);
     FA_LAUNCH_CHECK();
   }
@@ -565,9 +631,9 @@ FA_API int fa_gpu_rel_attention_backward(
     return window_backward(dtype, a, w, rows, dtable, device, s);
   }
   switch (dtype) {
-    case FA_F16: return backward<_Float16>(a, g, rows, dtable, s);
-    case FA_BF16: return backward<__bf16>(a, g, rows, dtable, s);
-    case FA_F32: return backward<float>(a, g, rows, dtable, s);
+    case FA_F16: return backward<_Float16>(a, g, rows, dtable, device, s);
+    case FA_BF16: return backward<__bf16>(a, g, rows, dtable, device, s);
+    case FA_F32: return backward<float>(a, g, rows, dtable, device, s);
     default: return FA_E_DTYPE;
   }
 }

@@ -101,7 +101,8 @@ TRAIN_SIGNATURES = {
     "fa_gpu_rel_attention":
         ([_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _L, _P, _P, _P, _I,
           _P, _I, _D, _P, _P, _P, _L, _I, _P], _I),
-    "fa_gpu_rel_attention_backward_workspace": ([_I, _I, _I, _I, _I, _P], _I),
+    "fa_gpu_rel_attention_backward_workspace":
+        ([_I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P], _I),
     "fa_gpu_rel_attention_backward":
         ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _I, _I, _L, _P,
           _P, _P, _I, _P, _I, _D, _P, _P, _P, _P, _P, _L, _I, _P], _I),

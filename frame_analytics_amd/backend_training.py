@@ -152,8 +152,8 @@ def rel_attention_backward(g, q, k, v, out, lse, table, plan: AttentionPlan, nee
     dq, dk, dv = _like(q), _like(k), _like(v)
     dtable = torch.empty_like(table) if need_table else None
     dev, stream = _site(q)
-    ws, n = _workspace("fa_gpu_rel_attention_backward_workspace", q.device, b, h, lq,
-                       plan.positions.slots, int(need_table))
+    ws, n = _workspace("fa_gpu_rel_attention_backward_workspace", q.device, b, h, hk, lq, lk, d,
+                       plan.positions.slots, plan.positions.grid_w, int(need_table), dev)
     _run("fa_gpu_rel_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
          g.data_ptr(), lse.data_ptr(), _DTYPE_CODE[q.dtype], b, h, hk, lq, lk, d,
          _strides(q, k, v, out, g, dq, dk, dv),

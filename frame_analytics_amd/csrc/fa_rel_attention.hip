@@ -193,25 +193,28 @@ int launch_one(const RelAttn& a, T* out, const View& os, int ovec, float* lse, h
 }
 
 template <typename T, int DP>
-int launch_dim(const RelAttn& a, T* out, const View& os, int ovec, float* lse, hipStream_t s) {
+int launch_dim(const RelAttn& a, T* out, const View& os, int ovec, float* lse, int device, hipStream_t s) {
+  // two waves to a workgroup where four leave compute units without one (256 workgroups of
+  // four took 86 us where 512 of two took 101, a causal line of 2048)
+  const bool few = a.Lq <= 64 || static_cast<int64_t>(a.B) * a.H * ((a.Lq + 127) / 128) < cu_count(device);
   if (a.vec * sizeof(T) == 16)
-    return a.Lq <= 64 ? launch_one<T, DP, 2, true>(a, out, os, ovec, lse, s)
-                      : launch_one<T, DP, 4, true>(a, out, os, ovec, lse, s);
-  return a.Lq <= 64 ? launch_one<T, DP, 2, false>(a, out, os, ovec, lse, s)
-                    : launch_one<T, DP, 4, false>(a, out, os, ovec, lse, s);
+    return few ? launch_one<T, DP, 2, true>(a, out, os, ovec, lse, s)
+               : launch_one<T, DP, 4, true>(a, out, os, ovec, lse, s);
+  return few ? launch_one<T, DP, 2, false>(a, out, os, ovec, lse, s)
+             : launch_one<T, DP, 4, false>(a, out, os, ovec, lse, s);
 }
 
 template <typename T>
-int forward(RelAttn a, void* out, const View& os, float* lse, hipStream_t s) {
+int forward(RelAttn a, void* out, const View& os, float* lse, int device, hipStream_t s) {
   const void* in[3] = {a.q, a.k, a.v};
   const View iv[3] = {a.qs, a.ks, a.vs};
   a.vec = widest_load<T>(in, iv, 3, a.D);
   const void* op[1] = {out};
   const int ovec = widest_load<T>(op, &os, 1, a.D);
   T* o = static_cast<T*>(out);
-  if (a.D <= 32) return launch_dim<T, 32>(a, o, os, ovec, lse, s);
-  if (a.D <= 64) return launch_dim<T, 64>(a, o, os, ovec, lse, s);
-  return launch_dim<T, 128>(a, o, os, ovec, lse, s);
+  if (a.D <= 32) return launch_dim<T, 32>(a, o, os, ovec, lse, device, s);
+  if (a.D <= 64) return launch_dim<T, 64>(a, o, os, ovec, lse, device, s);
+  return launch_dim<T, 128>(a, o, os, ovec, lse, device, s);
 }
 
 }  // namespace
@@ -251,9 +254,9 @@ FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int
   if (window_serve(a)) return window_forward(dtype, a, out, os, lse, device, s);
   if (rows_serve(a)) return rows_forward(dtype, a, out, os, lse, workspace, workspace_bytes, device, s);
   switch (dtype) {
-    case FA_F16: return forward<_Float16>(a, out, os, lse, s);
-    case FA_BF16: return forward<__bf16>(a, out, os, lse, s);
-    case FA_F32: return forward<float>(a, out, os, lse, s);
+    case FA_F16: return forward<_Float16>(a, out, os, lse, device, s);
+    case FA_BF16: return forward<__bf16>(a, out, os, lse, device, s);
+    case FA_F32: return forward<float>(a, out, os, lse, device, s);
     default: return FA_E_DTYPE;
   }
 }

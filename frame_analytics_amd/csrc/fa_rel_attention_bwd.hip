@@ -23,9 +23,8 @@ struct Grads {
   View dqs, dks, dvs;
   int dqvec, dkvec;
   float* parts;  // [H][B * q_tiles][n], or null: the table needs no gradient
+  float* joint;  // [splits][dk, dv][B, Hk, Lk, D] where heads that share a key are split
 };
-
-constexpr int NW = 4, NT = NW * 64;
 
 template <typename T, int DP> struct Shape {
   static constexpr int BN = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
@@ -49,8 +48,10 @@ template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<
 // them in registers, to reach the table's differences once at the end.  (By LDS atomics
 // for each window: 1617 us of 2270 for 512 windows of 16 x 16, 8 heads.)  On a line most
 // blocks are far from the wave's queries and are one sum.
-template <typename T, int DP, bool TABLE, bool WIDE, int KEYS>
-__global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g, int q_tiles, int chunks) {
+template <typename T, int DP, int NW, bool TABLE, bool WIDE, int KEYS>
+__global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Grads g, int q_tiles,
+                                                                    int chunks) {
+  constexpr int NT = NW * 64;
   using M = Mat<T>;
   using TL = Tile<T, DP>;
   constexpr int BN = Shape<T, DP>::BN, NB = BN / 32, CH = DP / 16, OB = DP / 32;
@@ -307,8 +308,12 @@ __global__ __launch_bounds__(NT) void rel_attention_dq_kernel(RelAttn a, Grads g
 // ---------------------------------------------------------------------------
 // dK and dV
 // ---------------------------------------------------------------------------
-template <typename T, int DP, bool WIDE>
-__global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads g, int k_tiles) {
+// The query heads that share a key head may be split between workgroups, whose float32
+// sums dkv_join_kernel adds in order.
+template <typename T, int DP, int NW, bool WIDE>
+__global__ __launch_bounds__(NW * 64) void rel_attention_dkv_kernel(RelAttn a, Grads g, int k_tiles,
+                                                                    int splits) {
+  constexpr int NT = NW * 64;
   using M = Mat<T>;
   using TL = Tile<T, DP>;
   constexpr int BM = Shape<T, DP>::BN, NB = BM / 32, CH = DP / 16, OB = DP / 32;
@@ -323,8 +328,9 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
   int* codes = reinterpret_cast<int*>(dd + 2 * BM);  // of a window's queries
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
-  const int tile = int(wg % k_tiles), hk = int(wg / k_tiles) % a.Hk, b = int(wg / k_tiles) / a.Hk;
-  const int group = a.H / a.Hk;
+  const int tile = int(wg % k_tiles), split = int(wg / k_tiles) % splits;
+  const int hk = int(wg / k_tiles / splits) % a.Hk, b = int(wg / k_tiles / splits) / a.Hk;
+  const int group = a.H / a.Hk, hg0 = split * group / splits, hg1 = (split + 1) * group / splits;
   const int kw = tile * (NW * 32) + wave * 32;  // the wave's first key
   const int key = kw + col, kc = min(key, a.Lk - 1), s0 = a.start(b), len = a.keys(b);
   const int ck = a.pos.code(kc);
@@ -355,7 +361,7 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
   float lse_r = 0.0f, d_r = 0.0f;
   float row_lse[TileLoad<T, DP, BM, NT, WIDE>::N];  // of the rows that this thread brings
 
-  for (int hg = 0; hg < group; ++hg) {
+  for (int hg = hg0; hg < hg1; ++hg) {
     const int h = hk * group + hg;
     const uint8_t* mask = a.mask_of(b, h);
     const T* qb = static_cast<const T*>(a.q) + b * a.qs.b + h * a.qs.h;
@@ -485,7 +491,21 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
       }
     }
   }
-  if (key < a.Lk) {
+  if (key < a.Lk && splits > 1) {
+    const int64_t each = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.D;
+    float* krow = g.joint + 2 * split * each + ((static_cast<int64_t>(b) * a.Hk + hk) * a.Lk + key) * a.D;
+    float* vrow = krow + each;
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = 32 * i + 8 * (r / 4) + 4 * hh + r % 4;
+        if (d < a.D) {
+          krow[d] = dk[i][r] * a.scale;
+          vrow[d] = dv[i][r];
+        }
+      }
+  } else if (key < a.Lk) {
     T* krow_o = static_cast<T*>(g.dk) + b * g.dks.b + hk * g.dks.h + key * g.dks.t;
     T* vrow_o = static_cast<T*>(g.dv) + b * g.dvs.b + hk * g.dvs.h + key * g.dvs.t;
 #pragma unroll
@@ -504,49 +524,105 @@ __global__ __launch_bounds__(NT) void rel_attention_dkv_kernel(RelAttn a, Grads 
   }
 }
 
-inline int tiles_of(int n) { return (n + NW * 32 - 1) / (NW * 32); }
+template <typename T>
+__global__ __launch_bounds__(256) void dkv_join_kernel(RelAttn a, Grads g, int splits) {
+  const int64_t each = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.D;
+  for (int64_t t = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x; t < 2 * each;
+       t += static_cast<int64_t>(gridDim.x) * 256) {
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v += g.joint[2 * s * each + t];
+    const bool second = t >= each;
+    const int64_t e = second ? t - each : t, row = e / a.D;
+    const int d = static_cast<int>(e - row * a.D), key = static_cast<int>(row % a.Lk);
+    const int hk = static_cast<int>(row / a.Lk) % a.Hk, b = static_cast<int>(row / a.Lk / a.Hk);
+    const View& st = second ? g.dvs : g.dks;
+    static_cast<T*>(second ? g.dv : g.dk)[b * st.b + hk * st.h + key * st.t + d] = T(v);
+  }
+}
 
-// Batch entries that a workgroup of dQ leaves to others: all, except where windows'
-// sums stay in its registers (two workgroups for every compute unit then).
-inline bool sums_in_registers(int Lq, int D, int grid_w) { return grid_w > 0 && Lq <= 256 && D <= 64; }
-inline int chunks_of(int B, int H, int Lq, int D, int grid_w, int device) {
-  if (!sums_in_registers(Lq, D, grid_w)) return B;
-  const int each = H * tiles_of(Lq), want = (2 * cu_count(device) + each - 1) / each;
-  return want < B ? want : B;
+inline int tiles_of(int n, int nw) { return (n + nw * 32 - 1) / (nw * 32); }
+
+// How a call is laid out over the card.  Four waves to a workgroup, two where four leave
+// compute units without one (a causal line of 2048, 256 workgroups of four: dQ 91 us
+// against 105 of two, dK and dV 80 against 106; 112 and 28 of four, odd 777: 142 and 608
+// against 119 and, the shared heads split, 137).
+struct Plan {
+  int nw_q, nw_k;  // waves of the workgroups that own queries, and keys
+  int chunks;      // batch entries in parallel for dQ: all, unless windows' sums stay in registers
+  bool registers;
+  int splits;      // of the query heads of a key head
+};
+inline Plan plan_of(int B, int H, int Hk, int Lq, int Lk, int D, int grid_w, bool table, int device) {
+  Plan p;
+  const int64_t enough = 2 * cu_count(device);
+  p.registers = table && grid_w > 0 && Lq <= 256 && D <= 64;
+  p.nw_q = p.registers || static_cast<int64_t>(B) * H * tiles_of(Lq, 4) >= cu_count(device) ? 4 : 2;
+  p.nw_k = static_cast<int64_t>(B) * Hk * tiles_of(Lk, 4) >= cu_count(device) ? 4 : 2;
+  p.chunks = B;
+  if (p.registers) {  // two workgroups for every compute unit
+    const int64_t each = static_cast<int64_t>(H) * tiles_of(Lq, 4), want = (enough + each - 1) / each;
+    p.chunks = static_cast<int>(want < B ? want : B);
+  }
+  const int64_t wgs = static_cast<int64_t>(B) * Hk * tiles_of(Lk, p.nw_k), most = H / Hk;
+  const int64_t want = (enough + wgs - 1) / wgs;
+  p.splits = static_cast<int>(want < most ? want : most);
+  return p;
+}
+
+template <typename T, int DP, int NW, bool WIDE>
+int launch_dq(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
+  const int qt = tiles_of(a.Lq, NW);
+  const int64_t wgs = static_cast<int64_t>(p.chunks) * a.H * qt;
+  if (wgs > 0x7fffffff) return FA_E_SHAPE;
+  const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
+  const size_t lds = tiles + ((g.parts ? 1 + NW : 1) * np + 3) / 4 * 16 +
+                     (a.pos.grid_w ? codes_room(a.Lk) * sizeof(int) : 0);
+  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, NW, true, WIDE, 0>
+                    : rel_attention_dq_kernel<T, DP, NW, false, WIDE, 0>;
+  if constexpr (DP <= 64 && NW == 4)
+    if (p.registers)
+      dq = a.Lq <= 128 ? rel_attention_dq_kernel<T, DP, NW, true, WIDE, 4>
+                       : rel_attention_dq_kernel<T, DP, NW, true, WIDE, 8>;
+  if (const int e = launch_lds(dq, lds)) return e;
+  dq<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, g, qt, p.chunks);
+  FA_LAUNCH_CHECK();
+  return FA_OK;
+}
+
+template <typename T, int DP, int NW, bool WIDE>
+int launch_dkv(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
+  const int kt = tiles_of(a.Lk, NW);
+  const int64_t wgs = static_cast<int64_t>(a.B) * a.Hk * kt * p.splits;
+  if (wgs > 0x7fffffff) return FA_E_SHAPE;
+  const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
+  const size_t lds = tiles + ((np + 3) / 4 * 4 + 4 * Shape<T, DP>::BN) * sizeof(float) +
+                     (a.pos.grid_w ? codes_room(a.Lq) * sizeof(int) : 0);
+  auto dkv = rel_attention_dkv_kernel<T, DP, NW, WIDE>;
+  if (const int e = launch_lds(dkv, lds)) return e;
+  dkv<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, g, kt, p.splits);
+  FA_LAUNCH_CHECK();
+  return FA_OK;
 }
 
 template <typename T, int DP, bool WIDE>
-int launch_wide(const RelAttn& a, const Grads& g, int chunks, hipStream_t s) {
-  const int qt = tiles_of(a.Lq), kt = tiles_of(a.Lk);
-  const int64_t wq = static_cast<int64_t>(chunks) * a.H * qt, wk = static_cast<int64_t>(a.B) * a.Hk * kt;
-  if (wq > 0x7fffffff || wk > 0x7fffffff) return FA_E_SHAPE;
-  const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
-  const size_t code = a.pos.grid_w ? codes_room(a.Lk) * sizeof(int) : 0;
-  const size_t lds_q = tiles + ((g.parts ? 1 + NW : 1) * np + 3) / 4 * 16 + code;
-  const size_t lds_k = tiles + ((np + 3) / 4 * 4 + 4 * Shape<T, DP>::BN) * sizeof(float) + code;
-  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, true, WIDE, 0> : rel_attention_dq_kernel<T, DP, false, WIDE, 0>;
-  if constexpr (DP <= 64)
-    if (g.parts && sums_in_registers(a.Lq, a.D, a.pos.grid_w))
-      dq = a.Lq <= 128 ? rel_attention_dq_kernel<T, DP, true, WIDE, 4> : rel_attention_dq_kernel<T, DP, true, WIDE, 8>;
-  auto dkv = rel_attention_dkv_kernel<T, DP, WIDE>;
-  if (const int e = launch_lds(dq, lds_q)) return e;
-  if (const int e = launch_lds(dkv, lds_k)) return e;
-  dq<<<static_cast<unsigned>(wq), NT, lds_q, s>>>(a, g, qt, chunks);
-  FA_LAUNCH_CHECK();
-  dkv<<<static_cast<unsigned>(wk), NT, lds_k, s>>>(a, g, kt);
+int launch_wide(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
+  int e = p.nw_q == 4 ? launch_dq<T, DP, 4, WIDE>(a, g, p, s) : launch_dq<T, DP, 2, WIDE>(a, g, p, s);
+  if (e) return e;
+  e = p.nw_k == 4 ? launch_dkv<T, DP, 4, WIDE>(a, g, p, s) : launch_dkv<T, DP, 2, WIDE>(a, g, p, s);
+  if (e || p.splits == 1) return e;
+  const int64_t want = (2 * static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.D + 255) / 256;
+  dkv_join_kernel<T><<<static_cast<unsigned>(want < 4096 ? want : 4096), 256, 0, s>>>(a, g, p.splits);
   FA_LAUNCH_CHECK();
   return FA_OK;
 }
 
 template <typename T, int DP>
-int launch_dim(const RelAttn& a, const Grads& g, int chunks, hipStream_t s) {
-  return a.vec * sizeof(T) == 16 ? launch_wide<T, DP, true>(a, g, chunks, s)
-                                 : launch_wide<T, DP, false>(a, g, chunks, s);
+int launch_dim(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
+  return a.vec * sizeof(T) == 16 ? launch_wide<T, DP, true>(a, g, p, s) : launch_wide<T, DP, false>(a, g, p, s);
 }
 
 template <typename T>
-int backward(RelAttn a, Grads g, int rows, void* dtable, int device, hipStream_t s) {
-  const int chunks = g.parts ? chunks_of(a.B, a.H, a.Lq, a.D, a.pos.grid_w, device) : a.B;
+int backward(RelAttn a, Grads g, int rows, void* dtable, const Plan& p, hipStream_t s) {
   const void* in[5] = {a.q, a.k, a.v, g.out, g.dout};
   const View iv[5] = {a.qs, a.ks, a.vs, g.os, g.gs};
   a.vec = widest_load<T>(in, iv, 5, a.D);
@@ -556,12 +632,12 @@ int backward(RelAttn a, Grads g, int rows, void* dtable, int device, hipStream_t
   const View dkv[2] = {g.dks, g.dvs};
   g.dkvec = widest_load<T>(dkp, dkv, 2, a.D);
   int e;
-  if (a.D <= 32) e = launch_dim<T, 32>(a, g, chunks, s);
-  else if (a.D <= 64) e = launch_dim<T, 64>(a, g, chunks, s);
-  else e = launch_dim<T, 128>(a, g, chunks, s);
+  if (a.D <= 32) e = launch_dim<T, 32>(a, g, p, s);
+  else if (a.D <= 64) e = launch_dim<T, 64>(a, g, p, s);
+  else e = launch_dim<T, 128>(a, g, p, s);
   if (e) return e;
   if (dtable) {
-    launch_table_sum<T>(g.parts, chunks * tiles_of(a.Lq), a.pos.n, a.pos.row_of, rows, a.H,
+    launch_table_sum<T>(g.parts, p.chunks * tiles_of(a.Lq, p.nw_q), a.pos.n, a.pos.row_of, rows, a.H,
                         static_cast<T*>(dtable), s);
     FA_LAUNCH_CHECK();
   }
@@ -570,18 +646,36 @@ int backward(RelAttn a, Grads g, int rows, void* dtable, int device, hipStream_t
 
 inline int64_t align16(int64_t v) { return (v + 15) / 16 * 16; }
 
+// The workspace: D_i, the table's sums, the split heads' sums.
+struct Room {
+  int64_t parts, joint, bytes;
+};
+inline Room bwd_room(int B, int H, int Hk, int Lq, int Lk, int D, int n, int grid_w, bool table, int device) {
+  const Plan p = plan_of(B, H, Hk, Lq, Lk, D, grid_w, table, device);
+  Room r;
+  r.parts = align16(static_cast<int64_t>(B) * H * Lq * 4);
+  // (a row for each workgroup of dQ, or of the windows' kernel: at most one for each
+  // entry of the batch then)
+  int64_t rows = static_cast<int64_t>(p.chunks) * tiles_of(Lq, p.nw_q);
+  if (grid_w > 0 && Lq <= 64) rows = rows > window_parts(B, H, device) ? rows : window_parts(B, H, device);
+  r.joint = r.parts + (table ? align16(H * rows * n * 4) : 0);
+  r.bytes = r.joint + (p.splits > 1 ? 2 * p.splits * static_cast<int64_t>(B) * Hk * Lk * D * 4 : 0);
+  return r;
+}
+
 }  // namespace
 }  // namespace fa
 
 extern "C" {
 
-FA_API int fa_gpu_rel_attention_backward_workspace(int B, int H, int Lq, int n, int need_table,
+FA_API int fa_gpu_rel_attention_backward_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int n,
+                                                   int grid_w, int need_table, int device,
                                                    int64_t* out_bytes) {
+  using namespace fa;
   if (!out_bytes) return FA_E_ARG;
-  if (n < 1 || n > FA_REL_MAX) return FA_E_SHAPE;
-  if (const int e = fa::check_attention(B, H, H, Lq, 1, 1, nullptr, 1, nullptr)) return e;
-  const int64_t bh = static_cast<int64_t>(B) * H;
-  *out_bytes = fa::align16(bh * Lq * 4) + (need_table ? bh * fa::tiles_of(Lq) * n * 4 : 0);
+  if (n < 1 || n > FA_REL_MAX || grid_w < 0) return FA_E_SHAPE;
+  if (const int e = check_attention(B, H, Hk, Lq, Lk, D, nullptr, 1, nullptr)) return e;
+  *out_bytes = bwd_room(B, H, Hk, Lq, Lk, D, n, grid_w, need_table != 0, device).bytes;
   return FA_OK;
 }
 
@@ -599,10 +693,8 @@ FA_API int fa_gpu_rel_attention_backward(
   if (const int e = check_attention(B, H, Hk, Lq, Lk, D, mask, mask_b, mask_strides)) return e;
   if (const int e = check_relpos(row_of, rows, lo, n, grid_w, Lq, Lk, q_start, q_starts)) return e;
   if (const int e = check_strides(strides, 8, dtype)) return e;
-  int64_t need = 0;
-  if (const int e = fa_gpu_rel_attention_backward_workspace(B, H, Lq, n, dtable != nullptr, &need))
-    return e;
-  if (workspace_bytes < need) return FA_E_ARG;
+  const Room room = bwd_room(B, H, Hk, Lq, Lk, D, n, grid_w, dtable != nullptr, device);
+  if (workspace_bytes < room.bytes) return FA_E_ARG;
   DeviceScope scope(device);
   if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
   const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table,
@@ -618,22 +710,22 @@ FA_API int fa_gpu_rel_attention_backward(
   g.dvs = {strides[21], strides[22], strides[23]};
   g.lse = lse;
   g.dsum = static_cast<float*>(workspace);
-  g.parts = dtable ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                              align16(static_cast<int64_t>(B) * H * Lq * 4))
-                   : nullptr;
+  char* ws = static_cast<char*>(workspace);
+  g.parts = dtable ? reinterpret_cast<float*>(ws + room.parts) : nullptr;
+  g.joint = reinterpret_cast<float*>(ws + room.joint);
   g.dq = dq;
   g.dk = dk;
   g.dv = dv;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (window_serve(a)) {
-    // (its parts are no more than the workspace's: one for each batch entry at most)
     const WindowGrads w{dout, g.gs, dq, dk, dv, g.dqs, g.dks, g.dvs, g.parts};
     return window_backward(dtype, a, w, rows, dtable, device, s);
   }
+  const Plan p = plan_of(B, H, Hk, Lq, Lk, D, grid_w, dtable != nullptr, device);
   switch (dtype) {
-    case FA_F16: return backward<_Float16>(a, g, rows, dtable, device, s);
-    case FA_BF16: return backward<__bf16>(a, g, rows, dtable, device, s);
-    case FA_F32: return backward<float>(a, g, rows, dtable, device, s);
+    case FA_F16: return backward<_Float16>(a, g, rows, dtable, p, s);
+    case FA_BF16: return backward<__bf16>(a, g, rows, dtable, p, s);
+    case FA_F32: return backward<float>(a, g, rows, dtable, p, s);
     default: return FA_E_DTYPE;
   }
 }

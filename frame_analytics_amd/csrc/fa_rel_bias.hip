@@ -71,7 +71,7 @@ __global__ __launch_bounds__(NT) void rel_bias_kernel(const T* table, int H, int
 // band go to its own n slots (differences past either end into the end slots, through
 // LDS); rel_bias_sum_kernel adds the bands and the differences of a table row.
 // ---------------------------------------------------------------------------
-constexpr int BAND = 64;
+constexpr int BAND = 32;
 
 template <typename T>
 __global__ __launch_bounds__(NT) void rel_bias_bwd_kernel(const T* up, int64_t sh, int64_t si,
@@ -93,14 +93,28 @@ __global__ __launch_bounds__(NT) void rel_bias_bwd_kernel(const T* up, int64_t s
     const int delta = static_cast<int>(d);
     if (pos.grid_w == 0) {
       const int a = max(i0, delta - q0), b = min(i1, delta - q0 + Lk);  // 0 <= j = q0+i-delta < Lk
-      for (int i = a; i < b; ++i) acc += widen(u[i * si + (q0 + i - delta) * sj]);
+      // (eight reads on their way at a time, added in order)
+      const T* p = u + a * si + (static_cast<int64_t>(q0) + a - delta) * sj;
+      int i = a;
+      for (; i + 8 <= b; i += 8, p += 8 * (si + sj)) {
+        T v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = p[e * (si + sj)];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc += widen(v[e]);
+      }
+      for (; i < b; ++i, p += si + sj) acc += widen(*p);
     } else {
       const int w = pos.grid_w, m = 2 * w - 1;
       const int s = delta - pos.lo;  // (dy + hgt - 1) m + dx + w - 1
       const int hgt = Lq / w, dy = s / m - (hgt - 1), dx = s % m - (w - 1);
-      for (int i = i0; i < i1; ++i) {
-        const int y = i / w - dy, x = i % w - dx;
-        if (y >= 0 && y < hgt && x >= 0 && x < w) acc += widen(u[i * si + (y * w + x) * sj]);
+      // the queries of the band whose key, dy rows and dx columns before, is in the window:
+      // a run of columns in each row
+      const int x0 = max(0, dx), x1 = min(w, w + dx);
+      for (int y = max(i0 / w, dy); y <= min((i1 - 1) / w, hgt - 1 + dy); ++y) {
+        const int a = max(y * w + x0, i0), b = min(y * w + x1, i1);
+        const T* p = u + a * si + (a - dy * w - dx) * sj;
+        for (int i = a; i < b; ++i, p += si + sj) acc += widen(*p);
       }
     }
     const int t = delta - pos.lo;

@@ -78,7 +78,8 @@ FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int
  * Sums over heads that share a key head and over the batch are taken in float32 in
  * a fixed order; each result is rounded once.
  */
-FA_API int fa_gpu_rel_attention_backward_workspace(int B, int H, int Lq, int n, int need_table,
+FA_API int fa_gpu_rel_attention_backward_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int n,
+                                                   int grid_w, int need_table, int device,
                                                    int64_t* out_bytes);
 FA_API int fa_gpu_rel_attention_backward(
     const void* q, const void* k, const void* v, const void* out, const void* dout,

@@ -28,7 +28,8 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   T* kt = reinterpret_cast<T*>(smem);           // [2][BN][LD]
   T* vt = kt + 2 * BN * TL::LD;                 // [2][BN][LD]
   float* eb = reinterpret_cast<float*>(vt + 2 * BN * TL::LD);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = q_tiles - 1 - int(wg % q_tiles);  // the longest of a causal head first
   const int h = int(wg / q_tiles) % a.H, b = int(wg / q_tiles) / a.H, hk = h / (a.H / a.Hk);
@@ -70,16 +71,15 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
     kl.store(kt, tid);
     vl.store(vt, tid);
   }
-  for (int t = 0; t < tiles; ++t) {
-    __syncthreads();
+  // One tile of keys.  FAR: every pair of the wave is past one end of the bias table and
+  // counts; WINDOW: a window's pairs, which all count; ANY: the rest.  The first two run
+  // without a branch: with the tests of the third around each product (hidden pairs,
+  // values that are not finite) no instruction of one could overlap the next.
+  enum : int { ANY, FAR, WINDOW };
+  auto work = [&](int t, auto mode, float far) {
+    constexpr int MODE = decltype(mode)::value;
     const T* kk = kt + (t & 1) * BN * TL::LD;
     const T* vv = vt + (t & 1) * BN * TL::LD;
-    const bool more = t + 1 < tiles;
-    if (more) {
-      const int k1 = (t + 1) * BN;
-      kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
-      vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
-    }
     f32x16 s[NB];
     bool partial[NB];
     float top = -INF;
@@ -90,8 +90,22 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
 #pragma unroll
       for (int i = 0; i < CH; ++i)
         s[nb] = M::mma(TL::straight(kk, nb * 32 + col, 16 * i + 8 * hh), qf[i], s[nb]);
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
       const int k0 = t * BN + nb * 32;
-      if (a.pos.grid_w == 0) {
+      partial[nb] = false;
+      if (MODE == WINDOW || (MODE == ANY && a.pos.grid_w)) {
+        const float* e = eb + afresh(cq - a.pos.lo + PAD);
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int4 ck = *reinterpret_cast<const int4*>(codes + k0 + 4 * hh + 8 * r4);
+          s[nb][4 * r4] = s[nb][4 * r4] * c + e[-ck.x];
+          s[nb][4 * r4 + 1] = s[nb][4 * r4 + 1] * c + e[-ck.y];
+          s[nb][4 * r4 + 2] = s[nb][4 * r4 + 2] * c + e[-ck.z];
+          s[nb][4 * r4 + 3] = s[nb][4 * r4 + 3] * c + e[-ck.w];
+        }
+      } else if (MODE == ANY) {
         // differences of the whole block: uniform over the wave
         const int dmax = s0 + qw + 31 - k0, dmin = s0 + qw - (k0 + 31);
         const int kind = block_kind(a.pos, dmin, dmax);
@@ -106,22 +120,15 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[nb][r] = s[nb][r] * c + e;
         }
-      } else {
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const int4 ck = *reinterpret_cast<const int4*>(codes + k0 + 4 * hh + 8 * r4);
-          const float* e = eb + cq - a.pos.lo + PAD;
-          s[nb][4 * r4] = s[nb][4 * r4] * c + e[-ck.x];
-          s[nb][4 * r4 + 1] = s[nb][4 * r4 + 1] * c + e[-ck.y];
-          s[nb][4 * r4 + 2] = s[nb][4 * r4 + 2] * c + e[-ck.z];
-          s[nb][4 * r4 + 3] = s[nb][4 * r4 + 3] * c + e[-ck.w];
-        }
       }
-      partial[nb] = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
-      if (partial[nb]) hide(s[nb], seen_keys(a, mask, qc, qpos, k0 + 4 * hh, len));
+      if (MODE == ANY) {
+        partial[nb] = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
+        if (partial[nb]) hide(s[nb], seen_keys(a, mask, qc, qpos, k0 + 4 * hh, len));
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
     }
+    if (MODE == FAR) top = top * c + far;  // (c > 0)
     top = both_max(top);
     const float mn = fmaxf(m, top);
     if (__ballot(mn > m)) {  // a row's maximum grew: what was summed shrinks by it
@@ -138,7 +145,7 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[nb][r] = __builtin_amdgcn_exp2f(s[nb][r] - sub);
+        s[nb][r] = __builtin_amdgcn_exp2f(MODE == FAR ? s[nb][r] * c + (far - sub) : s[nb][r] - sub);
         l += s[nb][r];
       }
 #pragma unroll
@@ -155,6 +162,23 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
         }
       }
     }
+  };
+  for (int t = 0; t < tiles; ++t) {
+    __syncthreads();
+    const bool more = t + 1 < tiles;
+    const int k0 = t * BN, k1 = k0 + BN;
+    if (more) {
+      kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
+      vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
+    }
+    const bool all = !mask && k1 <= len && (!a.causal || k1 - 1 <= s0 + qw);
+    const int kind = block_kind(a.pos, s0 + qw - (k1 - 1), s0 + qw + 31 - k0);
+    if (all && a.pos.grid_w)
+      work(t, std::integral_constant<int, WINDOW>(), 0.0f);
+    else if (all && kind != NEAR && c > 0.0f)
+      work(t, std::integral_constant<int, FAR>(), kind == ALL_BELOW ? eb[0] : eb[a.pos.n + 2 * PAD - 1]);
+    else
+      work(t, std::integral_constant<int, ANY>(), 0.0f);
     if (more) {
       kl.store(kt + ((t + 1) & 1) * BN * TL::LD, tid);
       vl.store(vt + ((t + 1) & 1) * BN * TL::LD, tid);

@@ -14,6 +14,8 @@ namespace fa {
 
 namespace {
 
+enum : int { ANY, FAR, WINDOW };  // the pairs of a tile
+
 struct Grads {
   const void *out, *dout;
   View os, gs;
@@ -49,8 +51,8 @@ template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<
 // for each window: 1617 us of 2270 for 512 windows of 16 x 16, 8 heads.)  On a line most
 // blocks are far from the wave's queries and are one sum.
 template <typename T, int DP, int NW, bool TABLE, bool WIDE, int KEYS>
-__global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Grads g, int q_tiles,
-                                                                    int chunks) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2 : 1) void rel_attention_dq_kernel(
+    RelAttn a, Grads g, int q_tiles, int chunks) {
   constexpr int NT = NW * 64;
   using M = Mat<T>;
   using TL = Tile<T, DP>;
@@ -63,7 +65,8 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
   const int np = a.pos.n + 2 * PAD;
   float* sums = eb + np;  // [NW][np]: the table's sums by slot, one copy for each wave
   int* codes = reinterpret_cast<int*>(eb + ((TABLE ? 1 + NW : 1) * np + 3) / 4 * 4);  // of a window's keys
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = q_tiles - 1 - int(wg % q_tiles);
   const int h = int(wg / q_tiles) % a.H, chunk = int(wg / q_tiles) / a.H, hk = h / (a.H / a.Hk);
@@ -83,6 +86,7 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
     for (int t = tid; t < NW * np; t += NT) sums[t] = 0.0f;
   float* mine = sums + wave * np;
   float far_lo = 0.0f, far_hi = 0.0f;
+  bool far_below = false;
 
   for (int b = chunk; b < a.B; b += chunks) {
   const int s0 = a.start(b), len = a.keys(b), qpos = s0 + q, cq = s0 + a.pos.code(qc);
@@ -138,21 +142,19 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
     kl.store(kt, tid);
     vl.store(vt, tid);
   }
-  auto work = [&](int t, f32x16* pairs) {
-    __syncthreads();
+  // One tile of keys, as in the forward pass: FAR and WINDOW have no hidden pair and run
+  // without a branch.
+  auto work = [&](int t, f32x16* pairs, auto mode, float far) {
+    constexpr int MODE = decltype(mode)::value;
     const T* kk = kt + (t % BUFS) * BN * TL::LD;
     const T* vv = vt + (t % BUFS) * BN * TL::LD;
-    const bool more = t + 1 < tiles;
-    if (more) {
-      const int k1 = (t + 1) * BN;
-      kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
-      vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
-    }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int k0 = t * BN + nb * 32;
-      const bool hidden = a.causal && k0 > s0 + qw + 31;  // nothing for this wave
-      if (hidden || k0 >= len || qw >= a.Lq) continue;
+      if (MODE == ANY) {
+        const bool hidden = a.causal && k0 > s0 + qw + 31;  // nothing for this wave
+        if (hidden || k0 >= len || qw >= a.Lq) continue;
+      }
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
@@ -161,15 +163,10 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
         s = M::mma(TL::straight(kk, nb * 32 + col, 16 * i + 8 * hh), qf[i], s);
         dp = M::mma(TL::straight(vv, nb * 32 + col, 16 * i + 8 * hh), gf[i], dp);
       }
-      const bool partial = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
-      int kind = NEAR;
+      const bool partial = MODE == ANY && (mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw));
+      int kind = MODE == FAR ? ALL_BELOW : NEAR;
       int slot[16];  // of each pair, where it has one of its own
-      if (KEYS == 0 && a.pos.grid_w == 0) {
-        kind = block_kind(a.pos, s0 + qw - (k0 + 31), s0 + qw + 31 - k0);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          slot[r] = s0 + q - k0 - 4 * hh - a.pos.lo + PAD - (8 * (r / 4) + r % 4);
-      } else {
+      if (MODE == WINDOW || (MODE == ANY && a.pos.grid_w)) {
         // (codes are those of the window's keys, the last one's past its end)
         const int at = afresh(cq - a.pos.lo + PAD);
 #pragma unroll
@@ -180,20 +177,25 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
           slot[4 * r4 + 2] = at - ck.z;
           slot[4 * r4 + 3] = at - ck.w;
         }
-      }
-      if (KEYS > 0 || kind == NEAR) {
+      } else if (MODE == ANY) {
+        kind = block_kind(a.pos, s0 + qw - (k0 + 31), s0 + qw + 31 - k0);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + eb[slot[r]];
+        for (int r = 0; r < 16; ++r)
+          slot[r] = s0 + q - k0 - 4 * hh - a.pos.lo + PAD - (8 * (r / 4) + r % 4);
+      }
+      if (MODE == FAR) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + (far - lse);
+      } else if (MODE == WINDOW || kind == NEAR) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + eb[slot[r]] - lse;
       } else {
         const float e = kind == ALL_BELOW ? eb[0] : eb[np - 1];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + e;
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + e - lse;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(s[r] - lse);
-        s[r] = p * (dp[r] - dsum);
-      }
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]) * (dp[r] - dsum);
       if (partial) {
         const uint32_t seen = seen_keys(a, mask, qc, qpos, k0 + 4 * hh, len);
 #pragma unroll
@@ -203,7 +205,7 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
 #pragma unroll
         for (int r = 0; r < 16; ++r) pairs[nb][r] += s[r];
       } else if (TABLE) {
-        if (kind == NEAR) {
+        if (MODE != FAR && kind == NEAR) {
           // within one half of the lanes one key meets 32 queries: 32 slots.  The
           // halves add one after the other, so the order of every slot's sum is fixed.
           if (hh == 0) {
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc += s[r];
           acc = q < a.Lq ? acc : 0.0f;
-          if (kind == ALL_BELOW) far_lo += acc;
+          if (MODE == FAR ? far_below : kind == ALL_BELOW) far_lo += acc;
           else far_hi += acc;
         }
       }
@@ -240,6 +242,24 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
         }
       }
     }
+  };
+  auto step = [&](int t, f32x16* pairs) {
+    __syncthreads();
+    const bool more = t + 1 < tiles;
+    const int k0 = t * BN, k1 = k0 + BN;
+    if (more) {
+      kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
+      vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
+    }
+    const bool all = !mask && k1 <= len && (!a.causal || k1 - 1 <= s0 + qw) && qw < a.Lq;
+    const int kind = block_kind(a.pos, s0 + qw - (k1 - 1), s0 + qw + 31 - k0);
+    far_below = kind == ALL_BELOW;
+    if (KEYS > 0 && all)
+      work(t, pairs, std::integral_constant<int, WINDOW>(), 0.0f);
+    else if (KEYS == 0 && all && a.pos.grid_w == 0 && kind != NEAR)
+      work(t, pairs, std::integral_constant<int, KEYS == 0 ? FAR : ANY>(), far_below ? eb[0] : eb[np - 1]);
+    else
+      work(t, pairs, std::integral_constant<int, ANY>(), 0.0f);
     if (more) {
       if (BUFS == 1) __syncthreads();
       kl.store(kt + ((t + 1) % BUFS) * BN * TL::LD, tid);
@@ -249,9 +269,9 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
   if constexpr (KEYS > 0) {
 #pragma unroll
     for (int t = 0; t < KEYS / NB; ++t)
-      if (t < tiles) work(t, total + t * NB);
+      if (t < tiles) step(t, total + t * NB);
   } else {
-    for (int t = 0; t < tiles; ++t) work(t, total);
+    for (int t = 0; t < tiles; ++t) step(t, total);
   }
   if (q < a.Lq) {
     T* drow = static_cast<T*>(g.dq) + b * g.dqs.b + h * g.dqs.h + q * g.dqs.t;
@@ -311,8 +331,8 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dq_kernel(RelAttn a, Gr
 // The query heads that share a key head may be split between workgroups, whose float32
 // sums dkv_join_kernel adds in order.
 template <typename T, int DP, int NW, bool WIDE>
-__global__ __launch_bounds__(NW * 64) void rel_attention_dkv_kernel(RelAttn a, Grads g, int k_tiles,
-                                                                    int splits) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void rel_attention_dkv_kernel(
+    RelAttn a, Grads g, int k_tiles, int splits) {
   constexpr int NT = NW * 64;
   using M = Mat<T>;
   using TL = Tile<T, DP>;
@@ -326,7 +346,8 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dkv_kernel(RelAttn a, G
   float* ls = eb + (np + 3) / 4 * 4;  // [2][BM]: each query's log-sum
   float* dd = ls + 2 * BM;            // [2][BM]: and D_i
   int* codes = reinterpret_cast<int*>(dd + 2 * BM);  // of a window's queries
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = int(wg % k_tiles), split = int(wg / k_tiles) % splits;
   const int hk = int(wg / k_tiles / splits) % a.Hk, b = int(wg / k_tiles / splits) / a.Hk;
@@ -410,10 +431,12 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dkv_kernel(RelAttn a, G
       const float* dt = dd + (t & 1) * BM;
       const bool more = t + 1 < tiles;
       if (more) load(t + 1);
+      auto work = [&](auto mode, float far) {
+      constexpr int MODE = decltype(mode)::value;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const int i0 = t * BM + nb * 32;  // the block's first query
-        if ((a.causal && s0 + i0 + 31 < kw) || kw >= len || i0 >= a.Lq) continue;
+        if (MODE == ANY && ((a.causal && s0 + i0 + 31 < kw) || kw >= len || i0 >= a.Lq)) continue;
         f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
@@ -422,9 +445,12 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dkv_kernel(RelAttn a, G
           s = M::mma(TL::straight(qq, nb * 32 + col, 16 * i + 8 * hh), kf[i], s);
           dp = M::mma(TL::straight(gg, nb * 32 + col, 16 * i + 8 * hh), vf[i], dp);
         }
-        const bool partial = mask || kw + 32 > len || (a.causal && kw + 31 > s0 + i0);
+        const bool partial = MODE == ANY && (mask || kw + 32 > len || (a.causal && kw + 31 > s0 + i0));
         int kind = NEAR;
-        if (a.pos.grid_w == 0) {
+        if (MODE == FAR) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = s[r] * c + far;
+        } else if (MODE == ANY && a.pos.grid_w == 0) {
           kind = block_kind(a.pos, s0 + i0 - (kw + 31), s0 + i0 + 31 - kw);
           if (kind == NEAR) {
             const float* e = eb + (s0 + i0 + 4 * hh - key - a.pos.lo + PAD);
@@ -485,6 +511,16 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_dkv_kernel(RelAttn a, G
           }
         }
       }
+      };
+      const int q0 = t * BM, q1 = q0 + BM;  // the tile's queries
+      const bool all = !mask && kw + 32 <= len && q1 <= a.Lq && (!a.causal || kw + 31 <= s0 + q0);
+      const int kind = block_kind(a.pos, s0 + q0 - (kw + 31), s0 + q1 - 1 - kw);
+      if (all && a.pos.grid_w)
+        work(std::integral_constant<int, WINDOW>(), 0.0f);
+      else if (all && kind != NEAR)
+        work(std::integral_constant<int, FAR>(), kind == ALL_BELOW ? eb[0] : eb[np - 1]);
+      else
+        work(std::integral_constant<int, ANY>(), 0.0f);
       if (more) {
         if (BUFS == 1) __syncthreads();
         store(t + 1);

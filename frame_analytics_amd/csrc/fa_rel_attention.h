@@ -221,6 +221,8 @@ inline RelAttn rel_attn_args(const void* q, const void* k, const void* v, int B,
   return a;
 }
 
+constexpr size_t MOST_LDS = 160 * 1024;  // a workgroup's
+
 // Raises a kernel's limit of LDS per workgroup where a launch asks for more than the
 // default; the limit is the device's.
 template <typename K> inline int launch_lds(K kernel, size_t bytes) {

@@ -17,18 +17,21 @@ template <typename T, int DP> struct Shape {
   static constexpr size_t TILE = size_t(BN) * Tile<T, DP>::LD * sizeof(T);
 };
 
-template <typename T, int DP, int NW, bool WIDE>
-__global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* out, View os,
+// KG groups of NW waves take every KG-th tile of keys for the same queries, and join their
+// sums at the end: where there are few workgroups the longest row of tiles is the time.
+template <typename T, int DP, int NW, int KG, bool WIDE>
+__global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, T* out, View os,
                                                                 int ovec, float* lse,
                                                                 int q_tiles) {
   using M = Mat<T>;
   using TL = Tile<T, DP>;
   constexpr int NT = NW * 64, BN = Shape<T, DP>::BN, NB = BN / 32, CH = DP / 16, OB = DP / 32;
   extern __shared__ __align__(16) unsigned char smem[];
-  T* kt = reinterpret_cast<T*>(smem);           // [2][BN][LD]
-  T* vt = kt + 2 * BN * TL::LD;                 // [2][BN][LD]
-  float* eb = reinterpret_cast<float*>(vt + 2 * BN * TL::LD);
-  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+  T* kt = reinterpret_cast<T*>(smem) + kg * 4 * BN * TL::LD;  // [2][BN][LD] of each group
+  T* vt = kt + 2 * BN * TL::LD;                               // [2][BN][LD]
+  float* eb = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + KG * 4 * BN * TL::LD);
+  const int tid = threadIdx.x - kg * NT, lane = tid & 63, hh = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = q_tiles - 1 - int(wg % q_tiles);  // the longest of a causal head first
@@ -40,8 +43,8 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   const float c = a.scale * LOG2E;
 
   int* codes = reinterpret_cast<int*>(eb + (a.pos.n + 2 * PAD + 3) / 4 * 4);  // of a window's keys
-  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
-  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, tid, NT);
+  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, threadIdx.x, NT * KG);
+  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, threadIdx.x, NT * KG);
 
   typename M::V8 qf[CH];
   const int q_first = tile * (NW * 32);
@@ -65,9 +68,10 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   const T* vb = static_cast<const T*>(a.v) + b * a.vs.b + hk * a.vs.h;
   TileLoad<T, DP, BN, NT, WIDE> kl, vl;
   const int tiles = (end + BN - 1) / BN;
-  if (tiles > 0) {
-    kl.load(kb, a.ks.t, len, a.D, a.vec, tid);
-    vl.load(vb, a.vs.t, len, a.D, a.vec, tid);
+  if (kg < tiles) {
+    const int k1 = kg * BN;
+    kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
+    vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
   }
@@ -78,8 +82,8 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   enum : int { ANY, FAR, WINDOW };
   auto work = [&](int t, auto mode, float far) {
     constexpr int MODE = decltype(mode)::value;
-    const T* kk = kt + (t & 1) * BN * TL::LD;
-    const T* vv = vt + (t & 1) * BN * TL::LD;
+    const T* kk = kt + (t / KG & 1) * BN * TL::LD;
+    const T* vv = vt + (t / KG & 1) * BN * TL::LD;
     f32x16 s[NB];
     bool partial[NB];
     float top = -INF;
@@ -163,16 +167,19 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
       }
     }
   };
-  for (int t = 0; t < tiles; ++t) {
+  const int rounds = (tiles + KG - 1) / KG;
+  for (int round = 0; round < rounds; ++round) {
+    const int t = round * KG + kg;
     __syncthreads();
-    const bool more = t + 1 < tiles;
-    const int k0 = t * BN, k1 = k0 + BN;
+    if (t >= tiles) continue;  // (in the last round)
+    const bool more = t + KG < tiles;
+    const int k0 = t * BN, k1 = k0 + KG * BN;
     if (more) {
       kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
       vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
     }
-    const bool all = !mask && k1 <= len && (!a.causal || k1 - 1 <= s0 + qw);
-    const int kind = block_kind(a.pos, s0 + qw - (k1 - 1), s0 + qw + 31 - k0);
+    const bool all = !mask && k0 + BN <= len && (!a.causal || k0 + BN - 1 <= s0 + qw);
+    const int kind = block_kind(a.pos, s0 + qw - (k0 + BN - 1), s0 + qw + 31 - k0);
     if (all && a.pos.grid_w)
       work(t, std::integral_constant<int, WINDOW>(), 0.0f);
     else if (all && kind != NEAR && c > 0.0f)
@@ -180,9 +187,33 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
     else
       work(t, std::integral_constant<int, ANY>(), 0.0f);
     if (more) {
-      kl.store(kt + ((t + 1) & 1) * BN * TL::LD, tid);
-      vl.store(vt + ((t + 1) & 1) * BN * TL::LD, tid);
+      kl.store(kt + ((t / KG + 1) & 1) * BN * TL::LD, tid);
+      vl.store(vt + ((t / KG + 1) & 1) * BN * TL::LD, tid);
     }
+  }
+  if constexpr (KG > 1) {
+    static_assert(KG == 2, "the second group's sums join the first's");
+    float* sums = reinterpret_cast<float*>(smem) + wave * (OB * 16 + 2) * 64 + lane;
+    __syncthreads();
+    if (kg == 1) {
+#pragma unroll
+      for (int i = 0; i < OB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[(16 * i + r) * 64] = o[i][r];
+      sums[OB * 16 * 64] = m;
+      sums[(OB * 16 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const float m1 = sums[OB * 16 * 64], mn = fmaxf(m, m1);
+    const float f0 = m == -INF ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float f1 = m1 == -INF ? 0.0f : __builtin_amdgcn_exp2f(m1 - mn);
+    l = l * f0 + sums[(OB * 16 + 1) * 64] * f1;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] = o[i][r] * f0 + sums[(16 * i + r) * 64] * f1;
   }
   l = both_sum(l);
   if (q < a.Lq) {
@@ -202,30 +233,43 @@ __global__ __launch_bounds__(NW * 64) void rel_attention_kernel(RelAttn a, T* ou
   }
 }
 
-template <typename T, int DP, int NW, bool WIDE>
+template <typename T, int DP, int NW, int KG, bool WIDE>
 int launch_one(const RelAttn& a, T* out, const View& os, int ovec, float* lse, hipStream_t s) {
   const int q_tiles = (a.Lq + NW * 32 - 1) / (NW * 32);
   const int64_t wgs = static_cast<int64_t>(a.B) * a.H * q_tiles;
   if (wgs > 0x7fffffff) return FA_E_SHAPE;
-  const size_t lds = 4 * Shape<T, DP>::TILE + (a.pos.n + 2 * PAD + 3) / 4 * 16 +
+  const size_t lds = KG * 4 * Shape<T, DP>::TILE + (a.pos.n + 2 * PAD + 3) / 4 * 16 +
                      (a.pos.grid_w ? codes_room(a.Lk) * sizeof(int) : 0);
-  auto kernel = rel_attention_kernel<T, DP, NW, WIDE>;
+  if constexpr (KG > 1)  // a table that leaves no room for the second group's tiles
+    if (lds > MOST_LDS) return launch_one<T, DP, NW, 1, WIDE>(a, out, os, ovec, lse, s);
+  auto kernel = rel_attention_kernel<T, DP, NW, KG, WIDE>;
   if (const int e = launch_lds(kernel, lds)) return e;
-  kernel<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, out, os, ovec, lse, q_tiles);
+  kernel<<<static_cast<unsigned>(wgs), NW * 64 * KG, lds, s>>>(a, out, os, ovec, lse, q_tiles);
   FA_LAUNCH_CHECK();
   return FA_OK;
 }
 
+template <typename T, int DP, bool WIDE>
+int launch_wide(const RelAttn& a, T* out, const View& os, int ovec, float* lse, int device, hipStream_t s) {
+  // two waves to a workgroup where four leave compute units without one (256 workgroups of
+  // four took 86 us where 512 of two took 101, a causal line of 2048), and a second group
+  // of waves where there are less than two workgroups for every compute unit
+  const int cus = cu_count(device);
+  const int64_t four = static_cast<int64_t>(a.B) * a.H * ((a.Lq + 127) / 128);
+  const bool few = a.Lq <= 64 || four < cus;
+  const int64_t wgs = few ? static_cast<int64_t>(a.B) * a.H * ((a.Lq + 63) / 64) : four;
+  if constexpr (DP <= 64)
+    if (wgs < 2 * cus && a.Lk > 2 * Shape<T, DP>::BN)
+      return few ? launch_one<T, DP, 2, 2, WIDE>(a, out, os, ovec, lse, s)
+                 : launch_one<T, DP, 4, 2, WIDE>(a, out, os, ovec, lse, s);
+  return few ? launch_one<T, DP, 2, 1, WIDE>(a, out, os, ovec, lse, s)
+             : launch_one<T, DP, 4, 1, WIDE>(a, out, os, ovec, lse, s);
+}
+
 template <typename T, int DP>
 int launch_dim(const RelAttn& a, T* out, const View& os, int ovec, float* lse, int device, hipStream_t s) {
-  // two waves to a workgroup where four leave compute units without one (256 workgroups of
-  // four took 86 us where 512 of two took 101, a causal line of 2048)
-  const bool few = a.Lq <= 64 || static_cast<int64_t>(a.B) * a.H * ((a.Lq + 127) / 128) < cu_count(device);
-  if (a.vec * sizeof(T) == 16)
-    return few ? launch_one<T, DP, 2, true>(a, out, os, ovec, lse, s)
-               : launch_one<T, DP, 4, true>(a, out, os, ovec, lse, s);
-  return few ? launch_one<T, DP, 2, false>(a, out, os, ovec, lse, s)
-             : launch_one<T, DP, 4, false>(a, out, os, ovec, lse, s);
+  return a.vec * sizeof(T) == 16 ? launch_wide<T, DP, true>(a, out, os, ovec, lse, device, s)
+                                 : launch_wide<T, DP, false>(a, out, os, ovec, lse, device, s);
 }
 
 template <typename T>

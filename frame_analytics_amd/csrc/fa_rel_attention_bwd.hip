@@ -50,8 +50,9 @@ template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<
 // them in registers, to reach the table's differences once at the end.  (By LDS atomics
 // for each window: 1617 us of 2270 for 512 windows of 16 x 16, 8 heads.)  On a line most
 // blocks are far from the wave's queries and are one sum.
-template <typename T, int DP, int NW, bool TABLE, bool WIDE, int KEYS>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2 : 1) void rel_attention_dq_kernel(
+// KG groups of NW waves take every KG-th tile of keys, as in the forward pass.
+template <typename T, int DP, int NW, int KG, bool TABLE, bool WIDE, int KEYS>
+__global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2 : 1) void rel_attention_dq_kernel(
     RelAttn a, Grads g, int q_tiles, int chunks) {
   constexpr int NT = NW * 64;
   using M = Mat<T>;
@@ -59,13 +60,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
   constexpr int BN = Shape<T, DP>::BN, NB = BN / 32, CH = DP / 16, OB = DP / 32;
   constexpr int BUFS = Shape<T, DP>::BUFS;
   extern __shared__ __align__(16) unsigned char smem[];
-  T* kt = reinterpret_cast<T*>(smem);
+  static_assert(KG == 1 || (BUFS == 2 && KEYS == 0), "a second group");
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+  T* kt = reinterpret_cast<T*>(smem) + kg * 2 * BUFS * BN * TL::LD;
   T* vt = kt + BUFS * BN * TL::LD;
-  float* eb = reinterpret_cast<float*>(vt + BUFS * BN * TL::LD);
+  float* eb = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + KG * 2 * BUFS * BN * TL::LD);
   const int np = a.pos.n + 2 * PAD;
-  float* sums = eb + np;  // [NW][np]: the table's sums by slot, one copy for each wave
-  int* codes = reinterpret_cast<int*>(eb + ((TABLE ? 1 + NW : 1) * np + 3) / 4 * 4);  // of a window's keys
-  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
+  float* sums = eb + np;  // [KG * NW][np]: the table's sums by slot, one copy for each wave
+  int* codes = reinterpret_cast<int*>(eb + ((TABLE ? 1 + KG * NW : 1) * np + 3) / 4 * 4);  // of a window's keys
+  const int tid = threadIdx.x - kg * NT, lane = tid & 63, hh = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = q_tiles - 1 - int(wg % q_tiles);
@@ -74,8 +77,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
   const int q = qw + col, qc = min(q, a.Lq - 1);
   const float c = a.scale * LOG2E;
 
-  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
-  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, tid, NT);
+  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, threadIdx.x, NT * KG);
+  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, threadIdx.x, NT * KG);
   constexpr int TOTALS = KEYS > 0 ? KEYS : 1;
   f32x16 total[TOTALS];
 #pragma unroll
@@ -83,8 +86,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
 #pragma unroll
     for (int r = 0; r < 16; ++r) total[i][r] = 0.0f;
   if (TABLE && KEYS == 0)
-    for (int t = tid; t < NW * np; t += NT) sums[t] = 0.0f;
-  float* mine = sums + wave * np;
+    for (int t = threadIdx.x; t < KG * NW * np; t += KG * NT) sums[t] = 0.0f;
+  float* mine = sums + (kg * NW + wave) * np;
   float far_lo = 0.0f, far_hi = 0.0f;
   bool far_below = false;
 
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
   for (int r = 0; r < 16; ++r)
     if (8 * (r / 4) + 4 * hh + r % 4 == col) dsum = dd[r];
   dsum = both_sum(dsum);
-  if (q < a.Lq && hh == 0) g.dsum[row] = dsum;
+  if (kg == 0 && q < a.Lq && hh == 0) g.dsum[row] = dsum;
 
   f32x16 dq[OB];
 #pragma unroll
@@ -136,9 +139,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
   TileLoad<T, DP, BN, NT, WIDE> kl, vl;
   const int tiles = (end + BN - 1) / BN;
   if (KEYS > 0) __syncthreads();  // the window before is done with the tiles
-  if (tiles > 0) {
-    kl.load(kb, a.ks.t, len, a.D, a.vec, tid);
-    vl.load(vb, a.vs.t, len, a.D, a.vec, tid);
+  if (kg < tiles) {
+    const int k1 = kg * BN;
+    kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
+    vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
     kl.store(kt, tid);
     vl.store(vt, tid);
   }
@@ -146,8 +150,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
   // without a branch.
   auto work = [&](int t, f32x16* pairs, auto mode, float far) {
     constexpr int MODE = decltype(mode)::value;
-    const T* kk = kt + (t % BUFS) * BN * TL::LD;
-    const T* vv = vt + (t % BUFS) * BN * TL::LD;
+    const T* kk = kt + (t / KG % BUFS) * BN * TL::LD;
+    const T* vv = vt + (t / KG % BUFS) * BN * TL::LD;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int k0 = t * BN + nb * 32;
@@ -245,14 +249,15 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
   };
   auto step = [&](int t, f32x16* pairs) {
     __syncthreads();
-    const bool more = t + 1 < tiles;
-    const int k0 = t * BN, k1 = k0 + BN;
+    if (KG > 1 && t >= tiles) return;  // (in the last round)
+    const bool more = t + KG < tiles;
+    const int k0 = t * BN, k1 = k0 + KG * BN;
     if (more) {
       kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
       vl.load(vb + k1 * a.vs.t, a.vs.t, len - k1, a.D, a.vec, tid);
     }
-    const bool all = !mask && k1 <= len && (!a.causal || k1 - 1 <= s0 + qw) && qw < a.Lq;
-    const int kind = block_kind(a.pos, s0 + qw - (k1 - 1), s0 + qw + 31 - k0);
+    const bool all = !mask && k0 + BN <= len && (!a.causal || k0 + BN - 1 <= s0 + qw) && qw < a.Lq;
+    const int kind = block_kind(a.pos, s0 + qw - (k0 + BN - 1), s0 + qw + 31 - k0);
     far_below = kind == ALL_BELOW;
     if (KEYS > 0 && all)
       work(t, pairs, std::integral_constant<int, WINDOW>(), 0.0f);
@@ -262,8 +267,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
       work(t, pairs, std::integral_constant<int, ANY>(), 0.0f);
     if (more) {
       if (BUFS == 1) __syncthreads();
-      kl.store(kt + ((t + 1) % BUFS) * BN * TL::LD, tid);
-      vl.store(vt + ((t + 1) % BUFS) * BN * TL::LD, tid);
+      kl.store(kt + ((t / KG + 1) % BUFS) * BN * TL::LD, tid);
+      vl.store(vt + ((t / KG + 1) % BUFS) * BN * TL::LD, tid);
     }
   };
   if constexpr (KEYS > 0) {
@@ -271,9 +276,26 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
     for (int t = 0; t < KEYS / NB; ++t)
       if (t < tiles) step(t, total + t * NB);
   } else {
-    for (int t = 0; t < tiles; ++t) step(t, total);
+    const int rounds = (tiles + KG - 1) / KG;
+    for (int round = 0; round < rounds; ++round) step(round * KG + kg, total);
   }
-  if (q < a.Lq) {
+  if constexpr (KG > 1) {
+    static_assert(KG == 2, "the second group's sums join the first's");
+    float* joint = reinterpret_cast<float*>(smem) + wave * OB * 16 * 64 + lane;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (kg == 1) joint[(16 * i + r) * 64] = dq[i][r];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (kg == 0) dq[i][r] += joint[(16 * i + r) * 64];
+  }
+  if (kg == 0 && q < a.Lq) {
     T* drow = static_cast<T*>(g.dq) + b * g.dqs.b + h * g.dqs.h + q * g.dqs.t;
 #pragma unroll
     for (int i = 0; i < OB; ++i)
@@ -305,6 +327,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
     }
   }
   if (TABLE) {
+    __syncthreads();  // (the zeros, where no tile of keys came between)
     // what the padding holds belongs to the ends
     far_lo += mine[lane];  // slots 0 .. PAD - 1
     far_hi += mine[a.pos.n + PAD + lane];
@@ -316,10 +339,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
     }
     __syncthreads();
     float* dst = g.parts + (static_cast<int64_t>(h) * chunks * q_tiles + chunk * q_tiles + tile) * a.pos.n;
-    for (int t = tid; t < a.pos.n; t += NT) {
+    for (int t = threadIdx.x; t < a.pos.n; t += KG * NT) {
       float v = 0.0f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) v += sums[w * np + PAD + t];
+      for (int w = 0; w < KG * NW; ++w) v += sums[w * np + PAD + t];
       dst[t] = v;
     }
   }
@@ -330,8 +353,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2
 // ---------------------------------------------------------------------------
 // The query heads that share a key head may be split between workgroups, whose float32
 // sums dkv_join_kernel adds in order.
-template <typename T, int DP, int NW, bool WIDE>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void rel_attention_dkv_kernel(
+template <typename T, int DP, int NW, int KG, bool WIDE>
+__global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 ? (DP == 32 ? 3 : DP == 64 ? 2 : 1) : 1) void rel_attention_dkv_kernel(
     RelAttn a, Grads g, int k_tiles, int splits) {
   constexpr int NT = NW * 64;
   using M = Mat<T>;
@@ -339,14 +362,16 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void r
   constexpr int BM = Shape<T, DP>::BN, NB = BM / 32, CH = DP / 16, OB = DP / 32;
   constexpr int BUFS = Shape<T, DP>::BUFS;
   extern __shared__ __align__(16) unsigned char smem[];
-  T* qt = reinterpret_cast<T*>(smem);
+  static_assert(KG == 1 || BUFS == 2, "a second group");
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+  T* qt = reinterpret_cast<T*>(smem) + kg * 2 * BUFS * BM * TL::LD;
   T* gt = qt + BUFS * BM * TL::LD;
-  float* eb = reinterpret_cast<float*>(gt + BUFS * BM * TL::LD);
+  float* eb = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + KG * 2 * BUFS * BM * TL::LD);
   const int np = a.pos.n + 2 * PAD;
-  float* ls = eb + (np + 3) / 4 * 4;  // [2][BM]: each query's log-sum
-  float* dd = ls + 2 * BM;            // [2][BM]: and D_i
-  int* codes = reinterpret_cast<int*>(dd + 2 * BM);  // of a window's queries
-  const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, col = lane & 31;
+  float* ls = eb + (np + 3) / 4 * 4 + kg * 4 * BM;  // [2][BM]: each query's log-sum
+  float* dd = ls + 2 * BM;                          // [2][BM]: and D_i
+  int* codes = reinterpret_cast<int*>(eb + (np + 3) / 4 * 4 + KG * 4 * BM);  // of a window's queries
+  const int tid = threadIdx.x - kg * NT, lane = tid & 63, hh = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned wg = xcd_tile(blockIdx.x, gridDim.x);
   const int tile = int(wg % k_tiles), split = int(wg / k_tiles) % splits;
@@ -357,7 +382,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void r
   const int ck = a.pos.code(kc);
   const float c = a.scale * LOG2E;
   const int k_first = tile * (NW * 32);
-  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lq, tid, NT);
+  if (a.pos.grid_w) load_codes(codes, a.pos, a.Lq, threadIdx.x, NT * KG);
 
   typename M::V8 kf[CH], vf[CH];
   load_row<T, WIDE>(kf, Rows<T>(static_cast<const T*>(a.k) + b * a.ks.b + hk * a.ks.h + k_first * a.ks.t, a.ks.t),
@@ -376,7 +401,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void r
     const int64_t f = static_cast<int64_t>(k_first) - s0;
     first = static_cast<int>(max<int64_t>(0, min<int64_t>(f, a.Lq)));
   }
-  const int t0 = first / BM;
+  const int t0 = first / BM / KG * KG;  // (a tile's buffer goes by t / KG)
   const int tiles = k_first < len ? (a.Lq + BM - 1) / BM : 0;
   TileLoad<T, DP, BM, NT, WIDE> ql, gl;
   float lse_r = 0.0f, d_r = 0.0f;
@@ -410,27 +435,30 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void r
         if (row_lse[i] == INF)
 #pragma unroll
           for (int e = 0; e < 8; ++e) ql.r[i][e] = gl.r[i][e] = T(0);
-      ql.store(qt + (t % BUFS) * BM * TL::LD, tid);
-      gl.store(gt + (t % BUFS) * BM * TL::LD, tid);
+      ql.store(qt + (t / KG % BUFS) * BM * TL::LD, tid);
+      gl.store(gt + (t / KG % BUFS) * BM * TL::LD, tid);
       if (tid < BM) {
-        ls[(t & 1) * BM + tid] = lse_r;
-        dd[(t & 1) * BM + tid] = d_r;
+        ls[(t / KG & 1) * BM + tid] = lse_r;
+        dd[(t / KG & 1) * BM + tid] = d_r;
       }
     };
     __syncthreads();  // the head before is done with its tiles and bias
-    load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, tid, NT);
-    if (t0 < tiles) {
-      load(t0);
-      store(t0);
+    load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, threadIdx.x, NT * KG);
+    if (t0 + kg < tiles) {
+      load(t0 + kg);
+      store(t0 + kg);
     }
-    for (int t = t0; t < tiles; ++t) {
+    const int rounds = tiles > t0 ? (tiles - t0 + KG - 1) / KG : 0;
+    for (int round = 0; round < rounds; ++round) {
+      const int t = t0 + round * KG + kg;
       __syncthreads();
-      const T* qq = qt + (t % BUFS) * BM * TL::LD;
-      const T* gg = gt + (t % BUFS) * BM * TL::LD;
-      const float* lt = ls + (t & 1) * BM;
-      const float* dt = dd + (t & 1) * BM;
-      const bool more = t + 1 < tiles;
-      if (more) load(t + 1);
+      if (KG > 1 && t >= tiles) continue;  // (in the last round)
+      const T* qq = qt + (t / KG % BUFS) * BM * TL::LD;
+      const T* gg = gt + (t / KG % BUFS) * BM * TL::LD;
+      const float* lt = ls + (t / KG & 1) * BM;
+      const float* dt = dd + (t / KG & 1) * BM;
+      const bool more = t + KG < tiles;
+      if (more) load(t + KG);
       auto work = [&](auto mode, float far) {
       constexpr int MODE = decltype(mode)::value;
 #pragma unroll
@@ -523,9 +551,31 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && DP <= 64 ? 2 : 1) void r
         work(std::integral_constant<int, ANY>(), 0.0f);
       if (more) {
         if (BUFS == 1) __syncthreads();
-        store(t + 1);
+        store(t + KG);
       }
     }
+  }
+  if constexpr (KG > 1) {
+    static_assert(KG == 2, "the second group's sums join the first's");
+    float* joint = reinterpret_cast<float*>(smem) + wave * OB * 32 * 64 + lane;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (kg == 1) {
+          joint[(32 * i + r) * 64] = dk[i][r];
+          joint[(32 * i + 16 + r) * 64] = dv[i][r];
+        }
+    __syncthreads();
+    if (kg == 1) return;
+#pragma unroll
+    for (int i = 0; i < OB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        dk[i][r] += joint[(32 * i + r) * 64];
+        dv[i][r] += joint[(32 * i + 16 + r) * 64];
+      }
   }
   if (key < a.Lk && splits > 1) {
     const int64_t each = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.D;
@@ -584,6 +634,7 @@ inline int tiles_of(int n, int nw) { return (n + nw * 32 - 1) / (nw * 32); }
 // against 119 and, the shared heads split, 137).
 struct Plan {
   int nw_q, nw_k;  // waves of the workgroups that own queries, and keys
+  int kg_q, kg_k;  // groups of them
   int chunks;      // batch entries in parallel for dQ: all, unless windows' sums stay in registers
   bool registers;
   int splits;      // of the query heads of a key head
@@ -594,6 +645,11 @@ inline Plan plan_of(int B, int H, int Hk, int Lq, int Lk, int D, int grid_w, boo
   p.registers = table && grid_w > 0 && Lq <= 256 && D <= 64;
   p.nw_q = p.registers || static_cast<int64_t>(B) * H * tiles_of(Lq, 4) >= cu_count(device) ? 4 : 2;
   p.nw_k = static_cast<int64_t>(B) * Hk * tiles_of(Lk, 4) >= cu_count(device) ? 4 : 2;
+  p.kg_q = p.kg_k = 1;
+  if (D <= 64) {
+    if (!p.registers && static_cast<int64_t>(B) * H * tiles_of(Lq, p.nw_q) < enough && Lk > 128) p.kg_q = 2;
+    if (static_cast<int64_t>(B) * Hk * tiles_of(Lk, p.nw_k) < enough && Lq > 128) p.kg_k = 2;
+  }
   p.chunks = B;
   if (p.registers) {  // two workgroups for every compute unit
     const int64_t each = static_cast<int64_t>(H) * tiles_of(Lq, 4), want = (enough + each - 1) / each;
@@ -605,46 +661,61 @@ inline Plan plan_of(int B, int H, int Hk, int Lq, int Lk, int D, int grid_w, boo
   return p;
 }
 
-template <typename T, int DP, int NW, bool WIDE>
+template <typename T, int DP, int NW, int KG, bool WIDE>
 int launch_dq(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
   const int qt = tiles_of(a.Lq, NW);
   const int64_t wgs = static_cast<int64_t>(p.chunks) * a.H * qt;
   if (wgs > 0x7fffffff) return FA_E_SHAPE;
-  const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
-  const size_t lds = tiles + ((g.parts ? 1 + NW : 1) * np + 3) / 4 * 16 +
+  const size_t np = a.pos.n + 2 * PAD, tiles = KG * 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
+  const size_t lds = tiles + ((g.parts ? 1 + KG * NW : 1) * np + 3) / 4 * 16 +
                      (a.pos.grid_w ? codes_room(a.Lk) * sizeof(int) : 0);
-  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, NW, true, WIDE, 0>
-                    : rel_attention_dq_kernel<T, DP, NW, false, WIDE, 0>;
-  if constexpr (DP <= 64 && NW == 4)
+  if constexpr (KG > 1)  // a table that leaves no room for the second group's sums
+    if (lds > MOST_LDS) return launch_dq<T, DP, NW, 1, WIDE>(a, g, p, s);
+  auto dq = g.parts ? rel_attention_dq_kernel<T, DP, NW, KG, true, WIDE, 0>
+                    : rel_attention_dq_kernel<T, DP, NW, KG, false, WIDE, 0>;
+  if constexpr (DP <= 64 && NW == 4 && KG == 1)
     if (p.registers)
-      dq = a.Lq <= 128 ? rel_attention_dq_kernel<T, DP, NW, true, WIDE, 4>
-                       : rel_attention_dq_kernel<T, DP, NW, true, WIDE, 8>;
+      dq = a.Lq <= 128 ? rel_attention_dq_kernel<T, DP, NW, 1, true, WIDE, 4>
+                       : rel_attention_dq_kernel<T, DP, NW, 1, true, WIDE, 8>;
   if (const int e = launch_lds(dq, lds)) return e;
-  dq<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, g, qt, p.chunks);
+  dq<<<static_cast<unsigned>(wgs), NW * 64 * KG, lds, s>>>(a, g, qt, p.chunks);
   FA_LAUNCH_CHECK();
   return FA_OK;
 }
 
-template <typename T, int DP, int NW, bool WIDE>
+template <typename T, int DP, int NW, int KG, bool WIDE>
 int launch_dkv(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
   const int kt = tiles_of(a.Lk, NW);
   const int64_t wgs = static_cast<int64_t>(a.B) * a.Hk * kt * p.splits;
   if (wgs > 0x7fffffff) return FA_E_SHAPE;
-  const size_t np = a.pos.n + 2 * PAD, tiles = 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
-  const size_t lds = tiles + ((np + 3) / 4 * 4 + 4 * Shape<T, DP>::BN) * sizeof(float) +
+  const size_t np = a.pos.n + 2 * PAD, tiles = KG * 2 * Shape<T, DP>::BUFS * Shape<T, DP>::TILE;
+  const size_t lds = tiles + ((np + 3) / 4 * 4 + KG * 4 * Shape<T, DP>::BN) * sizeof(float) +
                      (a.pos.grid_w ? codes_room(a.Lq) * sizeof(int) : 0);
-  auto dkv = rel_attention_dkv_kernel<T, DP, NW, WIDE>;
+  auto dkv = rel_attention_dkv_kernel<T, DP, NW, KG, WIDE>;
   if (const int e = launch_lds(dkv, lds)) return e;
-  dkv<<<static_cast<unsigned>(wgs), NW * 64, lds, s>>>(a, g, kt, p.splits);
+  dkv<<<static_cast<unsigned>(wgs), NW * 64 * KG, lds, s>>>(a, g, kt, p.splits);
   FA_LAUNCH_CHECK();
   return FA_OK;
 }
 
 template <typename T, int DP, bool WIDE>
 int launch_wide(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
-  int e = p.nw_q == 4 ? launch_dq<T, DP, 4, WIDE>(a, g, p, s) : launch_dq<T, DP, 2, WIDE>(a, g, p, s);
-  if (e) return e;
-  e = p.nw_k == 4 ? launch_dkv<T, DP, 4, WIDE>(a, g, p, s) : launch_dkv<T, DP, 2, WIDE>(a, g, p, s);
+  int e;
+  if constexpr (DP <= 64) {
+    if (p.kg_q == 2)
+      e = p.nw_q == 4 ? launch_dq<T, DP, 4, 2, WIDE>(a, g, p, s) : launch_dq<T, DP, 2, 2, WIDE>(a, g, p, s);
+    else
+      e = p.nw_q == 4 ? launch_dq<T, DP, 4, 1, WIDE>(a, g, p, s) : launch_dq<T, DP, 2, 1, WIDE>(a, g, p, s);
+    if (e) return e;
+    if (p.kg_k == 2)
+      e = p.nw_k == 4 ? launch_dkv<T, DP, 4, 2, WIDE>(a, g, p, s) : launch_dkv<T, DP, 2, 2, WIDE>(a, g, p, s);
+    else
+      e = p.nw_k == 4 ? launch_dkv<T, DP, 4, 1, WIDE>(a, g, p, s) : launch_dkv<T, DP, 2, 1, WIDE>(a, g, p, s);
+  } else {
+    e = p.nw_q == 4 ? launch_dq<T, DP, 4, 1, WIDE>(a, g, p, s) : launch_dq<T, DP, 2, 1, WIDE>(a, g, p, s);
+    if (e) return e;
+    e = p.nw_k == 4 ? launch_dkv<T, DP, 4, 1, WIDE>(a, g, p, s) : launch_dkv<T, DP, 2, 1, WIDE>(a, g, p, s);
+  }
   if (e || p.splits == 1) return e;
   const int64_t want = (2 * static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.D + 255) / 256;
   dkv_join_kernel<T><<<static_cast<unsigned>(want < 4096 ? want : 4096), 256, 0, s>>>(a, g, p.splits);

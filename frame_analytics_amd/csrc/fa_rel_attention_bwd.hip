@@ -52,7 +52,7 @@ template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<
 // blocks are far from the wave's queries and are one sum.
 // KG groups of NW waves take every KG-th tile of keys, as in the forward pass.
 template <typename T, int DP, int NW, int KG, bool TABLE, bool WIDE, int KEYS>
-__global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS < 8 ? 2 : 1) void rel_attention_dq_kernel(
+__global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS / KG < 8 ? 2 : 1) void rel_attention_dq_kernel(
     RelAttn a, Grads g, int q_tiles, int chunks) {
   constexpr int NT = NW * 64;
   using M = Mat<T>;
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS < 
   constexpr int BN = Shape<T, DP>::BN, NB = BN / 32, CH = DP / 16, OB = DP / 32;
   constexpr int BUFS = Shape<T, DP>::BUFS;
   extern __shared__ __align__(16) unsigned char smem[];
-  static_assert(KG == 1 || (BUFS == 2 && KEYS == 0), "a second group");
+  static_assert(KG == 1 || BUFS == 2, "a second group");
   const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
   T* kt = reinterpret_cast<T*>(smem) + kg * 2 * BUFS * BN * TL::LD;
   T* vt = kt + BUFS * BN * TL::LD;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS < 
 
   load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, threadIdx.x, NT * KG);
   if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, threadIdx.x, NT * KG);
-  constexpr int TOTALS = KEYS > 0 ? KEYS : 1;
+  constexpr int TOTALS = KEYS > 0 ? KEYS / KG : 1;
   f32x16 total[TOTALS];
 #pragma unroll
   for (int i = 0; i < TOTALS; ++i)
@@ -273,8 +273,8 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS < 
   };
   if constexpr (KEYS > 0) {
 #pragma unroll
-    for (int t = 0; t < KEYS / NB; ++t)
-      if (t < tiles) step(t, total + t * NB);
+    for (int round = 0; round < KEYS / NB / KG; ++round)
+      if (round * KG < tiles) step(round * KG + kg, total + round * NB);
   } else {
     const int rounds = (tiles + KG - 1) / KG;
     for (int round = 0; round < rounds; ++round) step(round * KG + kg, total);
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS < 
   }
   if (TABLE && KEYS > 0) {
     __syncthreads();
-    for (int t = tid; t < NW * np; t += NT) sums[t] = 0.0f;
+    for (int t = threadIdx.x; t < KG * NW * np; t += KG * NT) sums[t] = 0.0f;
     __syncthreads();
     const int at = a.pos.code(qc) - a.pos.lo + PAD;
     for (int turn = 0; turn < 2; ++turn) {  // the halves one after the other, as above
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS < 
         for (int i = 0; i < TOTALS; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int key = 32 * i + 4 * hh + 8 * (r / 4) + r % 4;
+            const int key = (i / NB * KG + kg) * BN + i % NB * 32 + 4 * hh + 8 * (r / 4) + r % 4;
             if (key < a.Lk) unsafeAtomicAdd(mine + at - codes[key], total[i][r]);
           }
       }
@@ -647,7 +647,8 @@ inline Plan plan_of(int B, int H, int Hk, int Lq, int Lk, int D, int grid_w, boo
   p.nw_k = static_cast<int64_t>(B) * Hk * tiles_of(Lk, 4) >= cu_count(device) ? 4 : 2;
   p.kg_q = p.kg_k = 1;
   if (D <= 64) {
-    if (!p.registers && static_cast<int64_t>(B) * H * tiles_of(Lq, p.nw_q) < enough && Lk > 128) p.kg_q = 2;
+    // (windows: half of the sums by pair in each group leaves room for two waves on a SIMD)
+    if (p.registers || (static_cast<int64_t>(B) * H * tiles_of(Lq, p.nw_q) < enough && Lk > 128)) p.kg_q = 2;
     if (static_cast<int64_t>(B) * Hk * tiles_of(Lk, p.nw_k) < enough && Lq > 128) p.kg_k = 2;
   }
   p.chunks = B;
@@ -673,10 +674,10 @@ int launch_dq(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) {
     if (lds > MOST_LDS) return launch_dq<T, DP, NW, 1, WIDE>(a, g, p, s);
   auto dq = g.parts ? rel_attention_dq_kernel<T, DP, NW, KG, true, WIDE, 0>
                     : rel_attention_dq_kernel<T, DP, NW, KG, false, WIDE, 0>;
-  if constexpr (DP <= 64 && NW == 4 && KG == 1)
+  if constexpr (DP <= 64 && NW == 4)
     if (p.registers)
-      dq = a.Lq <= 128 ? rel_attention_dq_kernel<T, DP, NW, 1, true, WIDE, 4>
-                       : rel_attention_dq_kernel<T, DP, NW, 1, true, WIDE, 8>;
+      dq = a.Lq <= 128 ? rel_attention_dq_kernel<T, DP, NW, KG, true, WIDE, 4>
+                       : rel_attention_dq_kernel<T, DP, NW, KG, true, WIDE, 8>;
   if (const int e = launch_lds(dq, lds)) return e;
   dq<<<static_cast<unsigned>(wgs), NW * 64 * KG, lds, s>>>(a, g, qt, p.chunks);
   FA_LAUNCH_CHECK();

@@ -206,20 +206,25 @@ __global__ __launch_bounds__(NT * KG) void ortho_product_kernel(Bufs w, Step st,
     ap[s] = A[s] + abase + static_cast<int64_t>(ti) * TM * K;
     bp[s] = B[s] + bbase + static_cast<int64_t>(tj) * TM * K;
   }
-  TileLoad<f16, BK, TM, NT, true> al[PARTS], bl[PARTS];
-  auto load = [&](int piece) {  // past the end: zeros
+  // 128-wide tiles have two pieces of k on their way at a time (2 x 4096^2 4.44 -> 4.32 ms);
+  // 64-wide ones, more of which share a compute unit, one (two: 139 -> 153 us, 6 x 180^2)
+  constexpr bool TWO = TM == 128;
+  TileLoad<f16, BK, TM, NT, true> al[2][PARTS], bl[2][PARTS];
+  auto load = [&](auto stage, int piece) {  // past the end: zeros
+    constexpr int S = decltype(stage)::value;
     const int rows = piece * BK < K ? TM : 0, k = rows ? piece * BK : 0;
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) {
-      al[s].load(ap[s] + k, K, rows, BK, 8, tid);
-      bl[s].load(bp[s] + k, K, rows, BK, 8, tid);
+      al[S][s].load(ap[s] + k, K, rows, BK, 8, tid);
+      bl[S][s].load(bp[s] + k, K, rows, BK, 8, tid);
     }
   };
-  auto store = [&](int buf) {
+  auto store = [&](auto stage, int buf) {
+    constexpr int S = decltype(stage)::value;
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) {
-      al[s].store(lds + ((buf * 2 + 0) * PARTS + s) * PIECE, tid);
-      bl[s].store(lds + ((buf * 2 + 1) * PARTS + s) * PIECE, tid);
+      al[S][s].store(lds + ((buf * 2 + 0) * PARTS + s) * PIECE, tid);
+      bl[S][s].store(lds + ((buf * 2 + 1) * PARTS + s) * PIECE, tid);
     }
   };
   const int wi = (wave >> 1) * WT, wj = (wave & 1) * WT;
@@ -231,11 +236,15 @@ __global__ __launch_bounds__(NT * KG) void ortho_product_kernel(Bufs w, Step st,
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
   const int rounds = (K / BK + KG - 1) / KG;
-  load(kg);
-  store(0);
-  for (int k = 0; k < rounds; ++k) {
+  typedef std::integral_constant<int, 0> Even;
+  typedef std::integral_constant<int, 1> Odd;
+  load(Even(), kg);
+  if (TWO) load(Odd(), KG + kg);
+  store(Even(), 0);
+  auto round = [&](int k, auto stage, auto other) {
     __syncthreads();
-    if (k + 1 < rounds) load((k + 1) * KG + kg);
+    if (TWO) load(stage, (k + 2) * KG + kg);
+    else if (k + 1 < rounds) load(other, (k + 1) * KG + kg);
     const f16* la = lds + ((k % BUFS) * 2 + 0) * PARTS * PIECE;
     const f16* lb = lds + ((k % BUFS) * 2 + 1) * PARTS * PIECE;
 #pragma unroll
@@ -261,8 +270,12 @@ __global__ __launch_bounds__(NT * KG) void ortho_product_kernel(Bufs w, Step st,
     }
     if (k + 1 < rounds) {
       if (BUFS == 1) __syncthreads();
-      store((k + 1) % BUFS);
+      store(other, (k + 1) % BUFS);
     }
+  };
+  for (int k = 0; k < rounds; k += 2) {
+    round(k, Even(), Odd());
+    if (k + 1 < rounds) round(k + 1, Odd(), Even());
   }
   if constexpr (KG > 1) {
     // group g finishes the registers r with (r / 4) % KG = g
@@ -377,8 +390,9 @@ inline int plan(int dtype, int batch, int rows, int cols, Plan* p) {
   // up to 64 rows a product is a launch's time whatever its precision, and little
   // averages the noise of single float16
   p->parts = dtype == FA_BF16 && p->m > 64 ? 1 : 2;
-  // 128 x 128 tiles where they make two workgroups for every compute unit of the card
-  // (its 256 are assumed here: the workspace's size depends on the tile)
+  // rows and columns are padded to the tile: 128 where such tiles of X make two workgroups
+  // for every compute unit (the card's 256: the workspace's size depends on it; 288 of 128 took
+  // 31 us where 1152 of 64 took 27)
   const int64_t tiles = static_cast<int64_t>(batch) * ((p->m + 127) / 128) * ((p->n + 127) / 128);
   p->tile = tiles >= 512 ? 128 : 64;
   p->mp = (p->m + p->tile - 1) / p->tile * p->tile;
@@ -418,11 +432,17 @@ int launch_tiles(const Bufs& w, const Step& st, int64_t wgs, T* out, hipStream_t
 }
 
 template <bool PAIR, int MODE, typename T>
-int launch_product(const Bufs& w, const Step& st, int tile, int batch, int device, T* out, hipStream_t s) {
-  const int64_t per = MODE == STEP ? static_cast<int64_t>(st.tiles_i) * st.tiles_j
-                                   : static_cast<int64_t>(st.tiles_i) * (st.tiles_i + 1) / 2;
-  const int64_t wgs = per * batch;
-  if (wgs > 0x7fffffff) return FA_E_SHAPE;
+int launch_product(const Bufs& w, Step st, int tile, int batch, int device, T* out, hipStream_t s) {
+  // of the padded size's tiles, unless they leave compute units without a workgroup
+  auto count = [&](int t) {
+    const int64_t ti = st.mp / t, tj = st.np / t;
+    return batch * (MODE == STEP ? ti * tj : ti * (ti + 1) / 2);
+  };
+  int64_t wgs = count(tile);
+  if (wgs > 0x7fffffff / 4) return FA_E_SHAPE;
+  if (tile == 128 && wgs < cu_count(device)) tile = 64, wgs = count(64);
+  st.tiles_i = st.mp / tile;
+  st.tiles_j = st.np / tile;
   if (tile == 128) return launch_tiles<128, 1, PAIR, MODE, T>(w, st, wgs, out, s);
   // few workgroups: k is split between four groups of waves
   if (wgs < cu_count(device)) return launch_tiles<64, 4, PAIR, MODE, T>(w, st, wgs, out, s);
@@ -461,8 +481,6 @@ int orthogonalize(const void* g, int batch, int rows, int cols, int steps, const
   st.np = p.np;
   st.poly = poly;
   st.tall = rows > cols;
-  st.tiles_i = p.mp / p.tile;
-  st.tiles_j = p.np / p.tile;
   set(w.xt_out, p.off_xt1, xs);
   T* o = static_cast<T*>(out);
   for (int k = 0; k < steps; ++k) {

@@ -422,3 +422,15 @@ def test_orthogonalize_tiny_and_low_rank(gpu):
     for scale in (1e-4, 1e20):  # eps counts in the first
         x = g * scale
         near(fa.orthogonalize(x.cuda()), ref.orthogonalize(x.double().numpy(), 5, STEEP), 3e-4)
+
+
+def test_example_trains(gpu):
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "train_restorer.py"
+    spec = importlib.util.spec_from_file_location("train_restorer", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    losses = module.main(["--steps", "8", "--size", "64", "--batch", "2", "--device", "cuda"])
+    assert losses[-1] < losses[0]

@@ -251,3 +251,14 @@ def test_arguments_are_checked_before_any_gpu_work(lib):
     assert ort(p, 3, 1, 8, 8, 1, 1.0, 1.0, 1.0, 0.0, p, p, 1 << 40, 0, None) == 5   # no eps
     assert ort(p, 3, 1, 8, 8, 1, 1.0, 1.0, 1.0, 1e-7, p, p, 16, 0, None) == 5       # workspace
     assert ort(p, 0, 1, 8, 8, 1, 1.0, 1.0, 1.0, 1e-7, p, p, 1 << 40, 0, None) == 1  # uint8
+
+
+def test_example_trains():
+    import importlib.util
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "train_restorer.py"
+    spec = importlib.util.spec_from_file_location("train_restorer", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    losses = module.main(["--steps", "5", "--size", "32", "--batch", "2", "--device", "cpu"])
+    assert losses[-1] < losses[0]

@@ -134,7 +134,11 @@ def rel_attention(q, k, v, table, plan: AttentionPlan, need_lse: bool):
     b, h, lq, d = q.shape
     hk, lk = k.shape[1], k.shape[2]
     out = _like(q)
-    lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if need_lse else None
+    lse = None
+    if need_lse:  # the rows' log-sums, and on a line what the rounding of a 16-bit output left
+        n = b * h * lq
+        n = n if q.dtype == torch.float32 or plan.positions.grid_w else (n + 3) // 4 * 4 + (n * d + 1) // 2
+        lse = torch.empty(n, dtype=torch.float32, device=q.device)
     dev, stream = _site(q)
     ws, n = _workspace("fa_gpu_rel_attention_workspace", q.device, b, h, hk, lq, lk, d,
                        plan.positions.slots, dev)

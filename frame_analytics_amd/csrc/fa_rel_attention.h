@@ -74,6 +74,18 @@ __device__ inline void load_codes(int* codes, const RelPos& pos, int n, int tid,
   for (int t = tid; t < codes_room(n); t += nt) codes[t] = pos.code(min(t, n - 1));
 }
 
+// What the output's rounding left, kept behind the log-sums for 16-bit types on a line:
+// D_i = dout_i . out_i is subtracted from every dP of a row, and a row's far keys share one
+// entry of the table, which takes D_i's error as many times.  Measured on a causal line of
+// 2048 in bfloat16, three inputs: the largest relative error of a gradient 2.5e-3 without
+// it and 2.4e-3 with, the largest difference from plain float32 0.084 .. 0.11 and 0.053 ..
+// 0.068, 169 .. 172 us and 169 .. 171.  In a window an entry takes one pair of a row: 16 x
+// 16 windows had 3.0e-4 with it and without, and 740 us without against 776 with, so that
+// they keep none.
+template <typename T> __device__ inline T* low_of(const float* lse, int64_t rows) {
+  return reinterpret_cast<T*>(const_cast<float*>(lse) + (rows + 3) / 4 * 4);
+}
+
 // How the pairs of a 32 x 32 block stand to the bias table.
 enum : int { NEAR = 0, ALL_BELOW = 1, ALL_ABOVE = 2 };
 __device__ inline int block_kind(const RelPos& pos, int dmin, int dmax) {

@@ -227,6 +227,13 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = o[i][4 * g + e] * inv;
         store4<T>(orow, 32 * i + 8 * g + 4 * hh, a.D, ovec, w);
+        if (sizeof(T) == 2 && lse && a.pos.grid_w == 0) {
+          const int64_t all = static_cast<int64_t>(a.B) * a.H * a.Lq;
+          T* low = low_of<T>(lse, all) + ((static_cast<int64_t>(b) * a.H + h) * a.Lq + q) * a.D;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] -= widen(T(w[e]));
+          store4<T>(low, 32 * i + 8 * g + 4 * hh, a.D, a.D % 4 == 0 ? 8 : 1, w);
+        }
       }
     if (lse && hh == 0)
       lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + q] = l == 0.0f ? INF : m + __builtin_log2f(l);

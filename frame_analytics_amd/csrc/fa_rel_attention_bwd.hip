@@ -115,6 +115,13 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS / 
     load_row<T, WIDE>(of, rows(g.out, g.os), q - f, 8 * hh, a.D, a.vec, on);
 #pragma unroll
     for (int i = 0; i < CH; ++i) dd = M::mma(of[i], gf[i], dd);
+    if (sizeof(T) == 2 && KEYS == 0 && a.pos.grid_w == 0) {  // and what the output's rounding left
+      const T* low = low_of<T>(g.lse, static_cast<int64_t>(a.B) * a.H * a.Lq);
+      load_row<T, WIDE>(of, Rows<T>(low + ((static_cast<int64_t>(b) * a.H + h) * a.Lq + f) * a.D, a.D), q - f,
+                        8 * hh, a.D, a.vec, on);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) dd = M::mma(of[i], gf[i], dd);
+    }
   }
   float dsum = 0.0f;
 #pragma unroll

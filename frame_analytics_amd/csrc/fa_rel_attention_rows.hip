@@ -302,7 +302,11 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
       }
     } else {
       const int hr = hk * group + row / a.Lq, ir = row % a.Lq;
-      out[b * os.b + hr * os.h + ir * os.t + d] = T(total == 0.0f ? 0.0f : sum / total);
+      const float x = total == 0.0f ? 0.0f : sum / total;
+      out[b * os.b + hr * os.h + ir * os.t + d] = T(x);
+      if (sizeof(T) == 2 && lse)
+        low_of<T>(lse, static_cast<int64_t>(a.B) * a.H * a.Lq)[((static_cast<int64_t>(b) * a.H + hr) * a.Lq + ir) *
+                                                                   a.D + d] = T(x - widen(T(x)));
       if (lse && d == 0)
         lse[(static_cast<int64_t>(b) * a.H + hr) * a.Lq + ir] =
             total == 0.0f ? INF : top + __builtin_log2f(total);
@@ -357,8 +361,16 @@ __global__ __launch_bounds__(64) void rows_join_kernel(const float* part_o, cons
   total = wave_sum(total);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   T* o = out + b * os.b + h * os.h + i * os.t;
-  if (d0 < D) o[d0] = T(x0 * inv);
-  if (d1 < D) o[d1] = T(x1 * inv);
+  x0 *= inv;
+  x1 *= inv;
+  if (d0 < D) o[d0] = T(x0);
+  if (d1 < D) o[d1] = T(x1);
+  if (sizeof(T) == 2 && lse) {
+    const int64_t all = static_cast<int64_t>(gridDim.x / rows / Hk) * H * Lq;  // batch x heads x queries
+    T* low = low_of<T>(lse, all) + ((static_cast<int64_t>(b) * H + h) * Lq + i) * D;
+    if (d0 < D) low[d0] = T(x0 - widen(T(x0)));
+    if (d1 < D) low[d1] = T(x1 - widen(T(x1)));
+  }
   if (lse && threadIdx.x == 0)
     lse[(static_cast<int64_t>(b) * H + h) * Lq + i] = total == 0.0f ? INF : top + __builtin_log2f(total);
 }

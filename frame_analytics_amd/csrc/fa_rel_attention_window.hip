@@ -45,9 +45,10 @@ __device__ inline uint32_t reachable(const RelAttn& a, const Pairs& p, int len) 
 }
 
 // ... and by the mask.  Its bytes are 0 or 1.  Where its rows are 64 aligned bytes a lane
-// reads half of its query's row, 32 bytes in two reads (four bytes at a time, the bits
-// that it needs, cost 65 us of 208 in 24576 windows: each read touches 32 rows), and the
-// halves of the wave exchange every other word.  The words of the next window are read
+// reads half of its query's row, 32 bytes in two reads, and the halves of the wave exchange
+// every other word: four bytes at a time, the bits that it needs, each read touches 32
+// rows (24576 windows forward and backward 687 us so, and with scratch in the loops; 634 us
+// without both).  The words of the next window are read
 // with its tiles: memory answers in order, and a read made later would wait for them.
 struct MaskWords {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

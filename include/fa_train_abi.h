@@ -57,8 +57,10 @@ FA_API int fa_gpu_rel_bias_backward(const void* up, const int64_t* up_strides, i
  * of q, k, v and out; the last dimension has stride 1.  1 <= D <= 128.
  * start: q_starts[b] (int32, device) or, where that is null, q_start; both are taken
  * as within +-2^30.  mask_strides: {batch, head, query, key} in bytes.
- * lse: [B, H, Lq] float32 or null; log2 of each row's sum of exponentials, +inf for
- * a row that sees nothing (what the backward pass reads).
+ * lse: null, or what the backward pass reads: [B, H, Lq] float32, log2 of each row's
+ * sum of exponentials, +inf for a row that sees nothing; for FA_F16 and FA_BF16 with
+ * grid_w 0, from the next multiple of 16 bytes on, [B, H, Lq, D] of dtype: what the
+ * rounding of out left.
  * workspace: fa_gpu_rel_attention_workspace bytes, 16-byte aligned (0: may be null).
  */
 FA_API int fa_gpu_rel_attention_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int n,

@@ -261,12 +261,15 @@ def _buckets(case, q_pos, k_len):
 
 
 def _plain_bias(case, table, q_pos):
-    """(1 or batch, heads, q_len, k_len) from the float32 table."""
+    """(1 or batch, heads, q_len, k_len) from the float32 table.  ``q_pos``: the queries'
+    positions, (1 or batch, q_len); None: 0, 1, 2 and so on for all."""
     lq, lk = case["q_len"], case["k_len"]
-    if case["grid_w"] or q_pos.shape[0] > 1:
+    if case["grid_w"] or q_pos is not None:
+        q_pos = torch.arange(lq, device=table.device)[None] if q_pos is None else q_pos
         return table[_buckets(case, q_pos, lk)].permute(0, 3, 1, 2)
-    # a line: one value for each distance, j - i from 1 - lq to lk - 1, picked from the
-    # table by a product; laid out again and again, one element further in each row
+    # a line from position 0 on: one value for each distance, j - i from 1 - lq to lk - 1,
+    # picked from the table by a product; laid out again and again, one element further in
+    # each row
     wide = lq + lk - 1
     row = _buckets(case, torch.full((1,), lq - 1, device=table.device), wide)[0]
     pick = (row[:, None] == torch.arange(table.shape[0], device=table.device)).float()
@@ -285,7 +288,8 @@ def _plain_attention(state):
         k, v = (x.repeat_interleave(group, dim=1) for x in (k, v))
     start = torch.as_tensor(state["start"], device=dev).reshape(-1, 1)
     q_pos = start + torch.arange(lq, device=dev)  # (1 or batch, q_len)
-    s = (q @ k.transpose(-1, -2)) / math.sqrt(case["dim"]) + _plain_bias(case, table, q_pos)
+    s = (q @ k.transpose(-1, -2)) / math.sqrt(case["dim"]) + _plain_bias(
+        case, table, q_pos if torch.is_tensor(state["start"]) else None)
     keys = torch.arange(lk, device=dev)
     hidden = None
     if case["causal"]:
@@ -337,8 +341,7 @@ def run(state):
         if own:
             bias = fa.relative_bias(table, _positions(fa, case), case["q_len"], case["k_len"])
         else:
-            q_pos = torch.arange(case["q_len"], device=table.device)[None]
-            bias = _plain_bias(case, table.float(), q_pos)[0].to(table.dtype)
+            bias = _plain_bias(case, table.float(), None)[0].to(table.dtype)
         bias.backward(state["up"])
         return bias.detach(), table.grad
     q, k, v, table = (state[x] for x in ("q", "k", "v", "table"))

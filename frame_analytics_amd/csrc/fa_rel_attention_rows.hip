@@ -335,10 +335,10 @@ __global__ __launch_bounds__(64) void rows_join_kernel(const float* part_o, cons
     if (s0 + lane < splits) {
       const int64_t at = first + static_cast<int64_t>(s0 + lane) * rows;
       const float ms = part_ml[2 * at];
-      if (ms != -INF) {
-        f = __builtin_amdgcn_exp2f(ms - top);
-        total += f * part_ml[2 * at + 1];
-      }
+      // a split without a maximum saw no key, and its sum is 0, or NaN scores alone, which
+      // no maximum takes, and its sum is NaN: the row's has to be
+      f = ms != -INF ? __builtin_amdgcn_exp2f(ms - top) : 0.0f;
+      total += ms != -INF ? f * part_ml[2 * at + 1] : part_ml[2 * at + 1];
     }
     const int here = min(64, splits - s0);
     for (int s1 = 0; s1 < here; s1 += 8) {

@@ -1,0 +1,61 @@
+"""The training operators' kernels where their inputs are extreme: NaN, biases of the
+type's limits, wide strides, many matrices, coefficients that overflow.  Tolerances as in
+``test_gpu_training_ops``; what a test adds to them is derived in it."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import frame_analytics_amd as fa
+from oracle import training as ref
+from tests.test_gpu_training_ops import DT, attention_case, normal, run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------------------- #
+# NaN
+# --------------------------------------------------------------------------- #
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("lq,lk", [(1, 100), (1, 2500), (3, 700)])
+def test_a_nan_query_answers_nan(gpu, dt, lq, lk):
+    """Few queries against a cache, dealt out or not: the row of a NaN query, and it
+    alone, is NaN, and so are its gradients."""
+    b, h, hk, d = 2, 4, 2, 64
+    pos = fa.LinePositions(32, 128, bidirectional=False)
+    rows = ref.line_rows(lq, lk, lk - lq, 32, 128, False)
+    tensors, g, _ = attention_case(DT[dt], b, h, hk, lq, lk, d, pos, rows, q_start=lk - lq)
+    clean = run_attention(tensors, g, pos, q_start=lk - lq)
+    tensors[0][1, 2, 0, 5] = float("nan")
+    got = run_attention(tensors, g, pos, q_start=lk - lq)
+    with torch.no_grad():
+        only = fa.relative_attention(*(t.cuda() for t in tensors), pos, q_start=lk - lq)
+    bad = torch.zeros(b, h, lq, dtype=torch.bool, device="cuda")
+    bad[1, 2, 0] = True
+    for out in (got[0], only, got[1]):
+        assert torch.isnan(out[bad]).all() and not torch.isnan(out[~bad]).any()
+    assert torch.equal(got[0][~bad], clean[0][~bad]) and torch.equal(only[~bad], clean[0][~bad])
+    for x in got[2:4]:  # every key of its key head
+        assert torch.isnan(x[1, 1]).all() and not torch.isnan(x[0]).any()
+        assert not torch.isnan(x[1, 0]).any()
+    assert torch.isnan(got[4][:, 2]).any() and not torch.isnan(got[4][:, [0, 1, 3]]).any()
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("last", [128, 256, 640])
+def test_a_nan_key_that_stands_alone_in_its_run(gpu, dt, last):
+    """Keys are dealt out in runs of whole blocks: the one key past them is NaN."""
+    b, h, hk, lk, d = 2, 4, 2, 1000, 32
+    pos = fa.LinePositions(8, 20)
+    gen = torch.Generator().manual_seed(last)
+    q, k, v = (normal(gen, DT[dt], b, n, m, d).transpose(1, 2).cuda()
+               for n, m in ((1, h), (lk, hk), (lk, hk)))
+    table = normal(gen, DT[dt], 8, h).cuda()
+    lens = torch.tensor([last + 1, last], dtype=torch.int32, device="cuda")
+    k[:, 1, last] = float("nan")
+    out = fa.relative_attention(q, k, v, table, pos, key_lengths=lens)
+    assert torch.isnan(out[0, 2:]).all()                       # the heads of key head 1
+    assert not torch.isnan(out[0, :2]).any() and not torch.isnan(out[1]).any()

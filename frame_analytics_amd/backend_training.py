@@ -27,12 +27,22 @@ def serves(t: torch.Tensor) -> bool:
     return t.dtype in DTYPES and backend._gpu_ext(t) is not None
 
 
-@functools.lru_cache(maxsize=64)
+_row_tables: dict = {}
+
+
 def _row_of(positions, device: torch.device) -> torch.Tensor:
     """The table row of each slot, on the device: one per description of positions
     (a value, not a tensor), so made once.  Making it copies from the host: a graph
-    capture needs an eager call before it."""
-    return torch.tensor(positions.row_of(), dtype=torch.int32, device=device)
+    capture needs an eager call before it.
+
+    It is kept for the life of the process (17 KB at most): a captured graph holds its
+    address and no reference, and launches on other streams may still read it, so memory
+    given back would be read as rows of the table by a replay."""
+    rows = _row_tables.get((positions, device))
+    if rows is None:  # (of two threads that make it, both take the first's)
+        rows = _row_tables.setdefault(
+            (positions, device), torch.tensor(positions.row_of(), dtype=torch.int32, device=device))
+    return rows
 
 
 @functools.lru_cache(maxsize=256)

@@ -14,13 +14,14 @@ then linked.  ``FA_HIP_ARCHS`` overrides the target list (default ``gfx950``).
 from __future__ import annotations
 
 import concurrent.futures as _cf
+import contextlib
 import os
 import shutil
 import subprocess
 import sys
 import sysconfig
 from pathlib import Path
-from typing import List, Sequence
+from typing import Iterator, List, Sequence
 
 PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
@@ -117,6 +118,18 @@ def _run(cmd: Sequence[str], verbose: bool) -> None:
         raise RuntimeError(f"command failed ({res.returncode}): {' '.join(cmd)}\n{out}")
 
 
+@contextlib.contextmanager
+def _published(out: Path) -> Iterator[Path]:
+    """A path to write ``out`` to: it becomes ``out`` at once where the body succeeds (a
+    concurrent loader never sees half a file), and is removed where it fails."""
+    tmp = out.with_name(f".{out.name}.{os.getpid()}.tmp")
+    try:
+        yield tmp
+        os.replace(tmp, out)
+    finally:
+        tmp.unlink(missing_ok=True)
+
+
 def build_cpu(verbose: bool = False) -> Path:
     """Compile the host kernels into ``libfa_cpu.so``; returns its path.
 
@@ -126,12 +139,10 @@ def build_cpu(verbose: bool = False) -> Path:
     """
     LIBDIR.mkdir(exist_ok=True)
     out = cpu_library_path()
-    tmp = out.with_name(f".{out.name}.{os.getpid()}.tmp")
-    cmd = [cxx(), "-O3", "-std=c++17", "-fPIC", "-shared", "-pthread", "-mavx2", "-mfma",
-           "-fvisibility=hidden", "-fno-math-errno", f"-I{INCLUDE}",
-           *map(str, cpu_sources()), "-o", str(tmp)]
-    _run(cmd, verbose)
-    os.replace(tmp, out)
+    with _published(out) as tmp:
+        _run([cxx(), "-O3", "-std=c++17", "-fPIC", "-shared", "-pthread", "-mavx2", "-mfma",
+              "-fvisibility=hidden", "-fno-math-errno", f"-I{INCLUDE}",
+              *map(str, cpu_sources()), "-o", str(tmp)], verbose)
     return out
 
 
@@ -140,11 +151,10 @@ def build_call(verbose: bool = False) -> Path:
     nothing of its own); returns its path."""
     LIBDIR.mkdir(exist_ok=True)
     out = call_module_path()
-    tmp = out.with_name(f".{out.name}.{os.getpid()}.tmp")
-    _run([cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{INCLUDE}",
-          f"-I{python_include()}", *map(str, call_sources()), "-o", str(tmp)],
-         verbose)
-    os.replace(tmp, out)
+    with _published(out) as tmp:
+        _run([cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+              f"-I{INCLUDE}", f"-I{python_include()}", *map(str, call_sources()),
+              "-o", str(tmp)], verbose)
     return out
 
 
@@ -178,22 +188,17 @@ def build(verbose: bool = False, jobs: int = 0) -> Path:
         obj = objdir / (src.stem + ".o")
         objs.append(obj)
         cmds.append([cc, *flags, "-c", str(src), "-o", str(obj)])
-    # bench.py's read-bandwidth ceiling kernel, a library of its own
-    rb = readbw_library_path()
-    rb_tmp = rb.with_name(f".{rb.name}.{os.getpid()}.tmp")
-    cmds.append([cc, *flags, "-shared", *map(str, sorted((CSRC / "bench").glob("*.hip"))),
-                 "-o", str(rb_tmp)])
-    n = jobs or min(len(cmds), max(1, os.cpu_count() or 1))
-    with _cf.ThreadPoolExecutor(max_workers=n) as pool:
-        for f in [pool.submit(_run, c, verbose) for c in cmds]:
-            f.result()
     out = library_path()
-    tmp = out.with_name(f".{out.name}.{os.getpid()}.tmp")
-    link = [cc, *[f"--offload-arch={a}" for a in archs()], "-shared", "-fPIC",
-            *map(str, objs), "-o", str(tmp)]
-    _run(link, verbose)
-    os.replace(tmp, out)  # atomic: a concurrent loader never sees half a file
-    os.replace(rb_tmp, rb)
+    with _published(readbw_library_path()) as rb_tmp, _published(out) as tmp:
+        # bench.py's read-bandwidth ceiling kernel, a library of its own
+        cmds.append([cc, *flags, "-shared", *map(str, sorted((CSRC / "bench").glob("*.hip"))),
+                     "-o", str(rb_tmp)])
+        n = jobs or min(len(cmds), max(1, os.cpu_count() or 1))
+        with _cf.ThreadPoolExecutor(max_workers=n) as pool:
+            for f in [pool.submit(_run, c, verbose) for c in cmds]:
+                f.result()
+        _run([cc, *[f"--offload-arch={a}" for a in archs()], "-shared", "-fPIC",
+              *map(str, objs), "-o", str(tmp)], verbose)
     try_build_call(verbose)
     return out
 

@@ -3,8 +3,10 @@
 //
 // All the work is matrix products, on the matrix cores in float16 with float32
 // accumulators.  Matrices are held times a power of two (X and A 2^11, the polynomial
-// 2^10) so that float16's range serves them: singular values stay near or below one,
-// so entries do.  Two precisions:
+// 2^10) so that float16's range serves them: an entry is at most the largest singular
+// value, for which the default coefficients keep 1.2 (1.4 of A, 2.8 of the polynomial).
+// Coefficients for which X, A or the polynomial would pass 65504, or fade into float16's
+// smallest, are refused (fits).  Two precisions:
 //
 //   single (bfloat16 input of more than 64 rows): one float16 per entry.  Rounding X to 11 bits is noise
 //     in every direction, and a step multiplies a small singular direction by a, so X
@@ -379,6 +381,39 @@ struct Plan {
   int64_t off_x, off_xt0, off_xt1, off_a, off_p, off_xf, off_f, off_sums, bytes;
 };
 
+// Whether float16 holds every iterate of these coefficients.  A step takes each singular
+// value s of X to p(s) = a s + b s^3 + c s^5 by itself, from (0, 1] on, so the largest
+// that any input can have after k steps is the largest |p| over the range before: at its
+// end, or where p' = a + 3 b s^2 + 5 c s^4 is zero.  The polynomial's eigenvalues are
+// b s^2 + c s^4.  Each range is widened by what rounding may add.
+inline bool fits(double a, double b, double c, int steps) {
+  constexpr double MOST = 65504.0 * 0.99, NOISE = 1.0 + 1.0 / 512, LEAST = 1.0 / 64;
+  double top = NOISE, before = 0.0;
+  for (int k = 0; k < steps; ++k) {
+    const double t = top * top;
+    // (the negated form refuses NaN)
+    if (!(top * SX <= MOST && t * SX <= MOST && top >= LEAST)) return false;
+    auto poly = [&](double u) { return fabs(b * u + c * u * u); };  // of u = s^2
+    auto step = [&](double u) { return fabs(sqrt(u) * (a + b * u + c * u * u)); };
+    double most = poly(t), next = step(t);
+    auto at = [&](double u) {
+      if (u > 0.0 && u < t) most = fmax(most, poly(u)), next = fmax(next, step(u));
+    };
+    if (c != 0.0) {
+      at(-b / (2.0 * c));
+      const double disc = 9.0 * b * b - 20.0 * a * c;
+      if (disc >= 0.0) at((-3.0 * b + sqrt(disc)) / (10.0 * c)), at((-3.0 * b - sqrt(disc)) / (10.0 * c));
+    } else if (b != 0.0) {
+      at(-a / (3.0 * b));
+    }
+    if (!(most * SP <= MOST) || !(next < 1e30)) return false;
+    if (next == before) return true;  // so will every further step's
+    before = next;
+    top = next * NOISE;
+  }
+  return true;  // (what the last step leaves is held in float32)
+}
+
 inline int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 inline int plan(int dtype, int batch, int rows, int cols, Plan* p) {
@@ -518,7 +553,7 @@ FA_API int fa_gpu_orthogonalize(const void* g, int dtype, int batch, int rows, i
   if (!g || !out || !workspace) return FA_E_ARG;
   Plan p;
   if (const int e = plan(dtype, batch, rows, cols, &p)) return e;
-  if (steps < 1 || !(eps > 0.0) || workspace_bytes < p.bytes) return FA_E_ARG;
+  if (steps < 1 || !(eps > 0.0) || workspace_bytes < p.bytes || !fits(a, b, c, steps)) return FA_E_ARG;
   DeviceScope scope(device);
   if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
   const Poly poly{static_cast<float>(a), static_cast<float>(b), static_cast<float>(c)};

@@ -413,6 +413,41 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
 # --------------------------------------------------------------------------- #
 
 
+@functools.lru_cache(maxsize=256)
+def _held_in_float16(a: float, b: float, c: float, steps: int) -> bool:
+    """Whether the kernels' float16 operands hold what these coefficients lead to (the
+    entry point refuses the rest).
+
+    A step takes each singular value ``s`` to ``|a s + b s^3 + c s^5|`` by itself, from
+    (0, 1] on, so the largest possible one is the largest value over the range before: at
+    its end or at a zero of the derivative.  X and ``A`` are held times 2048, ``b A + c
+    A^2`` times 1024; a range is widened by 1/512, more than rounding adds.
+    """
+    most, noise = 65504 * 0.99, 1 + 1 / 512
+    top, before = noise, 0.0
+    for _ in range(steps):
+        if not (1 / 64 <= top and 2048 * max(top, top * top) <= most):
+            return False
+        turns = [top * top]  # squares of singular values
+        if c:
+            disc = 9 * b * b - 20 * a * c
+            turns.append(-b / (2 * c))
+            if disc >= 0:
+                turns += [(-3 * b + r) / (10 * c) for r in (math.sqrt(disc), -math.sqrt(disc))]
+        elif b:
+            turns.append(-a / (3 * b))
+        turns = [u for u in turns if 0 < u <= top * top]
+        if not 1024 * max(abs(b * u + c * u * u) for u in turns) <= most:
+            return False
+        after = max(math.sqrt(u) * abs(a + b * u + c * u * u) for u in turns)
+        if not after < 1e30:
+            return False
+        if after == before:  # so will every further step's
+            return True
+        before, top = after, after * noise
+    return True
+
+
 @torch.no_grad()
 def orthogonalize(update: torch.Tensor, *, steps: int = 5,
                   coefficients: Sequence[float] = (3.4445, -4.7750, 2.0315), eps: float = 1e-7,
@@ -425,7 +460,12 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     convolution's weight to ``(out, in * kh * kw)`` first); the result has its shape
     and type and carries no gradient.  The default coefficients lift small singular
     values fast and leave them between 0.7 and 1.2; ``(1.875, -1.25, 0.375)``
-    converges to one.  Coefficients whose iterates leave [0, 16] overflow.
+    converges to one.
+
+    The kernels hold their operands in float16: iterates of singular values within [1/64,
+    5.6] (the largest of each step but the last) with ``|b s^2 + c s^4|`` below 63.
+    Coefficients that leave this run the eager path, in float32 (``backend_hint="native"``
+    refuses them).
 
     bfloat16 runs single float16 products (the result is within 1.5e-3 of exact before
     its rounding), float16 and float32 pairs of float16 (22 bits).
@@ -441,6 +481,12 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     a, b, c = (float(x) for x in coefficients)
     if update.numel() == 0:
         return torch.empty_like(update)
+    if (backend_hint in ("auto", "native") and backend_training.serves(update)
+            and not _held_in_float16(a, b, c, int(steps))):
+        if backend_hint == "native":
+            raise RuntimeError("orthogonalize: the kernels' float16 operands do not hold the "
+                               f"iterates of the coefficients {(a, b, c)} over {steps} steps")
+        backend_hint = "torch"
     if _route(update, "orthogonalize", backend_hint):
         return backend_training.orthogonalize(update, int(steps), (a, b, c), float(eps))
     with _no_autocast(update):

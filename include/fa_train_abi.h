@@ -95,6 +95,9 @@ FA_API int fa_gpu_rel_attention_backward(
  * out = X_steps of X_0 = g / (|g| + eps), X <- a X + (b A + c A^2) X, A = X X^T,
  * for each of `batch` contiguous [rows, cols] matrices (transposed inside where rows
  * > cols); |g| is the Frobenius norm.  g, out: `dtype` (FA_F16, FA_BF16, FA_F32).
+ * FA_E_ARG where float16 would not hold what these coefficients lead to: the largest
+ * singular value that a step may be given, from 1 on, has to stay within 1/64 and 5.6,
+ * and |b s^2 + c s^4| below 63 for all up to it.
  */
 FA_API int fa_gpu_orthogonalize_workspace(int dtype, int batch, int rows, int cols,
                                           int64_t* out_bytes);

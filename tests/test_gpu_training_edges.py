@@ -4,12 +4,13 @@ type's limits, wide strides, many matrices, coefficients that overflow.  Toleran
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
 import frame_analytics_amd as fa
 from oracle import training as ref
-from tests.test_gpu_training_ops import DT, attention_case, normal, run_attention
+from tests.test_gpu_training_ops import DT, UNIT, attention_case, near, normal, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +60,62 @@ def test_a_nan_key_that_stands_alone_in_its_run(gpu, dt, last):
     out = fa.relative_attention(q, k, v, table, pos, key_lengths=lens)
     assert torch.isnan(out[0, 2:]).all()                       # the heads of key head 1
     assert not torch.isnan(out[0, :2]).any() and not torch.isnan(out[1]).any()
+
+
+# --------------------------------------------------------------------------- #
+# biases at the type's limits
+# --------------------------------------------------------------------------- #
+
+
+# --------------------------------------------------------------------------- #
+# views, tangents
+# --------------------------------------------------------------------------- #
+
+
+# --------------------------------------------------------------------------- #
+# updates
+# --------------------------------------------------------------------------- #
+
+
+#: outside what float16 operands hold: an iterate of 8 (its Gram entry), 1036, a polynomial
+#: of 70, an iterate of 34
+OUTSIDE = [((2.0, 0.0, 0.0), 5), ((3.0, 0.0, 1.0), 3), ((0.5, 70.0, 0.0), 1), ((1.0, 0.0, 1.0), 3)]
+#: inside: iterates of 4, 1.75 (8.5 after the last step), a polynomial of 60
+INSIDE = [((2.0, 0.0, 0.0), 3), ((1.0, 0.5, 0.25), 2), ((0.5, 60.0, 0.0), 1)]
+
+
+def growing(dt, m, n):
+    """Singular values from one down."""
+    gen = torch.Generator().manual_seed(5)
+    u, _, w = torch.linalg.svd(torch.randn(m, n, generator=gen), full_matrices=False)
+    return ((u * torch.linspace(1.0, 0.0, m) ** 2) @ w).to(DT[dt])
+
+
+@pytest.mark.portable_ok
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("coefficients,steps", OUTSIDE)
+@pytest.mark.parametrize("m,n", [(1, 1), (70, 90)])
+def test_coefficients_that_grow(gpu, dt, coefficients, steps, m, n):
+    """Served (in float32) where float16 operands would overflow."""
+    g = growing(dt, m, n)
+    want = ref.orthogonalize(g.double().numpy(), steps, coefficients)
+    if np.abs(want).max() > torch.finfo(DT[dt]).max / 2:
+        pytest.skip("the result itself does not fit the type")
+    # a step multiplies a relative error by 5 at most (s p'(s) / p(s) of these sets), three
+    # steps by 125, of 2^-24 sqrt(90) each; and one rounding
+    near(fa.orthogonalize(g.cuda(), steps=steps, coefficients=coefficients), want,
+         UNIT[dt] + 2e-4, (m, n))
+    with pytest.raises(RuntimeError):
+        fa.orthogonalize(g.cuda(), steps=steps, coefficients=coefficients, backend_hint="native")
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("coefficients,steps", INSIDE)
+@pytest.mark.parametrize("m,n", [(1, 1), (70, 90)])
+def test_coefficients_that_just_fit(gpu, dt, coefficients, steps, m, n):
+    g = growing(dt, m, n)
+    want = ref.orthogonalize(g.double().numpy(), steps, coefficients)
+    # before the rounding as the default coefficients, which multiply errors more; a single
+    # value's rounding is half a unit in the last place at most
+    near(fa.orthogonalize(g.cuda(), steps=steps, coefficients=coefficients, backend_hint="native"),
+         want, {"bf16": 1.5e-3 + 2.0 ** -8, "f16": 2.0 ** -11 + 3e-5, "f32": 3e-5}[dt], (m, n))

@@ -2,14 +2,16 @@
 
 from __future__ import annotations
 
+import ctypes
 import fnmatch
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
 
 import frame_analytics_amd as fa
-from frame_analytics_amd import _build, backend_training
+from frame_analytics_amd import _build, _cabi, backend_training, training
 
 
 def test_row_tables_are_never_given_back():
@@ -49,3 +51,45 @@ def test_a_failed_build_leaves_no_file(monkeypatch, tmp_path):
     assert wrote and not list(tmp_path.iterdir())
     for out in wrote:
         assert any(fnmatch.fnmatchcase(out.name, pattern) for pattern in ignored), out.name
+
+
+def test_what_float16_holds_of_an_update():
+    """The largest singular value that coefficients lead to, against a fine grid of them."""
+    held = training._held_in_float16
+    for coefficients, steps in (((3.4445, -4.7750, 2.0315), 5), ((1.875, -1.25, 0.375), 6),
+                                ((3.4445, -4.7750, 2.0315), 10 ** 6), ((2.0, 0.0, 0.0), 3),
+                                ((1.0, 0.5, 0.25), 2), ((0.5, 60.0, 0.0), 1), ((1.5, -0.5, 0.0), 9)):
+        assert held(*coefficients, steps), coefficients
+    nan, inf = float("nan"), float("inf")
+    for coefficients, steps in (((2.0, 0.0, 0.0), 5), ((3.0, 0.0, 1.0), 3), ((0.5, 70.0, 0.0), 1),
+                                ((1.0, 0.0, 1.0), 3), ((0.1, 0.0, 0.0), 5), ((nan, 0.0, 0.0), 1),
+                                ((1.0, inf, 0.0), 1), ((1.0, 0.0, nan), 2), ((1e300, 1e300, 1e300), 4)):
+        assert not held(*coefficients, steps), coefficients
+    rng = np.random.default_rng(0)
+    verdicts = []
+    for _ in range(300):
+        a, b, c = rng.normal(size=3) * (3.0, 5.0, 3.0)
+        s, fits, margin = np.linspace(0.0, 1.0, 20001), True, 1.0
+        for _ in range(3):
+            top = np.abs(s).max()
+            worst = max(2048 * top, 2048 * top ** 2, 1024 * np.abs(b * s ** 2 + c * s ** 4).max())
+            fits &= worst <= 65504 and top >= 1 / 64
+            margin = min(margin, abs(np.log(worst / 65504)), abs(np.log(top * 64)))
+            s = a * s + b * s ** 3 + c * s ** 5
+            if not fits:
+                break
+        if margin > 0.2:  # farther from the limit than the widening
+            verdicts.append(fits)
+            assert held(a, b, c, 3) == fits, (a, b, c)
+    assert 20 < sum(verdicts) < len(verdicts) - 20
+
+
+def test_the_entry_point_refuses_what_float16_does_not_hold():
+    if not _build.library_path().exists():
+        _build.build()
+    lib = _cabi.bind(ctypes.CDLL(str(_build.library_path())), _cabi.TRAIN_SIGNATURES)
+    p = ctypes.addressof(ctypes.create_string_buffer(4096))
+    nan = float("nan")
+    for a, b, c, steps in ((2.0, 0.0, 0.0, 5), (3.0, 0.0, 1.0, 3), (0.5, 70.0, 0.0, 1),
+                           (1.0, 0.0, 1.0, 3), (0.1, 0.0, 0.0, 5), (nan, 0.0, 0.0, 1), (1.0, nan, 0.0, 1)):
+        assert lib.fa_gpu_orthogonalize(p, 3, 1, 8, 8, steps, a, b, c, 1e-7, p, p, 1 << 40, 0, None) == 5

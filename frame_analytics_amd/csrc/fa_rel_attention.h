@@ -134,9 +134,10 @@ __device__ inline void hide(f32x16& s, uint32_t seen) {
 // acc += V^T P^T over 16 keys of which some are hidden from some queries: a value
 // that is not finite must not reach the queries that do not see it (0 x inf).  The
 // finite values go through the product; the others are counted by two more, with 1 in
-// the place of each value and of each visible pair.
+// the place of each value and of each visible pair (bit i of `seen`: a weight may be
+// rounded to zero and its pair count all the same).
 template <typename T>
-__device__ inline f32x16 guarded(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x16 acc) {
+__device__ inline f32x16 guarded(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x16 acc, uint32_t seen) {
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(widen(v[i])) < INF);
@@ -147,17 +148,17 @@ __device__ inline f32x16 guarded(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f
   acc = Mat<T>::mma(fine, p, acc);
 #pragma unroll 1
   for (float way = INF; way != 0.0f; way = way > 0.0f ? -INF : 0.0f) {
-    typename Mat<T>::V8 bad_v, seen;
+    typename Mat<T>::V8 bad_v, ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = widen(v[i]);
       bad_v[i] = x == way || x != x ? T(1) : T(0);  // NaN counts both ways
-      seen[i] = widen(p[i]) == 0.0f ? T(0) : T(1);
+      ones[i] = seen >> i & 1 ? T(1) : T(0);
     }
     f32x16 n;
 #pragma unroll
     for (int r = 0; r < 16; ++r) n[r] = 0.0f;
-    n = Mat<T>::mma(bad_v, seen, n);
+    n = Mat<T>::mma(bad_v, ones, n);
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] += n[r] > 0.0f ? way : 0.0f;
   }

@@ -86,6 +86,7 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
     const T* vv = vt + (t / KG & 1) * BN * TL::LD;
     f32x16 s[NB];
     bool partial[NB];
+    uint32_t seen[NB];
     float top = -INF;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
       }
       if (MODE == ANY) {
         partial[nb] = mask || k0 + 32 > len || (a.causal && k0 + 31 > s0 + qw);
-        if (partial[nb]) hide(s[nb], seen_keys(a, mask, qc, qpos, k0 + 4 * hh, len));
+        if (partial[nb]) hide(s[nb], seen[nb] = seen_keys(a, mask, qc, qpos, k0 + 4 * hh, len));
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[nb][r]);
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
 #pragma unroll
         for (int i = 0; i < OB; ++i) {
           const typename M::V8 vf = TL::transposed(vv, nb * 32 + 16 * half, 32 * i, lane);
-          o[i] = partial[nb] ? guarded<T>(vf, p, o[i]) : M::mma(vf, p, o[i]);
+          o[i] = partial[nb] ? guarded<T>(vf, p, o[i], seen[nb] >> 8 * half) : M::mma(vf, p, o[i]);
         }
       }
     }

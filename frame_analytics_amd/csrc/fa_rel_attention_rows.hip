@@ -83,7 +83,7 @@ __device__ inline typename Mat<T>::V8 transposed16(const T* t, int col0, int lan
 
 // As guarded<T>, for 16 x 16 blocks.
 template <typename T>
-__device__ inline f32x4 guarded16(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x4 acc) {
+__device__ inline f32x4 guarded16(typename Mat<T>::V8 v, typename Mat<T>::V8 p, f32x4 acc, uint32_t seen) {
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) bad |= !(__builtin_fabsf(widen(v[i])) < INF);
@@ -94,14 +94,14 @@ __device__ inline f32x4 guarded16(typename Mat<T>::V8 v, typename Mat<T>::V8 p, 
   acc = mma16<T>(fine, p, acc);
 #pragma unroll 1
   for (float way = INF; way != 0.0f; way = way > 0.0f ? -INF : 0.0f) {
-    typename Mat<T>::V8 bad_v, seen;
+    typename Mat<T>::V8 bad_v, ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = widen(v[i]);
       bad_v[i] = x == way || x != x ? T(1) : T(0);
-      seen[i] = widen(p[i]) == 0.0f ? T(0) : T(1);
+      ones[i] = seen >> i & 1 ? T(1) : T(0);
     }
-    const f32x4 n = mma16<T>(bad_v, seen, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    const f32x4 n = mma16<T>(bad_v, ones, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[r] += n[r] > 0.0f ? way : 0.0f;
   }
@@ -214,8 +214,10 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
     const int kind = block_kind(a.pos, s0 - (k0 + 31), s0 + a.Lq - 1 - k0);
     const bool partial = a.mask || k0 + 32 > len || (a.causal && k0 + 31 > s0);
     typename M::V8 p[NC];
+    uint32_t visible[NC];  // bit 4 w + r
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
+      visible[n] = 0;
       const float* e = eb + gi[n] * np + (s0 + qi[n] - k0 - 4 * gg - a.pos.lo + PAD);
       const float far = eb[gi[n] * np + (kind == ALL_BELOW ? 0 : np - 1)];
       float top = -INF;
@@ -229,6 +231,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
             bool seen = key < len && (!a.causal || key <= s0 + qi[n]);
             if (a.mask && seen) seen = mask[n][qi[n] * a.mq + key * a.mk] != 0;
             if (!seen) x = -INF;
+            visible[n] |= (seen ? 1u : 0u) << (4 * w + r);
           }
           s[n][w][r] = x;
           top = fmaxf(top, x);
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
       const typename M::V8 vf = transposed16<T, DP>(vt, 16 * i, lane);
 #pragma unroll
       for (int n = 0; n < NC; ++n)
-        o[n][i] = partial ? guarded16<T>(vf, p[n], o[n][i]) : mma16<T>(vf, p[n], o[n][i]);
+        o[n][i] = partial ? guarded16<T>(vf, p[n], o[n][i], visible[n]) : mma16<T>(vf, p[n], o[n][i]);
     }
     wave_sync();
   }

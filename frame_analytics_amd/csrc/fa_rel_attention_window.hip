@@ -241,7 +241,8 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
 #pragma unroll
         for (int i = 0; i < OB; ++i) {
           const typename M::V8 vf = TL::transposed(vt, 32 * nb + 16 * half, 32 * i, lane);
-          o[i] = all || tame ? M::mma(vf, pf, o[i]) : guarded<T>(vf, pf, o[i]);
+          o[i] = all || tame ? M::mma(vf, pf, o[i])
+                               : guarded<T>(vf, pf, o[i], seen >> (16 * nb + 8 * half));
         }
       }
     }

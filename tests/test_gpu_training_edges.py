@@ -62,6 +62,69 @@ def test_a_nan_key_that_stands_alone_in_its_run(gpu, dt, last):
     assert not torch.isnan(out[0, :2]).any() and not torch.isnan(out[1]).any()
 
 
+def hidden_case(form, dt):
+    """q, k, v, table, positions and arguments of a call with hidden pairs in each tile."""
+    gen = torch.Generator().manual_seed(11)
+    if form == "window":
+        b, h, lq, lk, pos = 3, 2, 64, 64, fa.GridPositions(8, 8)
+    elif form == "wide window":
+        b, h, lq, lk, pos = 2, 2, 144, 144, fa.GridPositions(12, 12)
+    else:
+        b, h, pos = 2, 2, fa.LinePositions(8, 20)
+        lq, lk = {"line": (80, 80), "few": (4, 600), "one run": (4, 100)}[form]
+    q, k, v = (normal(gen, DT[dt], b, h, n, 32) for n in (lq, lk, lk))
+    mask = torch.rand(1, 1, lq, lk, generator=gen) < 0.7
+    return q, k, v, torch.zeros(pos.rows, h, dtype=DT[dt]), pos, mask
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("form", ["window", "wide window", "line", "few", "one run"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_weight_too_small_for_the_type_still_sees(gpu, dt, form, bad):
+    """A value that is not finite reaches every query that sees its key, however little
+    that key counts (a weight of exp(-25): zero in float16, not in float32), and none
+    that does not."""
+    q, k, v, table, pos, mask = hidden_case(form, dt)
+    q[..., 0], k[..., 0] = 5.0, 0.0
+    k[:, :, 30, 0] = -5.0
+    q[..., 1:] *= 0.1
+    v[:, :, 30, 7] = bad
+    mask[..., 0, 30], mask[..., 1, 30] = True, False
+    out = fa.relative_attention(*(t.cuda() for t in (q, k, v, table)), pos, scale=1.0,
+                                mask=mask.cuda()).cpu()
+    see = mask[0, 0, :, 30]
+    assert not torch.isfinite(out[:, :, see, 7]).any()
+    assert torch.isfinite(out[:, :, ~see]).all()
+    other = torch.arange(32) != 7
+    assert torch.isfinite(out[..., other]).all()
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("form", ["window", "wide window", "few", "one run"])
+def test_what_no_query_sees_may_hold_anything(gpu, dt, form):
+    """NaN and infinities at keys that the mask or the lengths hide from all, and in
+    queries that see nothing, reach no result."""
+    q, k, v, table, pos, mask = hidden_case(form, dt)
+    gen = torch.Generator().manual_seed(12)
+    table = normal(gen, DT[dt], *table.shape)
+    g = normal(gen, DT[dt], *q.shape)
+    b, h, lq, lk = *q.shape[:3], k.shape[2]
+    mask[..., 2, :] = False
+    mask[..., :, 9] = False
+    lens = torch.tensor([lk, lk - 13, lk // 2][:b], dtype=torch.int32)
+    see = ref.visible(b, h, lq, lk, mask=mask.numpy(), key_lengths=lens.numpy())
+    rows = ref.grid_rows(pos.height, pos.width) if pos.grid_w else ref.line_rows(lq, lk, 0, 8, 20)
+    want = ref.attention(*(t.double().numpy() for t in (q, k, v, table)), rows, see, 32 ** -0.5,
+                         g.double().numpy())
+    q[:, :, 2], g[:, :, 2] = float("nan"), float("inf")
+    k[:, :, 9], v[:, :, 9] = float("inf"), float("nan")
+    for i, n in enumerate(lens.tolist()):
+        k[i, :, n:], v[i, :, n:] = float("nan"), -float("inf")
+    got = run_attention((q, k, v, table), g, pos, mask=mask.cuda(), key_lengths=lens.cuda())
+    for name, x, y, t in zip(("out", "dq", "dk", "dv", "dtable"), got, want, (2, 4, 4, 4, 4)):
+        near(x, y, t * UNIT[dt], name)
+
+
 # --------------------------------------------------------------------------- #
 # biases at the type's limits
 # --------------------------------------------------------------------------- #

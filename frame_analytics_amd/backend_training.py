@@ -145,9 +145,10 @@ def rel_attention(q, k, v, table, plan: AttentionPlan, need_lse: bool):
     hk, lk = k.shape[1], k.shape[2]
     out = _like(q)
     lse = None
-    if need_lse:  # the rows' log-sums, and on a line what the rounding of a 16-bit output left
-        n = b * h * lq
-        n = n if q.dtype == torch.float32 or plan.positions.grid_w else (n + 3) // 4 * 4 + (n * d + 1) // 2
+    if need_lse:  # two numbers a row, and on a line what the rounding of a 16-bit output left
+        n = 2 * b * h * lq
+        if q.dtype != torch.float32 and not plan.positions.grid_w:
+            n = (n + 3) // 4 * 4 + (b * h * lq * d + 1) // 2
         lse = torch.empty(n, dtype=torch.float32, device=q.device)
     dev, stream = _site(q)
     ws, n = _workspace("fa_gpu_rel_attention_workspace", q.device, b, h, hk, lq, lk, d,

@@ -41,6 +41,20 @@ struct RelAttn {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float INF = __builtin_inff();
 
+// A bias times log2(e).  Past 2^126 that product would leave float32 (the lowest values of
+// bfloat16 and float32 hide pairs in many a program): from there on it grows by 0.8, finite
+// at the type's limit and in the same order.  A row of equal extremes has equal weights so.
+__device__ inline float bias_log2(float v) {
+  constexpr float T = 0x1p126f;
+  const float m = __builtin_fabsf(v);
+  return m > T ? __builtin_copysignf(T * LOG2E + (m - T) * 0.8f, v) : v * LOG2E;
+}
+
+// The largest bias (times log2(e)) that may be taken with a row's maximum at once, s + (far -
+// maximum), and the largest maximum that may be kept with its sum in one number: larger ones
+// round the scores, and have to round all of a row alike.
+constexpr float FAR_MOST = 4096.0f;
+
 // The bias of `heads` heads from h on, by slot in LDS, times log2(e), with PAD copies
 // of either end's value: a 32 x 32 block that has one difference within (lo, lo + n -
 // 1) has none further than 62 past it, so its reads need no clamp.  The two reads of a
@@ -63,8 +77,15 @@ __device__ inline void load_bias(float* eb, const T* table, int H, int h, int he
     for (int e = 0; e < 4; ++e) v[e] = widen(table[static_cast<int64_t>(row[e]) * H + h + head[e]]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (t0 + e * nt < total) eb[t0 + e * nt] = v[e] * LOG2E;
+      if (t0 + e * nt < total) eb[t0 + e * nt] = bias_log2(v[e]);
   }
+}
+
+// Whether the biases past both ends of a head's table in LDS, np floats wide, are below
+// FAR_MOST: asked once, behind a barrier before the loop over tiles (read from memory at the
+// kernel's start, one load after the other, it took 1 us more of 43).
+__device__ inline bool far_serves(const float* eb, int np) {
+  return __builtin_amdgcn_readfirstlane(__builtin_fabsf(eb[0]) < FAR_MOST && __builtin_fabsf(eb[np - 1]) < FAR_MOST);
 }
 
 // The codes of a window's tokens in LDS, the last one's repeated to a whole tile (a
@@ -74,7 +95,20 @@ __device__ inline void load_codes(int* codes, const RelPos& pos, int n, int tid,
   for (int t = tid; t < codes_room(n); t += nt) codes[t] = pos.code(min(t, n - 1));
 }
 
-// What the output's rounding left, kept behind the log-sums for 16-bit types on a line:
+// What a call with gradients keeps of each row's softmax: a shift, and for all rows behind
+// them a factor, with which the weights are 2^(score - shift) times the factor.  The shift
+// is the log of the sum and the factor 1, unless the largest score would round the sum away
+// (a row whose biases are all the type's lowest): then that score and one over the sum.  A
+// row that sees nothing has a shift of +inf.
+__device__ inline void keep_row(float* rows, int64_t all, int64_t row, float top, float sum) {
+  const bool plain = sum == 0.0f || __builtin_fabsf(top) < FAR_MOST;
+  rows[row] = sum == 0.0f ? INF : plain ? top + __builtin_log2f(sum) : top;
+  rows[all + row] = plain ? 1.0f : 1.0f / sum;
+}
+// Whether a row may have a factor other than 1.
+__device__ inline bool has_factor(float shift) { return !(__builtin_fabsf(shift) < FAR_MOST) && shift != INF; }
+
+// What the output's rounding left, kept behind the rows' for 16-bit types on a line:
 // D_i = dout_i . out_i is subtracted from every dP of a row, and a row's far keys share one
 // entry of the table, which takes D_i's error as many times.  Measured on a causal line of
 // 2048 in bfloat16, three inputs: the largest relative error of a gradient 2.5e-3 without
@@ -83,13 +117,20 @@ __device__ inline void load_codes(int* codes, const RelPos& pos, int n, int tid,
 // 16 windows had 3.0e-4 with it and without, and 740 us without against 776 with, so that
 // they keep none.
 template <typename T> __device__ inline T* low_of(const float* lse, int64_t rows) {
-  return reinterpret_cast<T*>(const_cast<float*>(lse) + (rows + 3) / 4 * 4);
+  return reinterpret_cast<T*>(const_cast<float*>(lse) + (2 * rows + 3) / 4 * 4);
 }
 
 // How the pairs of a 32 x 32 block stand to the bias table.
 enum : int { NEAR = 0, ALL_BELOW = 1, ALL_ABOVE = 2 };
 __device__ inline int block_kind(const RelPos& pos, int dmin, int dmax) {
   return dmax <= pos.lo ? ALL_BELOW : dmin >= pos.lo + pos.n - 1 ? ALL_ABOVE : NEAR;
+}
+
+// The bias past an end of a head's table in LDS, np floats wide, in a scalar register (for
+// dK and dV: there far_serves and the bias in a vector register spill 40 registers, 16-bit
+// heads of 64).
+__device__ inline float far_bias(const float* eb, int np, int kind) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(kind == ALL_BELOW ? eb[0] : eb[np - 1])));
 }
 
 // Bit r: whether pair r of a lane's 16 counts, steps 8 (r / 4) + r % 4 from its first
@@ -267,8 +308,7 @@ struct WindowGrads {
 };
 bool window_serve(const RelAttn& a);
 int window_parts(int B, int H, int device);
-int window_forward(int dtype, const RelAttn& a, void* out, const View& os, float* lse, int device,
-                   hipStream_t s);
+int window_forward(int dtype, const RelAttn& a, void* out, const View& os, int device, hipStream_t s);
 int window_backward(int dtype, const RelAttn& a, const WindowGrads& g, int rows, void* dtable, int device,
                     hipStream_t s);
 

@@ -169,6 +169,8 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
     }
   };
   const int rounds = (tiles + KG - 1) / KG;
+  __syncthreads();
+  const bool far_on = c > 0.0f && far_serves(eb, a.pos.n + 2 * PAD);
   for (int round = 0; round < rounds; ++round) {
     const int t = round * KG + kg;
     __syncthreads();
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
     const int kind = block_kind(a.pos, s0 + qw - (k0 + BN - 1), s0 + qw + 31 - k0);
     if (all && a.pos.grid_w)
       work(t, std::integral_constant<int, WINDOW>(), 0.0f);
-    else if (all && kind != NEAR && c > 0.0f)
+    else if (all && kind != NEAR && far_on)
       work(t, std::integral_constant<int, FAR>(), kind == ALL_BELOW ? eb[0] : eb[a.pos.n + 2 * PAD - 1]);
     else
       work(t, std::integral_constant<int, ANY>(), 0.0f);
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
         }
       }
     if (lse && hh == 0)
-      lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + q] = l == 0.0f ? INF : m + __builtin_log2f(l);
+      keep_row(lse, static_cast<int64_t>(a.B) * a.H * a.Lq, (static_cast<int64_t>(b) * a.H + h) * a.Lq + q, m, l);
   }
 }
 
@@ -327,7 +329,7 @@ FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int
                                   mask, mask_b, mask_strides, causal, scale);
   const View os{strides[9], strides[10], strides[11]};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (window_serve(a)) return window_forward(dtype, a, out, os, lse, device, s);
+  if (window_serve(a)) return window_forward(dtype, a, out, os, device, s);
   if (rows_serve(a)) return rows_forward(dtype, a, out, os, lse, workspace, workspace_bytes, device, s);
   switch (dtype) {
     case FA_F16: return forward<_Float16>(a, out, os, lse, device, s);

@@ -1,6 +1,6 @@
 // Attention with a relative position bias, backward.
 //
-// With P the weights (formed again from the scores and each row's log-sum) and D_i =
+// With P the weights (formed again from the scores and what the forward pass kept) and D_i =
 // dout_i . out_i:  dS = P (dout V^T - D);  dQ = scale dS K;  dK = scale dS^T Q;
 // dV = P^T dout;  dtable[r] = the sum of dS over the pairs of row r.
 //
@@ -19,8 +19,8 @@ enum : int { ANY, FAR, WINDOW };  // the pairs of a tile
 struct Grads {
   const void *out, *dout;
   View os, gs;
-  const float* lse;
-  float* dsum;  // [B, H, Lq]: D_i
+  const float* lse;  // [2][B, H, Lq]: shifts and factors, see keep_row
+  float* dsum;       // [B, H, Lq]: D_i times the row's factor
   void *dq, *dk, *dv;
   View dqs, dks, dvs;
   int dqvec, dkvec;
@@ -40,6 +40,17 @@ template <typename T> __device__ inline typename Mat<T>::V8 finite(typename Mat<
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __builtin_fabsf(widen(v[i])) < INF ? v[i] : T(0);
   return v;
+}
+
+// A row's factor (rarely any but 1: read where it is used), and dout times it.
+__device__ inline float factor_of(const RelAttn& a, const Grads& g, int64_t row, float shift) {
+  return has_factor(shift) ? g.lse[static_cast<int64_t>(a.B) * a.H * a.Lq + row] : 1.0f;
+}
+template <typename T, int N> __device__ inline void scale_row(typename Mat<T>::V8 (&v)[N], float f) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = T(widen(v[i][e]) * f);
 }
 
 // ---------------------------------------------------------------------------
@@ -113,6 +124,9 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS / 
     load_row<T, WIDE>(qf, rows(a.q, a.qs), q - f, 8 * hh, a.D, a.vec, on);
     load_row<T, WIDE>(gf, rows(g.dout, g.gs), q - f, 8 * hh, a.D, a.vec, on);
     load_row<T, WIDE>(of, rows(g.out, g.os), q - f, 8 * hh, a.D, a.vec, on);
+    // a row's factor goes into dout, and so into dP and D_i: such a row's weights without it
+    // are nearly all 0 or 1, which round to no fewer bits
+    if (__ballot(has_factor(lse))) scale_row<T>(gf, factor_of(a, g, row, lse));
 #pragma unroll
     for (int i = 0; i < CH; ++i) dd = M::mma(of[i], gf[i], dd);
     if (sizeof(T) == 2 && KEYS == 0 && a.pos.grid_w == 0) {  // and what the output's rounding left
@@ -146,6 +160,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS / 
   TileLoad<T, DP, BN, NT, WIDE> kl, vl;
   const int tiles = (end + BN - 1) / BN;
   if (KEYS > 0) __syncthreads();  // the window before is done with the tiles
+  bool far_on = false;
   if (kg < tiles) {
     const int k1 = kg * BN;
     kl.load(kb + k1 * a.ks.t, a.ks.t, len - k1, a.D, a.vec, tid);
@@ -268,7 +283,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS / 
     far_below = kind == ALL_BELOW;
     if (KEYS > 0 && all)
       work(t, pairs, std::integral_constant<int, WINDOW>(), 0.0f);
-    else if (KEYS == 0 && all && a.pos.grid_w == 0 && kind != NEAR)
+    else if (KEYS == 0 && all && a.pos.grid_w == 0 && kind != NEAR && far_on)
       work(t, pairs, std::integral_constant<int, KEYS == 0 ? FAR : ANY>(), far_below ? eb[0] : eb[np - 1]);
     else
       work(t, pairs, std::integral_constant<int, ANY>(), 0.0f);
@@ -284,6 +299,8 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS / 
       if (round * KG < tiles) step(round * KG + kg, total + round * NB);
   } else {
     const int rounds = (tiles + KG - 1) / KG;
+    __syncthreads();
+    far_on = far_serves(eb, np);
     for (int round = 0; round < rounds; ++round) step(round * KG + kg, total);
   }
   if constexpr (KG > 1) {
@@ -444,6 +461,20 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 ? (DP == 32 ? 3 : DP =
           for (int e = 0; e < 8; ++e) ql.r[i][e] = gl.r[i][e] = T(0);
       ql.store(qt + (t / KG % BUFS) * BM * TL::LD, tid);
       gl.store(gt + (t / KG % BUFS) * BM * TL::LD, tid);
+      bool factors = false;
+#pragma unroll
+      for (int i = 0; i < ql.N; ++i) factors |= has_factor(row_lse[i]);
+      if (__ballot(factors)) {  // (as in dQ; each thread what it stored)
+        T* tile = gt + (t / KG % BUFS) * BM * TL::LD;
+#pragma unroll 1
+        for (int piece = afresh(tid); piece < BM * ql.PER_ROW; piece += NT) {
+          const int r = piece / ql.PER_ROW, i = t * BM + r;
+          const float f = i < a.Lq ? factor_of(a, g, row0 + i, g.lse[row0 + i]) : 1.0f;
+          T* p = tile + r * TL::LD + piece % ql.PER_ROW * 8;
+#pragma unroll 1
+          for (int e = 0; e < 8; ++e) p[e] = T(widen(p[e]) * f);
+        }
+      }
       if (tid < BM) {
         ls[(t / KG & 1) * BM + tid] = lse_r;
         dd[(t / KG & 1) * BM + tid] = d_r;
@@ -480,7 +511,9 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 ? (DP == 32 ? 3 : DP =
           s = M::mma(TL::straight(qq, nb * 32 + col, 16 * i + 8 * hh), kf[i], s);
           dp = M::mma(TL::straight(gg, nb * 32 + col, 16 * i + 8 * hh), vf[i], dp);
         }
-        const bool partial = MODE == ANY && (mask || kw + 32 > len || (a.causal && kw + 31 > s0 + i0));
+        // (a query that sees no key, or stands past Lq, hides its pairs by one of these)
+        const bool partial = MODE == ANY && (mask || kw + 32 > len || i0 + 32 > a.Lq ||
+                                             (a.causal && kw + 31 > s0 + i0));
         int kind = NEAR;
         if (MODE == FAR) {
 #pragma unroll
@@ -514,10 +547,8 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 ? (DP == 32 ? 3 : DP =
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * r4 + e;
-            // a row with a log-sum of +inf sees no key, whatever its query holds
-            const float p = l4[e] == INF ? 0.0f : __builtin_amdgcn_exp2f(s[r] - l4[e]);
-            s[r] = p;
-            dp[r] = l4[e] == INF ? 0.0f : p * (dp[r] - d4[e]);
+            s[r] = __builtin_amdgcn_exp2f(s[r] - l4[e]);
+            dp[r] = s[r] * (dp[r] - d4[e]);
           }
         }
         if (partial) {
@@ -552,8 +583,8 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 ? (DP == 32 ? 3 : DP =
       const int kind = block_kind(a.pos, s0 + q0 - (kw + 31), s0 + q1 - 1 - kw);
       if (all && a.pos.grid_w)
         work(std::integral_constant<int, WINDOW>(), 0.0f);
-      else if (all && kind != NEAR)
-        work(std::integral_constant<int, FAR>(), kind == ALL_BELOW ? eb[0] : eb[np - 1]);
+      else if (const float far = far_bias(eb, np, kind); all && kind != NEAR && __builtin_fabsf(far) < FAR_MOST)
+        work(std::integral_constant<int, FAR>(), far);
       else
         work(std::integral_constant<int, ANY>(), 0.0f);
       if (more) {
@@ -722,7 +753,12 @@ int launch_wide(const RelAttn& a, const Grads& g, const Plan& p, hipStream_t s) 
   } else {
     e = p.nw_q == 4 ? launch_dq<T, DP, 4, 1, WIDE>(a, g, p, s) : launch_dq<T, DP, 2, 1, WIDE>(a, g, p, s);
     if (e) return e;
-    e = p.nw_k == 4 ? launch_dkv<T, DP, 4, 1, WIDE>(a, g, p, s) : launch_dkv<T, DP, 2, 1, WIDE>(a, g, p, s);
+    // (float32: a thread of two waves would hold 64 registers of tiles on their way beside
+    // 256 of fragments and sums, which the compiler does not allocate)
+    if constexpr (sizeof(T) == 4)
+      e = launch_dkv<T, DP, 4, 1, WIDE>(a, g, p, s);
+    else
+      e = p.nw_k == 4 ? launch_dkv<T, DP, 4, 1, WIDE>(a, g, p, s) : launch_dkv<T, DP, 2, 1, WIDE>(a, g, p, s);
   }
   if (e || p.splits == 1) return e;
   const int64_t want = (2 * static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.D + 255) / 256;

@@ -311,8 +311,8 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
         low_of<T>(lse, static_cast<int64_t>(a.B) * a.H * a.Lq)[((static_cast<int64_t>(b) * a.H + hr) * a.Lq + ir) *
                                                                    a.D + d] = T(x - widen(T(x)));
       if (lse && d == 0)
-        lse[(static_cast<int64_t>(b) * a.H + hr) * a.Lq + ir] =
-            total == 0.0f ? INF : top + __builtin_log2f(total);
+        keep_row(lse, static_cast<int64_t>(a.B) * a.H * a.Lq, (static_cast<int64_t>(b) * a.H + hr) * a.Lq + ir, top,
+                 total);
     }
   }
 }
@@ -368,14 +368,14 @@ __global__ __launch_bounds__(64) void rows_join_kernel(const float* part_o, cons
   x1 *= inv;
   if (d0 < D) o[d0] = T(x0);
   if (d1 < D) o[d1] = T(x1);
-  if (sizeof(T) == 2 && lse) {
-    const int64_t all = static_cast<int64_t>(gridDim.x / rows / Hk) * H * Lq;  // batch x heads x queries
+  if (!lse) return;
+  const int64_t all = static_cast<int64_t>(gridDim.x / rows / Hk) * H * Lq;  // batch x heads x queries
+  if (lane == 0) keep_row(lse, all, (static_cast<int64_t>(b) * H + h) * Lq + i, top, total);
+  if (sizeof(T) == 2) {
     T* low = low_of<T>(lse, all) + ((static_cast<int64_t>(b) * H + h) * Lq + i) * D;
     if (d0 < D) low[d0] = T(x0 - widen(T(x0)));
     if (d1 < D) low[d1] = T(x1 - widen(T(x1)));
   }
-  if (lse && threadIdx.x == 0)
-    lse[(static_cast<int64_t>(b) * H + h) * Lq + i] = total == 0.0f ? INF : top + __builtin_log2f(total);
 }
 
 template <typename T, int DP, int NC>

@@ -136,7 +136,7 @@ __device__ inline void load_pair_bias(float (&bias)[2][16], const RelAttn& a, co
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int row = a.pos.row_of[a.pos.slot(cq - a.pos.code(min(p.key(nb, r), a.Lk - 1)))];
-      bias[nb][r] = widen(table[static_cast<int64_t>(row) * a.H + h]) * LOG2E;
+      bias[nb][r] = bias_log2(widen(table[static_cast<int64_t>(row) * a.H + h]));
     }
 }
 
@@ -166,7 +166,7 @@ __device__ inline float scores(f32x16 (&s)[2], const T* kt, const typename Mat<T
 }
 
 template <typename T, int DP, int ACCESS>
-__global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View os, float* lse, int chunks) {
+__global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View os, int chunks) {
   using M = Mat<T>;
   using TL = Tile<T, DP>;
   constexpr int CH = DP / 16, OB = DP / 32;
@@ -253,10 +253,6 @@ __global__ __launch_bounds__(NT, 2) void window_kernel(RelAttn a, T* out, View o
     if (more) store(b + chunks);
     store_rows<T, DP, ACCESS>(ot + wave * 32 * TL::LD, o, l == 0.0f ? 0.0f : 1.0f / l, out + b * os.b + h * os.h, os.t, wave * 32,
                               a.Lq, a.D, lane);
-    if (lse && p.q < a.Lq) {
-      if (hh == 0)
-        lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + p.q] = l == 0.0f ? INF : m + __builtin_log2f(l);
-    }
   }
 }
 
@@ -471,11 +467,11 @@ inline int chunks_of(int B, int H, int device, int fit) {
 }
 
 template <typename T, int DP, int ACCESS>
-int launch_forward(const RelAttn& a, T* out, const View& os, float* lse, int chunks, hipStream_t s) {
+int launch_forward(const RelAttn& a, T* out, const View& os, int chunks, hipStream_t s) {
   const size_t lds = 4 * tile_bytes<T, DP>();
   auto kernel = window_kernel<T, DP, ACCESS>;
   if (const int e = launch_lds(kernel, lds)) return e;
-  kernel<<<static_cast<unsigned>(chunks * a.H), NT, lds, s>>>(a, out, os, lse, chunks);
+  kernel<<<static_cast<unsigned>(chunks * a.H), NT, lds, s>>>(a, out, os, chunks);
   FA_LAUNCH_CHECK();
   return FA_OK;
 }
@@ -501,7 +497,7 @@ template <typename T, typename Go> int with_access(int vec, const Go& go) {
 }
 
 template <typename T>
-int forward(RelAttn a, void* out, const View& os, float* lse, int device, hipStream_t s) {
+int forward(RelAttn a, void* out, const View& os, int device, hipStream_t s) {
   const void* views[4] = {a.q, a.k, a.v, out};
   const View vs[4] = {a.qs, a.ks, a.vs, os};
   a.vec = widest_load<T>(views, vs, 4, a.D);
@@ -509,8 +505,8 @@ int forward(RelAttn a, void* out, const View& os, float* lse, int device, hipStr
   T* o = static_cast<T*>(out);
   auto go = [&](auto access) {
     constexpr int ACCESS = decltype(access)::value;
-    return a.D <= 32 ? launch_forward<T, 32, ACCESS>(a, o, os, lse, chunks, s)
-                     : launch_forward<T, 64, ACCESS>(a, o, os, lse, chunks, s);
+    return a.D <= 32 ? launch_forward<T, 32, ACCESS>(a, o, os, chunks, s)
+                     : launch_forward<T, 64, ACCESS>(a, o, os, chunks, s);
   };
   return with_access<T>(a.vec, go);
 }
@@ -543,12 +539,11 @@ bool window_serve(const RelAttn& a) {
 
 int window_parts(int B, int H, int device) { return chunks_of(B, H, device, 4); }
 
-int window_forward(int dtype, const RelAttn& a, void* out, const View& os, float* lse, int device,
-                   hipStream_t s) {
+int window_forward(int dtype, const RelAttn& a, void* out, const View& os, int device, hipStream_t s) {
   switch (dtype) {
-    case FA_F16: return forward<_Float16>(a, out, os, lse, device, s);
-    case FA_BF16: return forward<__bf16>(a, out, os, lse, device, s);
-    case FA_F32: return forward<float>(a, out, os, lse, device, s);
+    case FA_F16: return forward<_Float16>(a, out, os, device, s);
+    case FA_BF16: return forward<__bf16>(a, out, os, device, s);
+    case FA_F32: return forward<float>(a, out, os, device, s);
     default: return FA_E_DTYPE;
   }
 }

@@ -57,10 +57,11 @@ FA_API int fa_gpu_rel_bias_backward(const void* up, const int64_t* up_strides, i
  * of q, k, v and out; the last dimension has stride 1.  1 <= D <= 128.
  * start: q_starts[b] (int32, device) or, where that is null, q_start; both are taken
  * as within +-2^30.  mask_strides: {batch, head, query, key} in bytes.
- * lse: null, or what the backward pass reads: [B, H, Lq] float32, log2 of each row's
- * sum of exponentials, +inf for a row that sees nothing; for FA_F16 and FA_BF16 with
- * grid_w 0, from the next multiple of 16 bytes on, [B, H, Lq, D] of dtype: what the
- * rounding of out left.
+ * lse: null, or what the backward pass reads, 16-byte aligned: [2, B, H, Lq] float32, with
+ * which a row's weights are 2^(score log2(e) - the first) times the second (the first +inf
+ * for a row that sees nothing); for FA_F16 and FA_BF16 with grid_w 0, from the next multiple
+ * of 16 bytes on, [B, H, Lq, D] of dtype: what the rounding of out left.  (Windows of up to
+ * 64 tokens may leave it unwritten.)
  * workspace: fa_gpu_rel_attention_workspace bytes, 16-byte aligned (0: may be null).
  */
 FA_API int fa_gpu_rel_attention_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int n,

@@ -130,6 +130,64 @@ def test_what_no_query_sees_may_hold_anything(gpu, dt, form):
 # --------------------------------------------------------------------------- #
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("form", ["line", "causal", "few", "one", "window", "wide window"])
+@pytest.mark.parametrize("extreme", ["lowest", "largest", "-inf"])
+def test_biases_at_the_limits_of_the_type(gpu, dt, form, extreme):
+    """Head 0: every entry; head 1: every other; head 2: the farthest; head 3: none.  A
+    row of equal extremes has equal weights, whatever its scores (which such a bias
+    rounds away); a row of -inf alone sees nothing."""
+    gen = torch.Generator().manual_seed(21)
+    b, h, d, kw, start = 2, 4, 32, {}, 0
+    if form == "window":
+        pos, lq = fa.GridPositions(8, 8), 64
+        lk, rows = lq, ref.grid_rows(8, 8)
+    elif form == "wide window":
+        pos, lq = fa.GridPositions(9, 10), 90
+        lk, rows = lq, ref.grid_rows(9, 10)
+    else:
+        pos = fa.LinePositions(8, 20)
+        lq, lk = {"line": (150, 400), "causal": (300, 300), "few": (5, 700), "one": (1, 90)}[form]
+        start = 40 if form in ("few", "one") else 0
+        rows = ref.line_rows(lq, lk, start, 8, 20)
+        kw = {"causal": form == "causal", "q_start": start}
+    q, k, v, g = (normal(gen, DT[dt], b, h, n, d) for n in (lq, lk, lk, lq))
+    table = normal(gen, DT[dt], pos.rows, h)
+    info = torch.finfo(DT[dt])
+    value = {"lowest": info.min, "largest": info.max, "-inf": -float("inf")}[extreme]
+    table[:, 0] = value
+    table[::2, 1] = value
+    table[-1, 2] = value
+    see = ref.visible(b, h, lq, lk, causal=form == "causal", q_start=start)
+    finite = np.where(np.isinf(table.double().numpy()), 0.0, table.double().numpy())
+    if extreme == "-inf":  # such a pair is hidden
+        see = see & ~np.isinf(table.double().numpy())[rows].transpose(2, 0, 1)[None]
+    want = ref.attention(*(t.double().numpy() for t in (q, k, v)), finite, rows, see, d ** -0.5,
+                         g.double().numpy())
+    got = run_attention((q, k, v, table), g, pos, **kw)
+    # float16's limits round a score by 65504 2^-24, and as much the maximum beside it
+    more = 4 * 65504 * 2.0 ** -24 if dt == "f16" and extreme != "-inf" else 0.0
+    for name, x, y, t in zip(("out", "dq", "dk", "dv", "dtable"), got, want, (2, 4, 4, 4, 4)):
+        near(x, y, t * UNIT[dt] / (1 if dt == "f32" else 2) + more, name)
+
+
+def test_large_biases_keep_their_order(gpu):
+    """Entries near the limits that differ: the larger takes the whole weight."""
+    pos = fa.LinePositions(4, 5, bidirectional=False)
+    top = torch.finfo(torch.float32).max
+    v = torch.eye(12, device="cuda")[None, None]
+    z = torch.zeros(1, 1, 12, 12, device="cuda")
+    for values in ((-top, -0.9 * top, -0.5 * top, -0.25 * top), (top, 0.99 * top, 0.5 * top, 0.2 * top),
+                   (-0.25 * top, -0.24 * top, -0.26 * top, -0.3 * top), (1e30, 1.1e30, -1e30, 1e37)):
+        table = torch.tensor(values, device="cuda")[:, None]
+        out = fa.relative_attention(z, z, v, table, pos, causal=True)[0, 0]
+        bias = fa.relative_bias(table, pos, 12)[0].double()
+        bias = bias.masked_fill(torch.ones_like(bias).triu(1).bool(), -float("inf"))
+        want = torch.softmax(bias, -1)
+        assert torch.equal(out.double() > 0, want > 0), values
+        near(out, want.cpu().numpy(), 2e-5)
+
+
 # --------------------------------------------------------------------------- #
 # views, tangents
 # --------------------------------------------------------------------------- #

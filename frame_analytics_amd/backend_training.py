@@ -58,8 +58,10 @@ def _workspace(name: str, device, *shape: int):
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
-    """``t``, copied unless its last dimension has stride 1."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """``t`` (batch, heads, tokens, dim), copied unless its last dimension has stride 1 and
+    256 tokens lie within the 2^31 bytes that a kernel's offsets reach."""
+    near = t.shape[2] == 1 or 256 * t.element_size() * t.stride(2) < 1 << 31
+    return t if near and (t.stride(-1) == 1 or t.shape[-1] == 1) else t.contiguous()
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
@@ -77,7 +79,8 @@ def _int32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 def _strides(*views: torch.Tensor):
-    flat = [s for v in views for s in v.stride()[:3]]
+    """The first three of each; 0 where there is one element, whose stride says nothing."""
+    flat = [s if n > 1 else 0 for v in views for n, s in zip(v.shape[:3], v.stride()[:3])]
     return (ctypes.c_int64 * len(flat))(*flat)
 
 

@@ -374,8 +374,9 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
 
     ``q`` is ``(batch, heads, tokens, dim)``, ``k`` and ``v`` ``(batch, key heads, keys,
     dim)`` with the key heads dividing the heads (each is shared by neighbouring query
-    heads); any strides, the last dimension contiguous (else copied); ``dim`` up to 128.
-    The result is laid out as q is.  A table of another type is rounded to q's first.
+    heads); any strides, the last dimension contiguous (else copied, as is a view of which
+    256 tokens span 2 GiB); ``dim`` up to 128.  The result is laid out as q is (as its copy
+    where it was copied).  A table of another type is rounded to q's first.
 
     ``scale`` defaults to ``dim ** -0.5``.  A pair counts where all of these allow it:
     ``causal`` (the key's position is not after the query's), ``key_lengths`` ((batch,)

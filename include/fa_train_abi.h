@@ -54,7 +54,8 @@ FA_API int fa_gpu_rel_bias_backward(const void* up, const int64_t* up_strides, i
  *
  * q, out: [B, H, Lq, D]; k, v: [B, Hk, Lk, D], H a multiple of Hk: query head h
  * reads key head h / (H / Hk).  strides: 12 int64 in elements, {batch, head, token}
- * of q, k, v and out; the last dimension has stride 1.  1 <= D <= 128.
+ * of q, k, v and out; the last dimension has stride 1, and 256 tokens lie within 2^31
+ * bytes (FA_E_SHAPE).  1 <= D <= 128.
  * start: q_starts[b] (int32, device) or, where that is null, q_start; both are taken
  * as within +-2^30.  mask_strides: {batch, head, query, key} in bytes.
  * lse: null, or what the backward pass reads, 16-byte aligned: [2, B, H, Lq] float32, with

@@ -193,6 +193,32 @@ def test_large_biases_keep_their_order(gpu):
 # --------------------------------------------------------------------------- #
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("lq", [1, 3, 40])
+def test_token_strides_of_any_width(gpu, dt, lq):
+    """Tokens first: a token's stride is the whole batch's width."""
+    wide = 2 ** 31 // (256 * DT[dt].itemsize) + 24
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    pos = fa.LinePositions(8, 20)
+    table = torch.randn(8, 2, generator=gen, device="cuda").to(DT[dt])
+
+    def spread(n):
+        flat = torch.empty(n * wide, dtype=DT[dt], device="cuda")
+        t = flat.as_strided((1, 2, n, 16), (64, 16, wide, 1))
+        t.copy_(torch.randn(t.shape, generator=gen, device="cuda"))
+        return t
+
+    ts, g = [spread(n) for n in (lq, 50, 50)], spread(lq)
+    plain = [t.contiguous().requires_grad_(True) for t in ts]
+    want = fa.relative_attention(*plain, table, pos)
+    want.backward(g.contiguous())
+    ts = [t.requires_grad_(True) for t in ts]
+    got = fa.relative_attention(*ts, table, pos)
+    got.backward(g)
+    assert torch.equal(got, want)
+    assert all(torch.equal(x.grad, y.grad) for x, y in zip(ts, plain))
+
+
 # --------------------------------------------------------------------------- #
 # updates
 # --------------------------------------------------------------------------- #

@@ -30,6 +30,7 @@ namespace {
 typedef _Float16 f16;
 constexpr int NT = 256;
 constexpr int SUMS = 512;                    // most partial sums of squares per matrix
+constexpr int MOST_BATCH = 65535;            // matrices at a time: a grid's height
 constexpr float SX = 2048.0f, SP = 1024.0f;  // scale of X and A, of the polynomial
 
 template <typename T> __device__ inline float widen(T v) { return static_cast<float>(v); }
@@ -418,8 +419,8 @@ inline int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 inline int plan(int dtype, int batch, int rows, int cols, Plan* p) {
   if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return FA_E_DTYPE;
-  if (batch < 1 || rows < 1 || cols < 1 || batch > 65535 || rows > (1 << 20) || cols > (1 << 20))
-    return FA_E_SHAPE;
+  if (batch < 1 || rows < 1 || cols < 1 || rows > (1 << 20) || cols > (1 << 20)) return FA_E_SHAPE;
+  if (batch > MOST_BATCH) batch = MOST_BATCH;
   p->m = rows < cols ? rows : cols;
   p->n = rows < cols ? cols : rows;
   // up to 64 rows a product is a launch's time whatever its precision, and little
@@ -559,14 +560,23 @@ FA_API int fa_gpu_orthogonalize(const void* g, int dtype, int batch, int rows, i
   const Poly poly{static_cast<float>(a), static_cast<float>(b), static_cast<float>(c)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  switch (dtype) {
-    case FA_BF16:
-      return p.parts == 1
-                 ? orthogonalize<__bf16, false>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s)
-                 : orthogonalize<__bf16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s);
-    case FA_F16: return orthogonalize<f16, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s);
-    default: return orthogonalize<float, true>(g, batch, rows, cols, steps, poly, eps, out, ws, p, device, s);
+  auto some = [&](const void* from, void* to, int count) {
+    switch (dtype) {
+      case FA_BF16:
+        return p.parts == 1
+                   ? orthogonalize<__bf16, false>(from, count, rows, cols, steps, poly, eps, to, ws, p, device, s)
+                   : orthogonalize<__bf16, true>(from, count, rows, cols, steps, poly, eps, to, ws, p, device, s);
+      case FA_F16: return orthogonalize<f16, true>(from, count, rows, cols, steps, poly, eps, to, ws, p, device, s);
+      default: return orthogonalize<float, true>(from, count, rows, cols, steps, poly, eps, to, ws, p, device, s);
+    }
+  };
+  const int64_t each = static_cast<int64_t>(rows) * cols * (dtype == FA_F32 ? 4 : 2);
+  for (int64_t b0 = 0; b0 < batch; b0 += MOST_BATCH) {
+    const int count = static_cast<int>(batch - b0 < MOST_BATCH ? batch - b0 : MOST_BATCH);
+    if (const int e = some(static_cast<const char*>(g) + b0 * each, static_cast<char*>(out) + b0 * each, count))
+      return e;
   }
+  return FA_OK;
 }
 
 }  // extern "C"

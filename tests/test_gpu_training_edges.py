@@ -10,7 +10,7 @@ import torch
 
 import frame_analytics_amd as fa
 from oracle import training as ref
-from tests.test_gpu_training_ops import DT, UNIT, attention_case, near, normal, run_attention
+from tests.test_gpu_training_ops import DT, STEEP, UNIT, attention_case, near, normal, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -222,6 +222,16 @@ def test_token_strides_of_any_width(gpu, dt, lq):
 # --------------------------------------------------------------------------- #
 # updates
 # --------------------------------------------------------------------------- #
+
+
+def test_more_matrices_than_a_grid_holds(gpu):
+    n = 65535 + 70
+    gen = torch.Generator().manual_seed(3)
+    g = torch.randn(n, 3, 2, generator=gen)
+    got = fa.orthogonalize(g.cuda())
+    for i in (0, 1, 65533, 65534, 65535, 65536, n - 1):
+        near(got[i], ref.orthogonalize(g[i].double().numpy(), 5, STEEP), 3e-5, i)
+    assert torch.isfinite(got).all()
 
 
 #: outside what float16 operands hold: an iterate of 8 (its Gram entry), 1036, a polynomial

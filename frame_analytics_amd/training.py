@@ -22,6 +22,7 @@ from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import backend, backend_training
@@ -275,6 +276,13 @@ class _RelativeAttention(torch.autograd.Function):
         return (*(x if want else None for x, want in zip(grads, ctx.needs_input_grad)), None)
 
 
+def _tangents(*tensors: torch.Tensor) -> bool:
+    """Whether any carries a forward-mode tangent, which autograd then refuses (there is no
+    formula for it here): called past autograd, the kernels would drop it without a word."""
+    return (forward_ad._current_level >= 0
+            and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+
+
 class _Nothing(torch.autograd.Function):
     """No pairs: zeros, and zero gradients."""
 
@@ -402,8 +410,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
         positions, float(q.shape[3] ** -0.5 if scale is None else scale), bool(causal), mask,
         key_lengths, q_start)
     if _route(q, "relative_attention", backend_hint):
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                        or table.requires_grad):
+        if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                         or table.requires_grad)) or _tangents(q, k, v, table):
             return _RelativeAttention.apply(q, k, v, table, plan)
         return backend_training.rel_attention(q, k, v, table, plan, False)[0]
     return _portable_attention(q, k, v, table, plan)

@@ -219,6 +219,21 @@ def test_token_strides_of_any_width(gpu, dt, lq):
     assert all(torch.equal(x.grad, y.grad) for x, y in zip(ts, plain))
 
 
+def test_a_tangent_is_not_dropped(gpu):
+    import torch.autograd.forward_ad as fwd
+
+    pos = fa.LinePositions(8, 20)
+    q, k, v = (torch.randn(1, 2, 9, 8, device="cuda") for _ in range(3))
+    table = torch.randn(8, 2, device="cuda")
+    fa.relative_attention(q, k, v, table, pos)  # (a kernel ran in this test)
+    with fwd.dual_level():
+        dual = fwd.make_dual(q, torch.ones_like(q))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            fa.relative_attention(dual, k, v, table, pos)
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            fa.relative_bias(fwd.make_dual(table, torch.ones_like(table)), pos, 9)
+
+
 # --------------------------------------------------------------------------- #
 # updates
 # --------------------------------------------------------------------------- #

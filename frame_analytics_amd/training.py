@@ -86,12 +86,16 @@ class LinePositions:
         for name, value in (("num_buckets", int(num_buckets)), ("max_distance", int(max_distance)),
                             ("bidirectional", bool(bidirectional))):
             object.__setattr__(self, name, value)
-        starts = _bucket_starts(n, self.max_distance)
+        # about the logarithm of the last bucket's start: a search for the exact one would
+        # take as long as it is far
+        wide = n - n // 2
+        about = (math.log(n // 2) + (wide - 1) * math.log(self.max_distance)) / wide
+        starts = _bucket_starts(n, self.max_distance) if about < math.log(2 * _MOST_SLOTS) else ()
         object.__setattr__(self, "_starts", starts)
         object.__setattr__(self, "_far", starts[-1] if starts else n // 2)
-        if self.slots > _MOST_SLOTS:
-            raise ValueError(f"{self.slots} distances before the last bucket; at most "
-                             f"{_MOST_SLOTS} are supported")
+        if about >= math.log(2 * _MOST_SLOTS) or self.slots > _MOST_SLOTS:
+            raise ValueError(f"about {math.exp(min(about, 700)):.3g} distances each way before the "
+                             f"last bucket; at most {_MOST_SLOTS} in all are supported")
 
     @property
     def rows(self) -> int:

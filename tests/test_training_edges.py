@@ -93,3 +93,12 @@ def test_the_entry_point_refuses_what_float16_does_not_hold():
     for a, b, c, steps in ((2.0, 0.0, 0.0, 5), (3.0, 0.0, 1.0, 3), (0.5, 70.0, 0.0, 1),
                            (1.0, 0.0, 1.0, 3), (0.1, 0.0, 0.0, 5), (nan, 0.0, 0.0, 1), (1.0, nan, 0.0, 1)):
         assert lib.fa_gpu_orthogonalize(p, 3, 1, 8, 8, steps, a, b, c, 1e-7, p, p, 1 << 40, 0, None) == 5
+
+
+@pytest.mark.timeout(60)
+@pytest.mark.parametrize("args", [(32, 10 ** 18), (32, 10 ** 30), (16, 10 ** 400), (10 ** 7, 10 ** 8)])
+@pytest.mark.parametrize("both", [True, False])
+def test_distances_too_far_are_refused_at_once(args, both):
+    """Not after a search that counts up to them."""
+    with pytest.raises(ValueError, match="supported"):
+        fa.LinePositions(*args, bidirectional=both)

@@ -117,6 +117,11 @@ def rel_bias_backward(up, rows: int, positions, q_start: int) -> torch.Tensor:
 # --------------------------------------------------------------------------- #
 
 
+def _types(q: torch.Tensor, table: torch.Tensor) -> int:
+    """The dtype code of an attention; FA_TABLE_F32 where the table is wider than q."""
+    return _DTYPE_CODE[q.dtype] | (0x100 if table.dtype != q.dtype else 0)
+
+
 class AttentionPlan:
     """What a call's forward and backward pass hand to the library alike."""
 
@@ -156,7 +161,7 @@ def rel_attention(q, k, v, table, plan: AttentionPlan, need_lse: bool):
     dev, stream = _site(q)
     ws, n = _workspace("fa_gpu_rel_attention_workspace", q.device, b, h, hk, lq, lk, d,
                        plan.positions.slots, dev)
-    _run("fa_gpu_rel_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPE_CODE[q.dtype],
+    _run("fa_gpu_rel_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), _types(q, table),
          b, h, hk, lq, lk, d, _strides(q, k, v, out),
          *plan.tail(table, _row_of(plan.positions, q.device)), out.data_ptr(), _ptr(lse), _ptr(ws),
          n, dev, stream)
@@ -173,7 +178,7 @@ def rel_attention_backward(g, q, k, v, out, lse, table, plan: AttentionPlan, nee
     ws, n = _workspace("fa_gpu_rel_attention_backward_workspace", q.device, b, h, hk, lq, lk, d,
                        plan.positions.slots, plan.positions.grid_w, int(need_table), dev)
     _run("fa_gpu_rel_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-         g.data_ptr(), lse.data_ptr(), _DTYPE_CODE[q.dtype], b, h, hk, lq, lk, d,
+         g.data_ptr(), lse.data_ptr(), _types(q, table), b, h, hk, lq, lk, d,
          _strides(q, k, v, out, g, dq, dk, dv),
          *plan.tail(table, _row_of(plan.positions, q.device)), dq.data_ptr(), dk.data_ptr(),
          dv.data_ptr(), _ptr(dtable), _ptr(ws), n, dev, stream)

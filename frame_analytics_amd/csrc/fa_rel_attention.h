@@ -17,6 +17,7 @@ struct RelAttn {
   int B, H, Hk, Lq, Lk, D;
   int vec;  // elements per load that q, k, v (and the backward's views) allow
   const void* table;
+  int table_f32;  // the table is float32 whatever the type of q
   RelPos pos;
   int q0;               // position of query 0 where q_starts is null
   const int* q_starts;  // [B]
@@ -37,6 +38,13 @@ struct RelAttn {
     return mask ? mask + (b % mask_b) * mb + h * mh : nullptr;
   }
 };
+
+// go(table), once, with the table in its type: a test at each entry would hold up the reads
+// (24576 windows of 8 x 8 with gradients 633 us, and 644 so).
+template <typename T, typename Go> __device__ inline void with_table(const RelAttn& a, const Go& go) {
+  if (sizeof(T) == 2 && a.table_f32) go(static_cast<const float*>(a.table));
+  else go(static_cast<const T*>(a.table));
+}
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float INF = __builtin_inff();
@@ -61,24 +69,26 @@ constexpr float FAR_MOST = 4096.0f;
 // value depend on one another; four of each are under way at once.
 constexpr int PAD = 64;
 template <typename T>
-__device__ inline void load_bias(float* eb, const T* table, int H, int h, int heads, const RelPos& pos,
-                                 int tid, int nt) {
+__device__ inline void load_bias(float* eb, const RelAttn& a, int h, int heads, int tid, int nt) {
+  const RelPos& pos = a.pos;
   const int np = pos.n + 2 * PAD, total = heads * np;
-  for (int t0 = tid; t0 < total; t0 += 4 * nt) {
-    int row[4], head[4];
-    float v[4];
+  with_table<T>(a, [&](auto* table) {
+    for (int t0 = tid; t0 < total; t0 += 4 * nt) {
+      int row[4], head[4];
+      float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int t = min(t0 + e * nt, total - 1);
-      head[e] = heads == 1 ? 0 : t / np;
-      row[e] = pos.row_of[min(max(t - head[e] * np - PAD, 0), pos.n - 1)];
+      for (int e = 0; e < 4; ++e) {
+        const int t = min(t0 + e * nt, total - 1);
+        head[e] = heads == 1 ? 0 : t / np;
+        row[e] = pos.row_of[min(max(t - head[e] * np - PAD, 0), pos.n - 1)];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = widen(table[static_cast<int64_t>(row[e]) * a.H + h + head[e]]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (t0 + e * nt < total) eb[t0 + e * nt] = bias_log2(v[e]);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = widen(table[static_cast<int64_t>(row[e]) * H + h + head[e]]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (t0 + e * nt < total) eb[t0 + e * nt] = bias_log2(v[e]);
-  }
+  });
 }
 
 // Whether the biases past both ends of a head's table in LDS, np floats wide, are below
@@ -239,7 +249,7 @@ inline int check_strides(const int64_t* st, int count, int dtype) {
 
 inline RelAttn rel_attn_args(const void* q, const void* k, const void* v, int B, int H, int Hk,
                              int Lq, int Lk, int D, const int64_t* st, const void* table,
-                             const RelPos& pos, int64_t q_start, const int* q_starts,
+                             bool table_f32, const RelPos& pos, int64_t q_start, const int* q_starts,
                              const int* key_lengths, const uint8_t* mask, int mask_b,
                              const int64_t* ms, int causal, double scale) {
   RelAttn a{};
@@ -256,6 +266,7 @@ inline RelAttn rel_attn_args(const void* q, const void* k, const void* v, int B,
   a.Lk = Lk;
   a.D = D;
   a.table = table;
+  a.table_f32 = table_f32;
   a.pos = pos;
   a.q0 = clamp_pos(q_start);
   a.q_starts = q_starts;
@@ -291,6 +302,14 @@ template <typename K> inline int launch_lds(K kernel, size_t bytes) {
 template <typename T>
 void launch_table_sum(const float* partial, int parts, int n, const int* row_of, int rows, int H,
                       T* dtable, hipStream_t s);
+
+template <typename T>
+void launch_table_sum(const RelAttn& a, const float* partial, int parts, int rows, void* dtable, hipStream_t s) {
+  if (sizeof(T) == 2 && a.table_f32)
+    launch_table_sum<float>(partial, parts, a.pos.n, a.pos.row_of, rows, a.H, static_cast<float*>(dtable), s);
+  else
+    launch_table_sum<T>(partial, parts, a.pos.n, a.pos.row_of, rows, a.H, static_cast<T*>(dtable), s);
+}
 
 // fa_rel_attention_rows.hip: few queries against many keys
 int rows_workspace(int B, int H, int Hk, int Lq, int Lk, int D, int device, int64_t* bytes);

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(NW * 64 * KG) void rel_attention_kernel(RelAttn a, 
   const float c = a.scale * LOG2E;
 
   int* codes = reinterpret_cast<int*>(eb + (a.pos.n + 2 * PAD + 3) / 4 * 4);  // of a window's keys
-  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, threadIdx.x, NT * KG);
+  load_bias<T>(eb, a, h, 1, threadIdx.x, NT * KG);
   if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, threadIdx.x, NT * KG);
 
   typename M::V8 qf[CH];
@@ -319,12 +319,14 @@ FA_API int fa_gpu_rel_attention(const void* q, const void* k, const void* v, int
                                 void* stream) {
   using namespace fa;
   if (!q || !k || !v || !strides || !table || !out) return FA_E_ARG;
+  const bool table_f32 = dtype & FA_TABLE_F32;
+  dtype &= ~FA_TABLE_F32;
   if (const int e = check_attention(B, H, Hk, Lq, Lk, D, mask, mask_b, mask_strides)) return e;
   if (const int e = check_relpos(row_of, rows, lo, n, grid_w, Lq, Lk, q_start, q_starts)) return e;
   if (const int e = check_strides(strides, 4, dtype)) return e;
   DeviceScope scope(device);
   if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
-  const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table,
+  const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table, table_f32,
                                   RelPos{row_of, lo, n, grid_w}, q_start, q_starts, key_lengths,
                                   mask, mask_b, mask_strides, causal, scale);
   const View os{strides[9], strides[10], strides[11]};

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 && DP <= 64 && KEYS / 
   const int q = qw + col, qc = min(q, a.Lq - 1);
   const float c = a.scale * LOG2E;
 
-  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, threadIdx.x, NT * KG);
+  load_bias<T>(eb, a, h, 1, threadIdx.x, NT * KG);
   if (a.pos.grid_w) load_codes(codes, a.pos, a.Lk, threadIdx.x, NT * KG);
   constexpr int TOTALS = KEYS > 0 ? KEYS / KG : 1;
   f32x16 total[TOTALS];
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 ? (DP == 32 ? 3 : DP =
       }
     };
     __syncthreads();  // the head before is done with its tiles and bias
-    load_bias<T>(eb, static_cast<const T*>(a.table), a.H, h, 1, a.pos, threadIdx.x, NT * KG);
+    load_bias<T>(eb, a, h, 1, threadIdx.x, NT * KG);
     if (t0 + kg < tiles) {
       load(t0 + kg);
       store(t0 + kg);
@@ -788,8 +788,7 @@ int backward(RelAttn a, Grads g, int rows, void* dtable, const Plan& p, hipStrea
   else e = launch_dim<T, 128>(a, g, p, s);
   if (e) return e;
   if (dtable) {
-    launch_table_sum<T>(g.parts, p.chunks * tiles_of(a.Lq, p.nw_q), a.pos.n, a.pos.row_of, rows, a.H,
-                        static_cast<T*>(dtable), s);
+    launch_table_sum<T>(a, g.parts, p.chunks * tiles_of(a.Lq, p.nw_q), rows, dtable, s);
     FA_LAUNCH_CHECK();
   }
   return FA_OK;
@@ -841,6 +840,8 @@ FA_API int fa_gpu_rel_attention_backward(
   if (!q || !k || !v || !out || !dout || !lse || !strides || !table || !dq || !dk || !dv ||
       !workspace)
     return FA_E_ARG;
+  const bool table_f32 = dtype & FA_TABLE_F32;
+  dtype &= ~FA_TABLE_F32;
   if (const int e = check_attention(B, H, Hk, Lq, Lk, D, mask, mask_b, mask_strides)) return e;
   if (const int e = check_relpos(row_of, rows, lo, n, grid_w, Lq, Lk, q_start, q_starts)) return e;
   if (const int e = check_strides(strides, 8, dtype)) return e;
@@ -848,7 +849,7 @@ FA_API int fa_gpu_rel_attention_backward(
   if (workspace_bytes < room.bytes) return FA_E_ARG;
   DeviceScope scope(device);
   if (scope.status != hipSuccess) return -static_cast<int>(scope.status);
-  const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table,
+  const RelAttn a = rel_attn_args(q, k, v, B, H, Hk, Lq, Lk, D, strides, table, table_f32,
                                   RelPos{row_of, lo, n, grid_w}, q_start, q_starts, key_lengths,
                                   mask, mask_b, mask_strides, causal, scale);
   Grads g{};

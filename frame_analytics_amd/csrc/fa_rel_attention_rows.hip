@@ -186,7 +186,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(RelAttn a, T* out, View os,
       else qf[n][i] = qr.single(at, d, a.D, on);
     }
   }
-  load_bias<T>(eb, static_cast<const T*>(a.table), a.H, hk * group, group, a.pos, tid, NT);
+  load_bias<T>(eb, a, hk * group, group, tid, NT);
 
   f32x4 o[NC][OB];
   float m[NC], l[NC];

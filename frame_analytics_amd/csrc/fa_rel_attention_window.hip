@@ -129,15 +129,16 @@ __device__ inline void store_rows(T* own, const f32x16 (&acc)[DP / 32], float f,
 
 template <typename T>
 __device__ inline void load_pair_bias(float (&bias)[2][16], const RelAttn& a, const Pairs& p, int h) {
-  const T* table = static_cast<const T*>(a.table);
   const int cq = a.pos.code(p.qc);
+  with_table<T>(a, [&](auto* table) {
 #pragma unroll
-  for (int nb = 0; nb < 2; ++nb)
+    for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = a.pos.row_of[a.pos.slot(cq - a.pos.code(min(p.key(nb, r), a.Lk - 1)))];
-      bias[nb][r] = bias_log2(widen(table[static_cast<int64_t>(row) * a.H + h]));
-    }
+      for (int r = 0; r < 16; ++r) {
+        const int row = a.pos.row_of[a.pos.slot(cq - a.pos.code(min(p.key(nb, r), a.Lk - 1)))];
+        bias[nb][r] = bias_log2(widen(table[static_cast<int64_t>(row) * a.H + h]));
+      }
+  });
 }
 
 // Scores of the wave's queries, hidden ones -inf; their maximum (0 where there is none).
@@ -525,7 +526,7 @@ int backward(RelAttn a, const WindowGrads& g, int rows, void* dtable, int device
   const int e = with_access<T>(a.vec, go);
   if (e) return e;
   if (dtable) {
-    launch_table_sum<T>(g.parts, chunks, a.pos.n, a.pos.row_of, rows, a.H, static_cast<T*>(dtable), s);
+    launch_table_sum<T>(a, g.parts, chunks, rows, dtable, s);
     FA_LAUNCH_CHECK();
   }
   return FA_OK;

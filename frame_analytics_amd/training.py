@@ -388,7 +388,8 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     dim)`` with the key heads dividing the heads (each is shared by neighbouring query
     heads); any strides, the last dimension contiguous (else copied, as is a view of which
     256 tokens span 2 GiB); ``dim`` up to 128.  The result is laid out as q is (as its copy
-    where it was copied).  A table of another type is rounded to q's first.
+    where it was copied).  A table of another type than q counts in float32, as
+    does its gradient (a float32 parameter beside 16-bit activations loses nothing).
 
     ``scale`` defaults to ``dim ** -0.5``.  A pair counts where all of these allow it:
     ``causal`` (the key's position is not after the query's), ``key_lengths`` ((batch,)
@@ -402,12 +403,12 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     ``q_start=key_lengths - 1``.
 
     The scores, the softmax and all sums are float32; its weights are rounded to q's
-    type for the product with v, and results once.  Results and gradients are the same
-    bits from run to run.
+    type for the product with v, the weights and the scores' gradient for the gradients'
+    products, and results once.  Results and gradients are the same bits from run to run.
     """
     mask = _check_attention(q, k, v, table, positions, mask, key_lengths, q_start)
     if table.dtype != q.dtype:
-        table = table.to(q.dtype)
+        table = table.to(torch.float64 if q.dtype == torch.float64 else torch.float32)
     if q.numel() == 0 or k.shape[2] == 0:
         return _Nothing.apply(q, k, v, table)
     plan = backend_training.AttentionPlan(

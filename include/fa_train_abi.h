@@ -25,6 +25,9 @@ extern "C" {
  * standing next to one another.  1 <= n <= FA_REL_MAX. */
 #define FA_REL_MAX 4225
 
+/* OR-ed into an attention's dtype: table and dtable are float32, whatever q is. */
+#define FA_TABLE_F32 0x100
+
 /*
  * out[h, i, j] = table[row(i, j), h], i < Lq, j < Lk, query i standing at position
  * q_start + i of a line (0 in a window).  table: [rows, H] contiguous, out: [H, Lq,

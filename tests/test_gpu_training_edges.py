@@ -291,3 +291,45 @@ def test_coefficients_that_just_fit(gpu, dt, coefficients, steps, m, n):
     # value's rounding is half a unit in the last place at most
     near(fa.orthogonalize(g.cuda(), steps=steps, coefficients=coefficients, backend_hint="native"),
          want, {"bf16": 1.5e-3 + 2.0 ** -8, "f16": 2.0 ** -11 + 3e-5, "f32": 3e-5}[dt], (m, n))
+
+
+# --------------------------------------------------------------------------- #
+# a float32 table beside 16-bit activations
+# --------------------------------------------------------------------------- #
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("form", ["line", "few", "one", "window", "wide window"])
+def test_a_float32_table_keeps_its_digits(gpu, dt, form):
+    """Entries of some size, whose rounding to 16 bits would show in the weights; and a
+    gradient that is not rounded to them."""
+    gen = torch.Generator().manual_seed(31)
+    b, h, d, start = 2, 2, 32, 0
+    if form == "window":
+        pos, lq = fa.GridPositions(8, 8), 64
+        lk, rows = lq, ref.grid_rows(8, 8)
+    elif form == "wide window":
+        pos, lq = fa.GridPositions(9, 10), 90
+        lk, rows = lq, ref.grid_rows(9, 10)
+    else:
+        pos = fa.LinePositions(8, 20)
+        lq, lk = {"line": (150, 160), "few": (5, 700), "one": (1, 90)}[form]
+        start = lk // 2 if form != "line" else 0
+        rows = ref.line_rows(lq, lk, start, 8, 20)
+    q, k, v, g = (normal(gen, DT[dt], b, h, n, d) for n in (lq, lk, lk, lq))
+    # what they have in common cancels in a row; rounded with it to the type they are off by
+    # up to 16 of its units (of one), a weight's error
+    table = 20.0 + 0.7 * torch.randn(pos.rows, h, generator=gen)
+    see = ref.visible(b, h, lq, lk)
+    want = ref.attention(*(t.double().numpy() for t in (q, k, v, table)), rows, see, d ** -0.5,
+                         g.double().numpy())
+    got = run_attention((q, k, v, table), g, pos, q_start=start)
+    assert got[4].dtype == torch.float32
+    for name, x, y, t in zip(("out", "dq", "dk", "dv", "dtable"), got, want, (2, 4, 4, 4, 4)):
+        near(x, y, t * UNIT[dt] / 2, name)
+    assert not torch.equal(got[4], got[4].to(DT[dt]).float())
+    with torch.no_grad():
+        only = fa.relative_attention(*(t.cuda() for t in (q, k, v, table)), pos, q_start=start)
+        same = fa.relative_attention(*(t.cuda() for t in (q, k, v, table.double())), pos, q_start=start)
+    near(only, want[0], UNIT[dt], "out, no gradients")
+    assert torch.equal(only, same)

@@ -12,6 +12,7 @@ import torch
 
 import frame_analytics_amd as fa
 from frame_analytics_amd import _build, _cabi, backend_training, training
+from oracle import training as ref
 
 
 def test_row_tables_are_never_given_back():
@@ -102,3 +103,20 @@ def test_distances_too_far_are_refused_at_once(args, both):
     """Not after a search that counts up to them."""
     with pytest.raises(ValueError, match="supported"):
         fa.LinePositions(*args, bidirectional=both)
+
+
+def test_a_float32_table_keeps_its_digits():
+    """Beside 16-bit activations, on the eager path; its gradient too."""
+    gen = torch.Generator().manual_seed(3)
+    pos, d = fa.LinePositions(8, 20), 8
+    q, k, v = (torch.randn(1, 2, 12, d, generator=gen).bfloat16() for _ in range(3))
+    table = (20 + torch.randn(8, 2, generator=gen)).requires_grad_(True)
+    up = torch.randn(1, 2, 12, d, generator=gen).bfloat16()
+    out = fa.relative_attention(q, k, v, table, pos)
+    out.backward(up)
+    want = ref.attention(*(t.detach().double().numpy() for t in (q, k, v, table)),
+                         ref.line_rows(12, 12, 0, 8, 20), ref.visible(1, 2, 12, 12), d ** -0.5,
+                         up.double().numpy())
+    assert table.grad.dtype == torch.float32
+    for x, y, tol in ((out, want[0], 2.0 ** -8), (table.grad, want[4], 1e-5)):
+        assert np.linalg.norm(x.detach().double().numpy() - y) <= tol * np.linalg.norm(y)

@@ -163,7 +163,8 @@ def test_lines_of_many_workgroups(gpu, dt, b, h, hk, n, d, causal):
     (12, 500, 1400),   # tiles of 128 in the last, of 64 in the symmetric ones
     (30, 250, 230),    # tiles of 64, one group of waves in every product
     (20, 130, 640),    # one group in the last, four in the symmetric ones
-    (600, 70, 65)])
+    (600, 70, 65),
+    (600, 40, 130)])  # of up to 64 rows: tiles of 64 however many
 def test_updates_of_many_tiles(gpu, dt, batch, m, n):
     gen = torch.Generator().manual_seed(m)
     g = (1e-3 * torch.randn(batch, m, n, generator=gen)).to(DT[dt])

@@ -120,3 +120,16 @@ def test_a_float32_table_keeps_its_digits():
     assert table.grad.dtype == torch.float32
     for x, y, tol in ((out, want[0], 2.0 ** -8), (table.grad, want[4], 1e-5)):
         assert np.linalg.norm(x.detach().double().numpy() - y) <= tol * np.linalg.norm(y)
+
+
+def test_stacks_of_small_matrices_are_not_padded_to_wide_tiles():
+    """Whatever their number, matrices of up to 64 rows take tiles of 64: each operand
+    (three of X, two of the square ones, hi and lo) is 64 x 64 of float16, beside the norm's
+    sums."""
+    if not _build.library_path().exists():
+        _build.build()
+    lib = _cabi.bind(ctypes.CDLL(str(_build.library_path())), _cabi.TRAIN_SIGNATURES)
+    out = ctypes.c_int64(0)
+    for batch, rows, cols in ((1, 16, 27), (4096, 16, 27), (600, 64, 64), (65535, 3, 2)):
+        assert lib.fa_gpu_orthogonalize_workspace(3, batch, rows, cols, ctypes.byref(out)) == 0
+        assert out.value <= batch * (5 * 2 * 64 * 64 * 2 + 512 * 8 + 4) + 8 * 256

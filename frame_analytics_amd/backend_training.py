@@ -1,9 +1,9 @@
 """Dispatch of the training operators to the gfx950 kernels: tensors in, raw
 pointers across ``include/fa_train_abi.h``.
 
-Every buffer -- outputs, log-sums, workspaces -- is allocated here through torch's
-caching allocator on the caller's current stream, and every launch goes to that
-stream, as in :mod:`frame_analytics_amd.backend`.  A kernel that refuses a call
+Every buffer -- outputs, what the backward pass reads, workspaces -- is allocated here
+through torch's caching allocator on the caller's current stream, and every launch goes
+to that stream, as in :mod:`frame_analytics_amd.backend`.  A kernel that refuses a call
 raises :class:`~frame_analytics_amd.backend.KernelError`.
 """
 
@@ -147,7 +147,7 @@ class AttentionPlan:
 
 
 def rel_attention(q, k, v, table, plan: AttentionPlan, need_lse: bool):
-    """``(out, lse, what the backward pass is given)``."""
+    """``(out, what is kept of the rows' softmax, the tensors as the kernels read them)``."""
     q, k, v, table = _unit(q), _unit(k), _unit(v), table.contiguous()
     b, h, lq, d = q.shape
     hk, lk = k.shape[1], k.shape[2]

@@ -209,7 +209,7 @@ __global__ __launch_bounds__(NT * KG) void ortho_product_kernel(Bufs w, Step st,
     ap[s] = A[s] + abase + static_cast<int64_t>(ti) * TM * K;
     bp[s] = B[s] + bbase + static_cast<int64_t>(tj) * TM * K;
   }
-  // 128-wide tiles have two pieces of k on their way at a time (2 x 4096^2 4.44 -> 4.32 ms);
+  // 128-wide tiles have two pieces of k on their way at a time (2 x 4096^2 4.44 -> 4.42 ms);
   // 64-wide ones, more of which share a compute unit, one (two: 139 -> 153 us, 6 x 180^2)
   constexpr bool TWO = TM == 128;
   TileLoad<f16, BK, TM, NT, true> al[2][PARTS], bl[2][PARTS];

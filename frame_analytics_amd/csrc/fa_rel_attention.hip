@@ -261,9 +261,10 @@ int launch_one(const RelAttn& a, T* out, const View& os, int ovec, float* lse, h
 
 template <typename T, int DP, bool WIDE>
 int launch_wide(const RelAttn& a, T* out, const View& os, int ovec, float* lse, int device, hipStream_t s) {
-  // two waves to a workgroup where four leave compute units without one (256 workgroups of
-  // four took 86 us where 512 of two took 101, a causal line of 2048), and a second group
-  // of waves where there are less than two workgroups for every compute unit
+  // two waves to a workgroup where four leave compute units without one (a causal line of
+  // 2048 in bfloat16: 256 workgroups of four 43 us, 512 of two 65; a line of 777 in float32:
+  // 112 of four 70, 208 of two 49), and a second group of waves where there are less than two
+  // workgroups for every compute unit
   const int cus = cu_count(device);
   const int64_t four = static_cast<int64_t>(a.B) * a.H * ((a.Lq + 127) / 128);
   const bool few = a.Lq <= 64 || four < cus;

@@ -392,7 +392,7 @@ __global__ __launch_bounds__(NW * 64 * KG, sizeof(T) == 2 ? (DP == 32 ? 3 : DP =
   T* gt = qt + BUFS * BM * TL::LD;
   float* eb = reinterpret_cast<float*>(reinterpret_cast<T*>(smem) + KG * 2 * BUFS * BM * TL::LD);
   const int np = a.pos.n + 2 * PAD;
-  float* ls = eb + (np + 3) / 4 * 4 + kg * 4 * BM;  // [2][BM]: each query's log-sum
+  float* ls = eb + (np + 3) / 4 * 4 + kg * 4 * BM;  // [2][BM]: each query's shift
   float* dd = ls + 2 * BM;                          // [2][BM]: and D_i
   int* codes = reinterpret_cast<int*>(eb + (np + 3) / 4 * 4 + KG * 4 * BM);  // of a window's queries
   const int tid = threadIdx.x - kg * NT, lane = tid & 63, hh = lane >> 5, col = lane & 31;
@@ -667,9 +667,9 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(RelAttn a, Grads g, int s
 inline int tiles_of(int n, int nw) { return (n + nw * 32 - 1) / (nw * 32); }
 
 // How a call is laid out over the card.  Four waves to a workgroup, two where four leave
-// compute units without one (a causal line of 2048, 256 workgroups of four: dQ 91 us
-// against 105 of two, dK and dV 80 against 106; 112 and 28 of four, odd 777: 142 and 608
-// against 119 and, the shared heads split, 137).
+// compute units without one (a causal line of 2048 in bfloat16, 256 workgroups of four: dQ
+// 75 us against 103 of two, dK and dV 56 against 116; a line of 777 in float32, 112 and 28
+// of four: dQ 132 against 83, dK and dV, the shared heads split, 137 against 84).
 struct Plan {
   int nw_q, nw_k;  // waves of the workgroups that own queries, and keys
   int kg_q, kg_k;  // groups of them

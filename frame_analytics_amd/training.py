@@ -259,8 +259,8 @@ def relative_bias(table: torch.Tensor, positions: Positions, q_len: int,
 
 
 class _RelativeAttention(torch.autograd.Function):
-    """Keeps q, k, v, the output and each row's log-sum; the backward pass forms the
-    weights again from them."""
+    """Keeps q, k, v, the output and two numbers of each row's softmax; the backward pass
+    forms the weights again from them."""
 
     @staticmethod
     def forward(ctx, q, k, v, table, plan):
